@@ -404,6 +404,36 @@ void* svae_plan_create(const int* items, const long long* user_off, const long l
 int svae_plan_pack(void* plan, void* dst, long long dst_bytes, long long* order, long long* lengths, int* row_off);
 void svae_plan_destroy(void* plan);
 
+/* ---- embedding lookup of any width and type, gradient by sorted tokens -------------------------------------
+ * No counterpart in the reference (its nn.Embedding is svae_embed_fwd / svae_embed_bwd: width 256, fp32, rows sorted by the
+ * host's plan).  Types: 0 fp32, 1 bf16, 2 fp16; tokens: int32, or int64 with tok64 != 0; ld: elements from one row to the
+ * next (>= D).  A token outside [0, V) marks a padded place.  R == 0 is allowed, pointers may then be NULL.
+ *   svae_lookup_fwd       out[r][0..D) = scale * table[tokens[r]][0..D), a zero row for a padded place
+ *   svae_token_sort       stable sort of the places by token: keys [R] ascending (padded places and the token `pad` as V,
+ *                         at the end; pad < 0: none), perm [R] the places; work: svae_token_sort_bytes(R, V, &bytes)
+ *   svae_lookup_bwd       grad[v][0..D) = scale * sum of dy[perm[i]] over the places i with keys[i] == v, in their order; rows
+ *                         without a place are written as zeros.  accumulate != 0: the sums are added to grad, other rows are
+ *                         left as they are.  work: svae_lookup_bwd_bytes(R, D, &bytes)
+ * Sums are fp32, rounded once to grad's type; no atomics on them: the same bits in every run. */
+int svae_lookup_fwd(const void* table, int table_type, long long ld_table, const void* tokens, int tok64, void* out,
+                    int out_type, long long ld_out, int R, int V, int D, float scale, void* stream);
+int svae_token_sort_bytes(int R, int V, long long* bytes);
+int svae_token_sort(const void* tokens, int tok64, int R, int V, int pad, int* keys, int* perm, void* work,
+                    long long work_bytes, void* stream);
+int svae_lookup_bwd_bytes(int R, int D, long long* bytes);
+int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* keys, const int* perm, int R, int V, int D,
+                    float scale, void* grad, int grad_type, long long ld_grad, int accumulate, void* work,
+                    long long work_bytes, void* stream);
+
+/* ---- dropout from a counter-based generator ------------------------------------------------------------------
+ * No counterpart in the reference.  y[r][c] = x[r][c] * 65536 / (65536 - k) where the 16 random bits of (r, c) are at least
+ * k = round(65536 p), else 0; the bits come from Philox4x32-10 with key seed and counter (row_key[r], c / 8 + 2^31, step), as
+ * csrc/dropout.hip says: replayable, never stored, independent of strides and of how rows are dealt to GPUs.  row_key [R] may
+ * be NULL (the row's index); step_dev != NULL: the step is read there on the device (low 32 bits), so that replays of a
+ * captured graph can draw new masks.  y may be x.  type: 0 fp32, 1 bf16, 2 fp16.  The gradient is the same call on dy. */
+int svae_dropout(const void* x, long long ldx, void* y, long long ldy, int type, int R, int C, double p,
+                 unsigned long long seed, unsigned step, const long long* step_dev, const long long* row_key, void* stream);
+
 /* ---- helpers -------------------------------------------------------------------------------------------- */
 int svae_colsum(const float* a, float* out, float* partials, int R, int N, int ld, int nparts, void* stream);
 int svae_transpose(const float* in, float* out, int rows, int cols, void* stream);

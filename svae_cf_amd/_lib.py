@@ -92,6 +92,13 @@ SIGNATURES = {
     "svae_rowgemm_ld": [_P, _I, _P, _P, _P, _I, _I, _P],
     "svae_wgrad_cols": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _I, _I, _P],
     "svae_zero": [_P, _LL, _P],
+    # operators of any width and type (ops.py)
+    "svae_lookup_fwd": [_P, _I, _LL, _P, _I, _P, _I, _LL, _I, _I, _I, _F, _P],
+    "svae_token_sort_bytes": [_I, _I, _P],
+    "svae_token_sort": [_P, _I, _I, _I, _I, _P, _P, _P, _LL, _P],
+    "svae_lookup_bwd_bytes": [_I, _I, _P],
+    "svae_lookup_bwd": [_P, _I, _LL, _P, _P, _I, _I, _I, _F, _P, _I, _LL, _I, _P, _LL, _P],
+    "svae_dropout": [_P, _LL, _P, _LL, _I, _I, _I, _c.c_double, _ULL, _U, _P, _P, _P],
     # split instantiations (prec 2) of the fused kernels
     "svae_wgrad_cols_prec": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _I, _I, _I, _P],
     "svae_rowgemm_prep_prec": [_P, _I, _P, _I, _P],

@@ -4,6 +4,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "philox.h"
 
 namespace {
 
@@ -883,19 +884,6 @@ __global__ __launch_bounds__(1024) void masked_topk_kernel(const float* __restri
 // Philox4x32-10 + Box-Muller N(0,1), keyed by (seed) and counter (row_key[r], col/4, step):
 // replayable and independent of how users are sharded over GPUs.
 // ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void philox4x32_10(uint32_t c[4], uint32_t k0, uint32_t k1) {
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint64_t p0 = (uint64_t)0xD2511F53u * c[0];
-        const uint64_t p1 = (uint64_t)0xCD9E8D57u * c[2];
-        const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c[1] ^ k0;
-        const uint32_t n1 = (uint32_t)p1;
-        const uint32_t n2 = (uint32_t)(p0 >> 32) ^ c[3] ^ k1;
-        const uint32_t n3 = (uint32_t)p0;
-        c[0] = n0; c[1] = n1; c[2] = n2; c[3] = n3;
-        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-    }
-}
 __global__ void philox_normal_kernel(float* __restrict__ out, const long long* __restrict__ row_key, int R,
                                      unsigned long long seed, unsigned step) {
     // thread -> (row, group of 4 columns); 16 groups per row
