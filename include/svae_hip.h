@@ -425,6 +425,30 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
                     float scale, void* grad, int grad_type, long long ld_grad, int accumulate, void* work,
                     long long work_bytes, void* stream);
 
+/* ---- softmax cross entropy behind a linear layer over a large vocabulary --------------------------------------
+ * No counterpart in the reference (its loss over the catalogue is svae_proj_nll_*: width 150, next-k targets).
+ * z = hidden weight^T + bias, [R][V], never kept.  hidden [R][D], weight [V][D] (rows ld elements apart), bias [V] or NULL, all
+ * of one type (0 fp32, 1 bf16, 2 fp16); targets [R] int32, or int64 with tok64 != 0.  A row whose target is outside [0, V) is
+ * left out: nll = lse = 0, no gradient, whatever the row holds.  Products of bf16 / fp16 run on the matrix units as they are,
+ * fp32 ones as six products of bf16 parts (24 bits); sums, statistics and losses are fp32.
+ *   svae_xent_fwd     lse[r] = log sum_v exp z[r][v], nll[r] = lse[r] - z[r][target] (fp32)
+ *   svae_xent_reduce  out[0] = the sum of nll or (mean != 0) its mean over the rows with a target (0 over none), out[1] = the
+ *                     weight of a row in it
+ *   svae_xent_bwd     gradients of sum_r row_weight[r] nll[r], given fwd's lse: dh [R][D], dw [V][D], db [V] in the inputs'
+ *                     type; dh or dw may be NULL (db comes with dw).  Made in pieces of the vocabulary, sized by the workspace.
+ *                     A row of weight 0 takes no part, whatever it holds.
+ * Workspace (aligned to 256 bytes): svae_xent_bytes(weight, ld_w, type, R, V, D, grad, &bytes), grad != 0 for svae_xent_bwd; the
+ * size depends on whether weight's rows can be loaded as they stand (16-bit types, address and row length multiples of 16 bytes). */
+int svae_xent_bytes(const void* weight, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes);
+int svae_xent_fwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                  const void* targets, int tok64, int type, int R, int V, int D, float* nll, float* lse, void* work,
+                  long long work_bytes, void* stream);
+int svae_xent_reduce(const float* nll, const void* targets, int tok64, int R, int V, int mean, float* out, void* stream);
+int svae_xent_bwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                  const void* targets, int tok64, int type, int R, int V, int D, const float* lse, const float* row_weight,
+                  void* dh, long long ld_dh, void* dw, long long ld_dw, void* db, void* work, long long work_bytes,
+                  void* stream);
+
 /* ---- dropout from a counter-based generator ------------------------------------------------------------------
  * No counterpart in the reference.  y[r][c] = x[r][c] * 65536 / (65536 - k) where the 16 random bits of (r, c) are at least
  * k = round(65536 p), else 0; the bits come from Philox4x32-10 with key seed and counter (row_key[r], c / 8 + 2^31, step), as

@@ -1,0 +1,900 @@
+// Softmax cross entropy behind a linear layer over a large vocabulary, in pieces of the vocabulary, without keeping the logits.
+//
+//   z = H W^T + b      lse_r = log sum_v exp z_rv      nll_r = lse_r - z[r][t_r]          (t_r outside [0, V): row left out)
+//   G_rv = w_r (exp(z_rv - lse_r) - [v = t_r])         dH = G W      dW = G^T H      db_v = sum_r G_rv
+//
+// Loss: one product over all tiles of z; each tile leaves the maximum and the sum of exponentials of its 256 columns per row and
+// the target's logit.  Gradient: for one piece of the vocabulary after the other, the tiles of z are made again and G of the
+// piece is written to the workspace, then two products take it up.  Everything is bound by the matrix units (6 R V D flops for
+// loss and gradient and 2 R V D for making z again), except that few rows leave the loss bound by reading W.
+//
+// All products run on one core: 256 x 256 (or 256 x 64) outputs a workgroup, 8 waves, steps of 64 along the contraction, two
+// stages of LDS filled by LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from
+// writes to the other and does not wait for the prefetch), v_mfma_f32_16x16x32.
+//   z^T tile: A = W rows, B = H rows, both with the contraction contiguous.  C has the row of H in the lane and four vocabulary
+//     entries in registers, so a row's maximum and sum are mostly in-lane work.
+//   G is kept as blocks of 16 rows x 32 vocabulary entries, 1 KiB: a lane's 16 bytes are the 8 values that it made, which are a
+//     B fragment of G W as they stand if W's rows are taken in the same order (16 (j / 4) + 4 (lane / 16) + j % 4), and that is
+//     the order in which transposing LDS reads deliver W.  For G^T H the same blocks are read with transposing LDS reads.
+//
+// Types: bf16 and fp16 go to the matrix units as they are; G is rounded to the inputs' type (relative 2^-8 / 2^-11 of each
+// term, as the inputs themselves are), for fp16 after scaling by a power of two that puts the largest row weight near 2^14, so
+// that small probabilities stay above fp16's subnormals.  fp32 is carried as three bf16 parts (24 bits) and every product by
+// its six leading terms.
+#include "elem.h"
+
+namespace {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+constexpr int BM = 256;                   // outputs of a workgroup along A
+constexpr int BK = 64;                    // contraction of a step
+constexpr unsigned BUF_FLAGS = 0x00020000u;
+constexpr unsigned NOWHERE = 0xFFFFFFF0u; // past every buffer's end: such a lane loads zeros
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename E>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mfma<__bf16>(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mfma<_Float16>(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, long long bytes) {
+    const long long n = bytes < 0 ? 0 : bytes > 0xFFFFFF00ll ? 0xFFFFFF00ll : bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (unsigned)n, BUF_FLAGS);
+}
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, char* lds, unsigned off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ s16x4 tr16(const char* p) {
+    return __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+__device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// the six leading products of two numbers in three parts each, smallest first: part of A, part of B
+__device__ __forceinline__ int part_a(int s) { return (0x001102 >> (4 * s)) & 15; }
+__device__ __forceinline__ int part_b(int s) { return (0x010120 >> (4 * s)) & 15; }
+
+// ------------------------------------------------------------------------------------------------
+// The core: acc[t][n] (16 x 16 each; A side t, B side n) += A B over `steps` steps of 64.
+//   AKIND 0: A [m][k], k contiguous (rows lda bytes apart)      LDS image [256 m][64 k]
+//   AKIND 1: A [k][m], m contiguous                             LDS image [64 k][256 m], read transposed
+//   BKIND 0: B [n][k] like A      BKIND 1: blocks of G, contraction over the vocabulary      BKIND 2: over the rows
+// LDS images hold 16-byte chunks; which chunk a lane fetches is permuted so that the 16 lanes that a read serves at a time
+// fall on different banks: [.][64] images: chunk c of row r at c ^ ((r / 2) % 8); [.][256]: pairs of chunks, c ^ 2 (r % 8).
+// PARTS 3: the step runs over the six pairs of parts; the parts of an operand lie apart by a_part / b_part bytes.
+// ------------------------------------------------------------------------------------------------
+struct Operand {
+    const char* p;        // first row (contraction step 0) of the tile
+    long long left;       // bytes from p to the end of what may be read
+    long long step;       // bytes from one step to the next
+    long long part;       // bytes from one part to the next
+    unsigned ld;          // bytes between rows (BKIND 1, 2: between blocks of 16 rows)
+    int kmax;             // AKIND / BKIND 0: length of a row in elements; chunks behind it are loaded as zeros
+};
+
+template <int BN>
+struct Lay {
+    static constexpr int WN = BN / 64;                  // waves along B, 64 outputs each
+    static constexpr int WM = 8 / WN;                   // waves along A
+    static constexpr int MT = BM / WM / 16;             // 16-wide tiles of a wave along A
+    static constexpr int NB = BN / 64;                  // LDS-DMA instructions of a wave for B and step (4 for A)
+};
+
+// lane offsets of the LDS-DMA instructions (global side)
+template <int KIND>
+__device__ __forceinline__ unsigned dma_off(int inst, int lane, unsigned ld) {
+    if (KIND == 0) {
+        const int row = inst * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+        return (unsigned)row * ld + (unsigned)c * 16u;
+    } else if (KIND == 1) {                              // [64 k][256 m]
+        const int row = inst * 2 + (lane >> 5), c = (lane & 31) ^ ((row & 7) << 1);
+        return (unsigned)row * ld + (unsigned)c * 16u;
+    }
+    return 0;
+}
+
+template <typename E, int BN, int AKIND, int BKIND, int PARTS, bool COLSUM>
+__device__ __forceinline__ void core(const Operand& A, const Operand& B, int steps, char* a0, char* a1, char* b0, char* b1,
+                                     f32x4 (&acc)[Lay<BN>::MT][4], f32x4 (&cs)[4]) {
+    typedef Lay<BN> L;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
+    const int i16 = lane & 15, q = lane >> 4;
+
+    unsigned oa[4], ob[L::NB];
+    int ca[4], cb[L::NB];                                // first element of the chunk inside the step (kind 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        oa[j] = dma_off<AKIND>(wave * 4 + j, lane, A.ld);
+        ca[j] = (int)((oa[j] - (unsigned)((wave * 4 + j) * 8 + (lane >> 3)) * A.ld) >> 1);
+    }
+#pragma unroll
+    for (int j = 0; j < L::NB; ++j) {
+        const int b = wave * L::NB + j;
+        if (BKIND == 0) {
+            ob[j] = dma_off<0>(b, lane, B.ld);
+            cb[j] = (int)((ob[j] - (unsigned)(b * 8 + (lane >> 3)) * B.ld) >> 1);
+        } else if (BKIND == 1) ob[j] = (unsigned)(b >> 1) * B.ld + (unsigned)(b & 1) * 1024u + (unsigned)lane * 16u;
+        else ob[j] = (unsigned)(b / (BN / 32)) * B.ld + (unsigned)(b % (BN / 32)) * 1024u + (unsigned)lane * 16u;
+    }
+    // fragment offsets inside a stage
+    unsigned fa[2], ft[L::MT], fb[2];
+    if (AKIND == 0) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) fa[kk] = (unsigned)(wm + i16) * 128u + (unsigned)((kk * 4 + q) ^ (i16 >> 1)) * 16u;
+    } else {
+        const int row = 4 * q + (i16 >> 2);
+#pragma unroll
+        for (int t = 0; t < L::MT; ++t)
+            ft[t] = (unsigned)row * 512u + (unsigned)(((wm >> 4) + t) ^ (row & 7)) * 32u + (unsigned)(i16 & 3) * 8u;
+    }
+    if (BKIND == 0) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) fb[kk] = (unsigned)(wn + i16) * 128u + (unsigned)((kk * 4 + q) ^ (i16 >> 1)) * 16u;
+    } else if (BKIND == 1) fb[0] = (unsigned)(wn >> 4) * 2048u + (unsigned)(q * 16 + (i16 ^ (4 * q))) * 16u;
+    else {
+        const int r = 4 * q + (i16 >> 2), qq = i16 & 3;
+        fb[0] = (unsigned)(wn >> 5) * 1024u + (unsigned)(qq * 16 + (r ^ (4 * qq))) * 16u;
+    }
+
+    auto fetch = [&](int it, char* sa, char* sb) {
+        const int k = PARTS == 1 ? it : it / 6, s = PARTS == 1 ? 0 : it % 6;
+        const long long pa = PARTS == 1 ? 0 : part_a(s) * A.part, pb = PARTS == 1 ? 0 : part_b(s) * B.part;
+        const __amdgpu_buffer_rsrc_t ra = buffer(A.p + pa + k * A.step, A.left - k * A.step);
+        const __amdgpu_buffer_rsrc_t rb = buffer(B.p + pb + k * B.step, B.left - k * B.step);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            dma16(ra, sa + (wave * 4 + j) * 1024, AKIND == 0 && ca[j] >= A.kmax - k * BK ? NOWHERE : oa[j]);
+#pragma unroll
+        for (int j = 0; j < L::NB; ++j)
+            dma16(rb, sb + (wave * L::NB + j) * 1024, BKIND == 0 && cb[j] >= B.kmax - k * BK ? NOWHERE : ob[j]);
+    };
+    auto multiply = [&](int it, const char* sa, const char* sb) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            s16x8 a[L::MT], b[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (BKIND == 0) b[n] = *reinterpret_cast<const s16x8*>(sb + fb[kk] + n * 2048);
+                else if (BKIND == 1) b[n] = *reinterpret_cast<const s16x8*>(sb + fb[0] + n * 2048 + kk * 1024);
+                else {
+                    const char* p = sb + fb[0] + (n >> 1) * 1024 + (n & 1) * 8 + kk * 2 * (BN / 32) * 1024;
+                    b[n] = join(tr16(p), tr16(p + (BN / 32) * 1024));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < L::MT; ++t) {
+                if (AKIND == 0) a[t] = *reinterpret_cast<const s16x8*>(sa + fa[kk] + t * 2048);
+                else a[t] = join(tr16(sa + ft[t] + kk * 16384), tr16(sa + ft[t] + kk * 16384 + 8192));
+            }
+#pragma unroll
+            for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) acc[t][n] = mfma<E>(a[t], b[n], acc[t][n]);
+            if (COLSUM && (PARTS == 1 || part_a(it % 6) == 0)) {
+                const short one = __builtin_bit_cast(short, (E)1.0f);
+                const s16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) cs[n] = mfma<E>(ones, b[n], cs[n]);
+            }
+            __builtin_amdgcn_sched_barrier(0);           // fragments of one half step at a time: 128 sums leave room for no more
+        }
+    };
+    auto arrive = [&]() {                                // own loads landed, own reads done; then everyone's
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const int n = steps * (PARTS == 1 ? 1 : 6);
+    if (n > 0) fetch(0, a0, b0);
+    int it = 0;
+    for (; it + 2 <= n; it += 2) {
+        arrive();
+        fetch(it + 1, a1, b1);
+        multiply(it, a0, b0);
+        arrive();
+        if (it + 2 < n) fetch(it + 2, a0, b0);
+        multiply(it + 1, a1, b1);
+    }
+    if (it < n) {
+        arrive();
+        multiply(it, a0, b0);
+    }
+}
+
+// position in the launch -> tile: consecutive workgroups go to the 8 XCDs in turn; each gets a run of consecutive tiles, so
+// that what they share is fetched into one L2
+__device__ __forceinline__ int tile_of(int total) {
+    const int per = (total + 7) / 8;
+    const int t = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    return (int)(blockIdx.x >> 3) < per && t < total ? t : -1;
+}
+inline unsigned launch_for(long long tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
+
+// ------------------------------------------------------------------------------------------------
+// z^T tiles: loss statistics (GRAD = false) or blocks of G (GRAD = true)
+// ------------------------------------------------------------------------------------------------
+struct LogitArgs {
+    const char* w;            // W, ldw bytes a row, parts w_part bytes apart
+    const char* h;            // copy of H, [Rp][Dp], parts h_part bytes apart
+    const float* bias;        // [Vp], -inf behind V
+    const int* tgt;           // [Rp], -1: left out
+    float2* part;             // loss: [vocabulary tiles][Rp] (maximum, sum of exponentials)
+    float* zt;                // loss: [Rp] the target's logit
+    const float* lse;         // gradient
+    const float* wrow;        // gradient: [Rp], 0 for rows without a part in it
+    const float* scale;       // gradient, fp16: the scale of G, or NULL
+    char* g;                  // gradient: blocks of G, [Rp / 16][vocabulary tiles * 8], parts g_part bytes apart
+    long long w_part, h_part, g_part;
+    unsigned ldw;
+    int V, D, Dp, Rp, v_begin, nvt, nrt;      // vocabulary of this launch: tiles v_begin / 256 ..., nvt of them
+};
+
+template <typename E, int BN, int PARTS, bool GRAD>
+__global__ __launch_bounds__(512, 2) void xent_logit_kernel(LogitArgs a) {
+    typedef Lay<BN> L;
+    __shared__ __attribute__((aligned(1024))) char sa0[BM * BK * 2], sa1[BM * BK * 2], sb0[BN * BK * 2], sb1[BN * BK * 2];
+    __shared__ float2 red[L::WM][BN];
+    const int tile = tile_of(a.nvt * a.nrt);
+    if (tile < 0) return;
+    // bands of 8 row tiles, vocabulary tiles outside: the workgroups of an XCD share a few vocabulary and 8 row tiles
+    const int band = tile / (8 * a.nvt), in = tile - band * 8 * a.nvt;
+    const int wide = a.nrt - band * 8 < 8 ? a.nrt - band * 8 : 8;
+    const int vt = in / wide, rt = band * 8 + in % wide;
+    const long long v0 = (long long)a.v_begin + (long long)vt * BM;
+    const long long r0 = (long long)rt * BN;
+
+    Operand A, B;
+    A.p = a.w + v0 * a.ldw;
+    A.left = ((a.V - v0 < BM ? a.V - v0 : BM) - 1) * a.ldw + a.D * 2ll;
+    A.step = BK * 2; A.part = a.w_part; A.ld = a.ldw; A.kmax = a.D;
+    B.p = a.h + r0 * a.Dp * 2;
+    B.left = (long long)BN * a.Dp * 2;
+    B.step = BK * 2; B.part = a.h_part; B.ld = (unsigned)a.Dp * 2u; B.kmax = a.Dp;
+
+    f32x4 acc[L::MT][4], none[4];
+#pragma unroll
+    for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    core<E, BN, 0, 0, PARTS, false>(A, B, a.Dp / BK, sa0, sa1, sb0, sb1, acc, none);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
+    const int i16 = lane & 15, q = lane >> 4;
+    const float* bias = a.bias + v0 + wm + 4 * q;
+    if (!GRAD) {
+        float top[4], sum[4];
+        int tg[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            top[n] = -INFINITY;
+            tg[n] = a.tgt[r0 + wn + 16 * n + i16];
+        }
+#pragma unroll
+        for (int t = 0; t < L::MT; ++t) {
+            const f32x4 bv = *reinterpret_cast<const f32x4*>(bias + 16 * t);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[t][n][i] += bv[i];
+                    top[n] = fmaxf(top[n], acc[t][n][i]);
+                    if (tg[n] == (int)v0 + wm + 16 * t + 4 * q + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            // fmaxf leaves NaN out; the sum below brings it back (exp(NaN - top))
+            const float m = top[n] == -INFINITY ? 0.f : top[n];
+            float s = 0.f;
+#pragma unroll
+            for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s += PARTS == 1 ? __builtin_amdgcn_exp2f((acc[t][n][i] - m) * LOG2E) : expf(acc[t][n][i] - m);
+            sum[n] = s;
+        }
+        // lanes 16 apart hold other vocabulary entries of the same row
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float m2 = __shfl_xor(top[n], o, 64), s2 = __shfl_xor(sum[n], o, 64);
+                const float m = fmaxf(top[n], m2), base = m == -INFINITY ? 0.f : m;
+                sum[n] = sum[n] * expf(top[n] - base) + s2 * expf(m2 - base);
+                top[n] = m;
+            }
+        if (q == 0) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) red[wave / L::WN][wn + 16 * n + i16] = make_float2(top[n], sum[n]);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < BN) {
+            float m = -INFINITY, s = 0.f;
+#pragma unroll
+            for (int w = 0; w < L::WM; ++w) m = fmaxf(m, red[w][threadIdx.x].x);
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < L::WM; ++w) s += red[w][threadIdx.x].y * expf(red[w][threadIdx.x].x - base);
+            a.part[(long long)vt * a.Rp + r0 + threadIdx.x] = make_float2(m, s);
+        }
+    } else {
+        const float up = a.scale != nullptr ? a.scale[0] : 1.f;
+        const long long nv32 = (long long)a.nvt * (BM / 32);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const long long r = r0 + wn + 16 * n + i16;
+            const float w = a.wrow[r] * up, lse = a.lse[r];
+            const int tg = a.tgt[r];
+            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + (q * 16 + (i16 ^ (4 * q))) * 16;
+#pragma unroll
+            for (int t = 0; t < L::MT; t += 2) {
+                float g[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int tt = t + (j >> 2), i = j & 3;
+                    const float x = acc[tt][n][i] + bias[16 * tt + i] - lse;
+                    float p = PARTS == 1 ? __builtin_amdgcn_exp2f(x * LOG2E) : expf(x);
+                    if (tg == (int)v0 + wm + 16 * tt + 4 * q + i) p -= 1.f;
+                    g[j] = w == 0.f ? 0.f : p * w;
+                }
+                char* to = dst + (t >> 1) * 1024;
+#pragma unroll
+                for (int s = 0; s < PARTS; ++s) {
+                    s16x8 out;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const E e = (E)g[j];
+                        out[j] = __builtin_bit_cast(short, e);
+                        g[j] -= (float)e;
+                    }
+                    *reinterpret_cast<s16x8*>(to + s * a.g_part) = out;
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// The two gradient products.  A = W or H with the width as its rows (256 of them a tile), read transposed; B = G.
+//   OVER_V true:  out[r][d] = sum over v of G[r][v] W[v][d]       rows of out: rows of H
+//   OVER_V false: out[v][d] = sum over r of G[r][v] H[r][d]       rows of out: the piece's vocabulary; bias gradient too
+// The contraction is cut into `splits` parts when there are too few tiles for the chip; each leaves fp32 sums in a slab.
+// ------------------------------------------------------------------------------------------------
+struct ProductArgs {
+    const char* x;            // W (from the piece's first row on) or the copy of H
+    const char* g;
+    float* slab;              // [splits][rows][Dp], added to when add != 0; NULL: out is written
+    float* bslab;             // [splits][rows] bias gradient, or NULL
+    void* out;                // [rows][ld_out] of the caller's type
+    void* bout;
+    const float* scale;       // fp16: scale[1] takes the scale of G out again (written only with the final result)
+    long long x_part, g_part, x_bytes, ld_out, slab_stride;
+    unsigned ldx;
+    int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
+};
+
+template <typename E, typename T, int BN, int PARTS, bool OVER_V>
+__global__ __launch_bounds__(512, 2) void xent_product_kernel(ProductArgs a) {
+    typedef Lay<BN> L;
+    __shared__ __attribute__((aligned(1024))) char sa0[BM * BK * 2], sa1[BM * BK * 2], sb0[BN * BK * 2], sb1[BN * BK * 2];
+    const int tile = tile_of(a.ndt * a.nnt * a.splits);
+    if (tile < 0) return;
+    const int dt = tile % a.ndt, nt = tile / a.ndt % a.nnt, split = tile / (a.ndt * a.nnt);
+    const int k0 = (int)((long long)a.steps * split / a.splits), k1 = (int)((long long)a.steps * (split + 1) / a.splits);
+
+    Operand A, B;
+    A.ld = a.ldx; A.part = a.x_part; A.step = (long long)BK * a.ldx; A.kmax = 0;
+    const long long aoff = k0 * A.step + (long long)dt * BM * 2;
+    A.p = a.x + aoff;
+    A.left = a.x_bytes - aoff;
+    B.kmax = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
+    if (OVER_V) {
+        B.step = 2048;
+        B.p = a.g + (long long)nt * (BN / 16) * B.ld + k0 * B.step;
+        B.left = (long long)(BN / 16) * B.ld;
+    } else {
+        B.step = 4ll * B.ld;
+        B.p = a.g + (long long)nt * (BN / 32) * 1024 + k0 * B.step;
+        B.left = (long long)(a.steps - k0) * B.step;
+    }
+    f32x4 acc[L::MT][4], cs[4];
+#pragma unroll
+    for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) cs[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    core<E, BN, 1, OVER_V ? 1 : 2, PARTS, !OVER_V>(A, B, k1 - k0, sa0, sa1, sb0, sb1, acc, cs);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
+    const int i16 = lane & 15, q = lane >> 4;
+    const float down = a.scale != nullptr ? a.scale[1] : 1.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int r = nt * BN + wn + 16 * n + i16;
+        if (r >= a.rows) continue;
+#pragma unroll
+        for (int t = 0; t < L::MT; ++t) {
+            const int d = dt * BM + wm + 16 * t + 4 * q;
+            if (a.slab != nullptr) {
+                if (d < a.Dp) {
+                    f32x4* s = reinterpret_cast<f32x4*>(a.slab + split * a.slab_stride + (long long)r * a.Dp + d);
+                    *s = a.add ? *s + acc[t][n] : acc[t][n];
+                }
+            } else {
+                T* o = reinterpret_cast<T*>(a.out) + (long long)r * a.ld_out + d;
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = acc[t][n][i] * down;
+                if (a.out_vec && d < a.D) sv_store<4>(o, v);
+                else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < a.D) o[i] = (T)v[i];
+                }
+            }
+        }
+        if (!OVER_V && dt == 0 && wm == 0 && q == 0) {
+            if (a.bslab != nullptr) a.bslab[(long long)split * a.rows + r] = cs[n][0];
+            else if (a.bout != nullptr) reinterpret_cast<T*>(a.bout)[r] = (T)(cs[n][0] * down);
+        }
+    }
+}
+
+// out[r][d] = sum of the slabs, in order; also the bias gradient's (bslabs [splits][rows]; the last workgroups)
+template <typename T>
+__global__ __launch_bounds__(256) void xent_slab_sum_kernel(const float* __restrict__ slab, long long slab_stride, int splits, int rows,
+                                                            int D, int Dp, T* __restrict__ out, long long ld_out,
+                                                            const float* __restrict__ bslab, T* __restrict__ bout,
+                                                            const float* __restrict__ scale, unsigned nmain) {
+    const float down = scale != nullptr ? scale[1] : 1.f;
+    if (blockIdx.x < nmain) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+        const int per = Dp / 4;
+        const long long r = i / per;
+        const int d = (int)(i - r * per) * 4;
+        if (r >= rows || d >= D) return;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(slab + k * slab_stride + r * Dp + d);
+        T* o = out + r * ld_out + d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (d + j < D) o[j] = (T)(s[j] * down);
+    } else {
+        const long long r = (long long)(blockIdx.x - nmain) * 256 + threadIdx.x;
+        if (r >= rows) return;
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += bslab[(long long)k * rows + r];
+        bout[r] = (T)(s * down);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Copies: rows of H that take part, padded with zeros to [Rp][Dp] (a row that does not is zeros, whatever it holds); targets
+// and weights of the rows; the bias in fp32 with -inf behind the vocabulary; W where it cannot be loaded as it stands (fp32, or
+// rows that are no multiples of 16 bytes).  One launch, workgroup ranges.
+// ------------------------------------------------------------------------------------------------
+struct PrepArgs {
+    const void *h, *w, *bias, *tok;
+    const float *row_weight, *lse;        // NULL: loss only
+    char *hc, *wc;                        // wc NULL: W is not copied
+    float *biasf, *wrow, *lsec;
+    int* tgt;
+    long long ldh, ldw, h_part, w_part;
+    int tok64, R, Rp, V, Vp, D, Dp, nh, nb;
+};
+
+// eight columns of one row: from T to E, in PARTS parts
+template <typename T, typename E, int PARTS>
+__device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool live, char* dst, long long part) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = live && j < left ? (float)src[j] : 0.f;
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+        s16x8 out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const E e = (E)v[j];
+            out[j] = __builtin_bit_cast(short, e);
+            v[j] -= (float)e;
+        }
+        *reinterpret_cast<s16x8*>(dst + s * part) = out;
+    }
+}
+
+template <typename T, typename E, int PARTS>
+__global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
+    const int per = a.Dp / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if ((int)blockIdx.x < a.nh) {
+        const long long r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        if (r >= a.Rp) return;
+        int tg = -1;
+        float w = 0.f;
+        if (r < a.R) {
+            const long long t = a.tok64 ? reinterpret_cast<const long long*>(a.tok)[r] : (long long)reinterpret_cast<const int*>(a.tok)[r];
+            if (t >= 0 && t < a.V) tg = (int)t;
+            if (tg >= 0 && a.row_weight != nullptr) w = a.row_weight[r];
+        }
+        const bool live = tg >= 0 && (a.row_weight == nullptr || w != 0.f);
+        if (c == 0) {
+            a.tgt[r] = tg;
+            if (a.row_weight != nullptr) {
+                a.wrow[r] = w;
+                a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
+            }
+        }
+        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.h) + (live ? r : 0) * a.ldh + c, a.D - c, live, a.hc + (r * a.Dp + c) * 2, a.h_part);
+    } else if ((int)blockIdx.x < a.nh + a.nb) {
+        const long long v = i - (long long)a.nh * 256;
+        if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
+    } else {
+        const long long j = i - (long long)(a.nh + a.nb) * 256, r = j / per;
+        const int c = (int)(j - r * per) * 8;
+        if (r >= a.V) return;
+        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + r * a.ldw + c, a.D - c, true, a.wc + (r * a.Dp + c) * 2, a.w_part);
+    }
+}
+
+// lse and loss of 16 rows a workgroup from the tiles' statistics
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
+                                                         const int* __restrict__ tgt, int R, int Rp, int nvt,
+                                                         float* __restrict__ nll, float* __restrict__ lse) {
+    __shared__ float2 red[64][17];
+    const int i = threadIdx.x & 15, s = threadIdx.x >> 4;
+    const long long r = (long long)blockIdx.x * 16 + i;
+    float m = -INFINITY, sum = 0.f;
+    for (int v = s; v < nvt; v += 64) {
+        const float2 p = part[(long long)v * Rp + r];
+        const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
+        sum = sum * expf(m - base) + p.y * expf(p.x - base);
+        m = m2;
+    }
+    red[s][i] = make_float2(m, sum);
+    __syncthreads();
+    if (threadIdx.x >= 16 || r >= R) return;
+    for (int k = 1; k < 64; ++k) {
+        const float2 p = red[k][i];
+        const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
+        sum = sum * expf(m - base) + p.y * expf(p.x - base);
+        m = m2;
+    }
+    const bool here = tgt[r] >= 0;
+    const float l = m + logf(sum);
+    lse[r] = here ? l : 0.f;
+    nll[r] = here ? l - zt[r] : 0.f;
+}
+
+// sum of the losses and number of rows with a target; in a fixed order, in 64 bits (a mean over no rows is 0)
+__global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restrict__ nll, const void* __restrict__ tok, int tok64,
+                                                           int R, int V, int mean, float* __restrict__ out) {
+    __shared__ double red[1024];
+    __shared__ int cnt[1024];
+    double s = 0.0;
+    int n = 0;
+    for (int r = threadIdx.x; r < R; r += 1024) {
+        const long long t = tok64 ? reinterpret_cast<const long long*>(tok)[r] : (long long)reinterpret_cast<const int*>(tok)[r];
+        s += (double)nll[r];
+        n += t >= 0 && t < V;
+    }
+    red[threadIdx.x] = s;
+    cnt[threadIdx.x] = n;
+    __syncthreads();
+    for (int o = 512; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) {
+            red[threadIdx.x] += red[threadIdx.x + o];
+            cnt[threadIdx.x] += cnt[threadIdx.x + o];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const int c = cnt[0] > 0 ? cnt[0] : 1;
+        out[0] = (float)(mean ? red[0] / c : red[0]);
+        out[1] = (float)(mean ? 1.0 / c : 1.0);
+    }
+}
+
+// fp16: the power of two that brings the largest row weight to 2^13 .. 2^14, and its reciprocal
+__global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restrict__ wrow, int Rp, float* __restrict__ scale) {
+    __shared__ float red[16];
+    float m = 0.f;
+    for (int r = threadIdx.x; r < Rp; r += 1024) m = fmaxf(m, fabsf(wrow[r]));
+    m = sv_wave_max(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; ++k) m = fmaxf(m, red[k]);
+        int e = 0;
+        if (m > 0.f && m < INFINITY) frexpf(m, &e);          // m = f 2^e, f in [1/2, 1)
+        e = e > 100 ? 100 : e < -100 ? -100 : e;
+        scale[0] = ldexpf(1.f, 14 - e);
+        scale[1] = ldexpf(1.f, e - 14);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side: shapes, workspace, launches
+// ------------------------------------------------------------------------------------------------
+constexpr long long PIECE_BYTES = 512ll << 20;           // what G of one piece may take
+constexpr int CUS = 256;
+
+struct Shape {
+    int parts, Rp, Vp, Dp, BN, nrt, nvt, copy_w, pieces, piece_tiles, dh_splits, dw_splits, ndt;
+    long long h, h_part, w, w_part, ldw, bias, tgt, wrow, zt, part, scale, g, g_part, dh_slab, dw_slab, db_slab, total;
+};
+
+// parts of the contraction: least (rounds of workgroups) x (steps of each + what a workgroup costs beside them), plus the slabs'
+// traffic, in steps of about a microsecond
+inline int pick_splits(long long tiles, int steps, long long slab_bytes) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
+        const double cost = (double)((tiles * s + CUS - 1) / CUS) * ((steps + s - 1) / s + 3) + (s > 1 ? 2.0 * s * slab_bytes / 4e6 + 4 : 0);
+        if (cost < least * 0.98) { least = cost; best = s; }
+    }
+    return best;
+}
+
+inline int shape_of(const void* weight, long long ld_w, int type, long long R, long long V, long long D, int grad, Shape* s) {
+    SV_CHECK_ARG(type >= 0 && type <= 2, "svae_xent: type %d", type);
+    SV_CHECK_ARG(R > 0 && R <= 1 << 24 && V > 0 && V <= 1 << 28 && D > 0 && D <= 1 << 16 && ld_w >= D && ld_w <= 1 << 20,
+                 "svae_xent: sizes R %lld, V %lld, D %lld, ld %lld", R, V, D, ld_w);
+    s->parts = type == SV_F32 ? 3 : 1;
+    s->BN = R <= 64 ? 64 : 256;
+    s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
+    s->Vp = (int)((V + BM - 1) / BM * BM);
+    s->Dp = (int)((D + BK - 1) / BK * BK);
+    s->nrt = s->Rp / s->BN;
+    s->nvt = s->Vp / BM;
+    s->ndt = (s->Dp + BM - 1) / BM;
+    s->copy_w = type == SV_F32 || D % 8 != 0 || ld_w % 8 != 0 || (unsigned long long)weight % 16 != 0;
+    SV_CHECK_ARG((long long)s->nvt * s->nrt < 0x7ffffff0ll, "svae_xent: R %lld and V %lld need too many workgroups", R, V);
+    long long at = 0;
+    auto take = [&](long long bytes) {
+        const long long p = at;
+        at += (bytes + 1023) / 1024 * 1024;
+        return p;
+    };
+    s->h_part = (long long)s->Rp * s->Dp * 2;
+    s->h = take(s->h_part * s->parts);
+    s->w_part = s->copy_w ? V * s->Dp * 2 : 0;
+    s->ldw = (s->copy_w ? s->Dp : ld_w) * 2;
+    s->w = take(s->w_part * s->parts);
+    s->bias = take(4ll * s->Vp);
+    s->tgt = take(4ll * s->Rp);
+    s->wrow = take(4ll * s->Rp);
+    s->zt = take(4ll * s->Rp);
+    s->scale = take(8);
+    s->g = s->part = at;                                   // the loss's statistics and the gradient's pieces share the rest
+    long long end = at + 8ll * s->nvt * s->Rp;
+    if (grad) {
+        long long tiles = PIECE_BYTES / (2ll * s->parts * s->Rp * BM);
+        tiles = tiles < 1 ? 1 : tiles > s->nvt ? s->nvt : tiles;
+        s->pieces = (int)((s->nvt + tiles - 1) / tiles);
+        s->piece_tiles = (s->nvt + s->pieces - 1) / s->pieces;
+        s->g_part = 2ll * s->Rp * s->piece_tiles * BM;
+        s->g = take(s->g_part * s->parts);
+        s->dh_splits = pick_splits((long long)s->ndt * s->nrt, s->piece_tiles * (BM / BK) * (s->parts == 1 ? 1 : 6), 4ll * s->Rp * s->Dp);
+        s->dh_slab = take(4ll * s->Rp * s->Dp * s->dh_splits);
+        s->dw_splits = pick_splits((long long)s->ndt * s->piece_tiles, s->Rp / BK * (s->parts == 1 ? 1 : 6), 4ll * s->piece_tiles * BM * s->Dp);
+        s->dw_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->Dp * s->dw_splits : 0);
+        s->db_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->dw_splits : 0);
+    }
+    s->total = at > end ? at : end;
+    return 0;
+}
+
+struct Call {
+    const void *hidden, *weight, *bias, *targets;
+    long long ld_h, ld_w;
+    int tok64, type, R, V, D;
+    char* work;
+    hipStream_t stream;
+};
+
+// calls f(T{}, E{}, parts) with the caller's and the matrix units' element types
+template <typename F>
+inline void by_type(int type, F f) {
+    if (type == SV_F32) f(float{}, __bf16{}, std::integral_constant<int, 3>{});
+    else if (type == SV_BF16) f(__bf16{}, __bf16{}, std::integral_constant<int, 1>{});
+    else f(_Float16{}, _Float16{}, std::integral_constant<int, 1>{});
+}
+
+inline int prepare(const Call& c, const Shape& s, const float* row_weight, const float* lse) {
+    PrepArgs p;
+    p.lse = lse;
+    p.lsec = (float*)(c.work + s.zt);
+    p.h = c.hidden; p.w = c.weight; p.bias = c.bias; p.tok = c.targets; p.row_weight = row_weight;
+    p.hc = c.work + s.h;
+    p.wc = s.copy_w ? c.work + s.w : nullptr;
+    p.biasf = (float*)(c.work + s.bias); p.wrow = (float*)(c.work + s.wrow); p.tgt = (int*)(c.work + s.tgt);
+    p.ldh = c.ld_h; p.ldw = c.ld_w; p.h_part = s.h_part; p.w_part = s.w_part;
+    p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.Vp = s.Vp; p.D = c.D; p.Dp = s.Dp;
+    const long long nh = ((long long)s.Rp * (s.Dp / 8) + 255) / 256, nb = (s.Vp + 255) / 256,
+                    nw = s.copy_w ? ((long long)c.V * (s.Dp / 8) + 255) / 256 : 0;
+    SV_CHECK_ARG(nh + nb + nw < 0x7ffffff0ll, "svae_xent: too large");
+    p.nh = (int)nh; p.nb = (int)nb;
+    by_type(c.type, [&](auto t, auto e, auto parts) {
+        hipLaunchKernelGGL((xent_prep_kernel<decltype(t), decltype(e), decltype(parts)::value>), dim3((unsigned)(nh + nb + nw)), dim3(256), 0, c.stream, p);
+    });
+    SV_LAUNCH_CHECK();
+    return 0;
+}
+
+inline LogitArgs logit_args(const Call& c, const Shape& s) {
+    LogitArgs a{};
+    a.w = s.copy_w ? c.work + s.w : (const char*)c.weight;
+    a.h = c.work + s.h;
+    a.bias = (const float*)(c.work + s.bias); a.tgt = (const int*)(c.work + s.tgt);
+    a.w_part = s.w_part; a.h_part = s.h_part; a.g_part = s.g_part;
+    a.ldw = (unsigned)s.ldw;
+    a.V = c.V; a.D = s.copy_w ? s.Dp : c.D; a.Dp = s.Dp; a.Rp = s.Rp; a.nrt = s.nrt;
+    return a;
+}
+
+template <bool GRAD>
+inline void logits(const Call& c, const Shape& s, const LogitArgs& a) {
+    by_type(c.type, [&](auto, auto e, auto parts) {
+        typedef decltype(e) E;
+        constexpr int P = decltype(parts)::value;
+        const dim3 grid(launch_for((long long)a.nvt * a.nrt));
+        if (s.BN == 64) hipLaunchKernelGGL((xent_logit_kernel<E, 64, P, GRAD>), grid, dim3(512), 0, c.stream, a);
+        else hipLaunchKernelGGL((xent_logit_kernel<E, 256, P, GRAD>), grid, dim3(512), 0, c.stream, a);
+    });
+}
+
+inline int check_call(const char* name, const Call& c, const void* work, long long work_bytes, int grad, Shape* s) {
+    SV_CHECK_ARG(c.hidden && c.weight && c.targets && work, "%s: null pointer", name);
+    SV_CHECK_ARG(c.ld_h >= c.D, "%s: ld %lld of the hidden rows is below D %d", name, c.ld_h, c.D);
+    SV_CHECK_ARG((unsigned long long)work % 256 == 0, "%s: the workspace must be aligned to 256 bytes", name);
+    const int rc = shape_of(c.weight, c.ld_w, c.type, c.R, c.V, c.D, grad, s);
+    if (rc != 0) return rc;
+    SV_CHECK_ARG(work_bytes >= s->total, "%s: workspace of %lld bytes, %lld needed", name, work_bytes, s->total);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int svae_xent_bytes(const void* weight, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes) {
+    SV_CHECK_ARG(bytes != nullptr, "svae_xent_bytes: null pointer");
+    Shape s{};
+    const int rc = shape_of(weight, ld_w, type, R, V, D, grad, &s);
+    if (rc != 0) return rc;
+    *bytes = s.total;
+    return 0;
+}
+
+extern "C" int svae_xent_fwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                             const void* targets, int tok64, int type, int R, int V, int D, float* nll, float* lse, void* work,
+                             long long work_bytes, void* stream) {
+    Call c{hidden, weight, bias, targets, ld_h, ld_w, tok64, type, R, V, D, (char*)work, (hipStream_t)stream};
+    Shape s{};
+    int rc = check_call("svae_xent_fwd", c, work, work_bytes, 0, &s);
+    if (rc != 0) return rc;
+    SV_CHECK_ARG(nll && lse, "svae_xent_fwd: null pointer");
+    rc = prepare(c, s, nullptr, nullptr);
+    if (rc != 0) return rc;
+    LogitArgs a = logit_args(c, s);
+    a.part = (float2*)(c.work + s.part);
+    a.zt = (float*)(c.work + s.zt);
+    a.v_begin = 0; a.nvt = s.nvt;
+    logits<false>(c, s, a);
+    SV_LAUNCH_CHECK();
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(s.Rp / 16), dim3(1024), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
+    SV_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int svae_xent_reduce(const float* nll, const void* targets, int tok64, int R, int V, int mean, float* out, void* stream) {
+    SV_CHECK_ARG(nll && targets && out && R > 0 && V > 0, "svae_xent_reduce: bad arguments");
+    hipLaunchKernelGGL(xent_reduce_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, nll, targets, tok64, R, V, mean, out);
+    SV_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                             const void* targets, int tok64, int type, int R, int V, int D, const float* lse,
+                             const float* row_weight, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db, void* work,
+                             long long work_bytes, void* stream) {
+    Call c{hidden, weight, bias, targets, ld_h, ld_w, tok64, type, R, V, D, (char*)work, (hipStream_t)stream};
+    Shape s{};
+    int rc = check_call("svae_xent_bwd", c, work, work_bytes, 1, &s);
+    if (rc != 0) return rc;
+    SV_CHECK_ARG(lse && row_weight, "svae_xent_bwd: null pointer");
+    SV_CHECK_ARG((!dh || ld_dh >= D) && (!dw || ld_dw >= D), "svae_xent_bwd: ld %lld, %lld below D %d", ld_dh, ld_dw, D);
+    SV_CHECK_ARG(!db || dw, "svae_xent_bwd: the bias gradient comes with the weight gradient");
+    if (!dh && !dw) return 0;
+    rc = prepare(c, s, row_weight, lse);
+    if (rc != 0) return rc;
+    LogitArgs a = logit_args(c, s);
+    a.lse = (const float*)(c.work + s.zt);
+    a.wrow = (const float*)(c.work + s.wrow);
+    a.g = c.work + s.g;
+    const float* scale = nullptr;
+    if (type == SV_F16) {
+        scale = (const float*)(c.work + s.scale);
+        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, c.stream, a.wrow, s.Rp, (float*)(c.work + s.scale));
+        SV_LAUNCH_CHECK();
+    }
+    a.scale = scale;
+    const int es = sv_elem_size(type);
+    for (int p = 0; p < s.pieces; ++p) {
+        const int t0 = p * s.piece_tiles, nt = s.nvt - t0 < s.piece_tiles ? s.nvt - t0 : s.piece_tiles;
+        if (nt <= 0) break;
+        const long long v0 = (long long)t0 * BM;
+        const int rows_v = (int)(V - v0 < (long long)nt * BM ? V - v0 : (long long)nt * BM);
+        a.v_begin = (int)v0; a.nvt = nt;
+        logits<true>(c, s, a);
+        SV_LAUNCH_CHECK();
+        ProductArgs d{};
+        d.g = a.g; d.scale = scale; d.g_part = s.g_part; d.D = D; d.Dp = s.Dp; d.ndt = s.ndt; d.nv32 = nt * (BM / 32);
+        if (dh) {
+            d.x = a.w + v0 * s.ldw;
+            d.x_bytes = (rows_v - 1) * s.ldw + (s.copy_w ? s.Dp : D) * 2ll;
+            d.x_part = s.w_part; d.ldx = (unsigned)s.ldw;
+            d.slab = (float*)(c.work + s.dh_slab); d.slab_stride = (long long)s.Rp * s.Dp;
+            d.rows = s.Rp; d.nnt = s.nrt; d.splits = s.dh_splits; d.steps = nt * (BM / BK); d.add = p > 0;
+            by_type(type, [&](auto t, auto e, auto parts) {
+                typedef decltype(t) T;
+                typedef decltype(e) E;
+                constexpr int P = decltype(parts)::value;
+                const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
+                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(512), 0, c.stream, d);
+                else hipLaunchKernelGGL((xent_product_kernel<E, T, 256, P, true>), grid, dim3(512), 0, c.stream, d);
+            });
+            SV_LAUNCH_CHECK();
+        }
+        if (dw) {
+            d.x = a.h; d.x_bytes = s.h_part; d.x_part = s.h_part; d.ldx = (unsigned)s.Dp * 2u;
+            d.rows = rows_v; d.nnt = nt; d.splits = s.dw_splits; d.steps = s.Rp / BK; d.add = 0;
+            d.out = (char*)dw + v0 * ld_dw * es; d.ld_out = ld_dw;
+            d.bout = db ? (char*)db + v0 * es : nullptr;
+            d.slab = s.dw_splits > 1 ? (float*)(c.work + s.dw_slab) : nullptr;
+            d.bslab = s.dw_splits > 1 && db ? (float*)(c.work + s.db_slab) : nullptr;
+            d.slab_stride = (long long)s.piece_tiles * BM * s.Dp;
+            const int wide = es * 4 < 16 ? es * 4 : 16;
+            d.out_vec = D % 4 == 0 && ld_dw * es % wide == 0 && (unsigned long long)d.out % wide == 0;
+            by_type(type, [&](auto t, auto e, auto parts) {
+                typedef decltype(t) T;
+                typedef decltype(e) E;
+                constexpr int P = decltype(parts)::value;
+                hipLaunchKernelGGL((xent_product_kernel<E, T, 256, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(512), 0, c.stream, d);
+                if (d.slab != nullptr) {
+                    const unsigned nmain = (unsigned)(((long long)rows_v * (s.Dp / 4) + 255) / 256), nbias = db ? (rows_v + 255) / 256 : 0;
+                    hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain + nbias), dim3(256), 0, c.stream, d.slab, d.slab_stride, d.splits, rows_v, D,
+                                       s.Dp, (T*)d.out, ld_dw, d.bslab, (T*)d.bout, scale, nmain);
+                }
+            });
+            SV_LAUNCH_CHECK();
+        }
+    }
+    if (dh) {
+        by_type(type, [&](auto t, auto, auto) {
+            typedef decltype(t) T;
+            const unsigned nmain = (unsigned)(((long long)R * (s.Dp / 4) + 255) / 256);
+            hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain), dim3(256), 0, c.stream, (const float*)(c.work + s.dh_slab), (long long)s.Rp * s.Dp,
+                               s.dh_splits, R, D, s.Dp, (T*)dh, ld_dh, (const float*)nullptr, (T*)nullptr, scale, nmain);
+        });
+        SV_LAUNCH_CHECK();
+    }
+    return 0;
+}

@@ -224,3 +224,125 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and shaped like x")
     return _dropout(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key, out)
+
+
+# ---- softmax cross entropy behind a linear layer ----------------------------------------------------------------------------
+def _xent_args(hidden, weight, targets, bias):
+    """Checks; returns (hidden rows, weight rows, bias, flat targets, R, V, D)."""
+    _check(hidden, "hidden")
+    _check(weight, "weight", {hidden.dtype: 0}, hidden.device)
+    _check(targets, "targets", _IDS, hidden.device)
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError("hidden %s and weight %s do not fit: [..., D] and [V, D]" % (tuple(hidden.shape), tuple(weight.shape)))
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError("targets %s do not have one entry for each row of hidden %s" % (tuple(targets.shape), tuple(hidden.shape)))
+    V, D = weight.shape
+    R = targets.numel()
+    _size(V, "vocabulary", 1 << 28)
+    _size(D, "width", 1 << 16)
+    _size(R + 1, "rows + 1", (1 << 24) + 1)
+    if bias is not None:
+        _check(bias, "bias", {hidden.dtype: 0}, hidden.device)
+        if tuple(bias.shape) != (V,):
+            raise ValueError("bias %s must be [%d]" % (tuple(bias.shape), V))
+        bias = bias.contiguous()
+    h, w = _rows(hidden.reshape(R, D)), _rows(weight)
+    return h, w if _ld(w) <= 1 << 20 else w.contiguous(), bias, targets.reshape(-1).contiguous(), R, V, D
+
+
+def _xent_work(w, h, R, V, D, grad):
+    n = _bytes("svae_xent_bytes", w.data_ptr(), _ld(w), _TYPES[h.dtype], R, V, D, int(grad))
+    return torch.empty(n, dtype=torch.uint8, device=h.device)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _xent_fwd(h, w, bias, tok, R, V, D, work, st):
+    nll, lse = torch.empty(2, R, dtype=torch.float32, device=h.device)
+    _lib.call("svae_xent_fwd", h.data_ptr(), _ld(h), w.data_ptr(), _ld(w), _ptr(bias), tok.data_ptr(), _IDS[tok.dtype], _TYPES[h.dtype],
+              R, V, D, nll.data_ptr(), lse.data_ptr(), work.data_ptr(), work.numel(), st)
+    return nll, lse
+
+
+def _xent_bwd(h, w, bias, tok, R, V, D, lse, row_weight, need, work, st):
+    new = dict(dtype=h.dtype, device=h.device)
+    dh = torch.empty((R, D), **new) if need[0] else None
+    dw = torch.empty((V, D), **new) if need[1] or need[2] else None
+    db = torch.empty(V, **new) if need[2] else None
+    _lib.call("svae_xent_bwd", h.data_ptr(), _ld(h), w.data_ptr(), _ld(w), _ptr(bias), tok.data_ptr(), _IDS[tok.dtype], _TYPES[h.dtype],
+              R, V, D, lse.data_ptr(), row_weight.data_ptr(), _ptr(dh), D, _ptr(dw), D, _ptr(db), work.data_ptr(), work.numel(), st)
+    return dh, dw if need[1] else None, db
+
+
+def linear_nll(hidden, weight, targets, bias=None):
+    """(nll, lse) of ``softmax(hidden @ weight.T + bias)`` for the targets, fp32, shaped like targets; no logits are kept.
+
+    hidden [..., D], weight [V, D], bias [V] of one type; targets int32 / int64.  A row whose target is outside [0, V) is left
+    out: both are 0.  For scoring, and for programs that run their own backward pass (``linear_nll_grad``)."""
+    h, w, bias, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
+    if R == 0:
+        nll = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
+        return nll, nll.clone()
+    with _On(h) as st:
+        nll, lse = _xent_fwd(h, w, bias, tok, R, V, D, _xent_work(w, h, R, V, D, False), st)
+    return nll.view(targets.shape), lse.view(targets.shape)
+
+
+def linear_nll_grad(hidden, weight, targets, row_weight, bias=None):
+    """(nll, lse, dhidden, dweight, dbias): ``linear_nll`` and the gradients of ``sum(row_weight * nll)`` in the inputs' type
+    (dbias None without a bias).  row_weight: fp32, shaped like targets; a row of weight 0 takes no part in the gradient."""
+    h, w, bias, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
+    _check(row_weight, "row_weight", {torch.float32: 0}, h.device)
+    if row_weight.shape != targets.shape:
+        raise ValueError("row_weight %s must be shaped like targets %s" % (tuple(row_weight.shape), tuple(targets.shape)))
+    if R == 0:
+        nll = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
+        return nll, nll.clone(), torch.empty_like(hidden), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias)
+    with _On(h) as st:
+        work = _xent_work(w, h, R, V, D, True)
+        nll, lse = _xent_fwd(h, w, bias, tok, R, V, D, work, st)
+        dh, dw, db = _xent_bwd(h, w, bias, tok, R, V, D, lse, row_weight.reshape(-1).contiguous(), (True, True, bias is not None), work, st)
+    return nll.view(targets.shape), lse.view(targets.shape), dh.view(hidden.shape), dw, db
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, targets, reduction):
+        h, w, b, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
+        ctx.shapes, ctx.reduction = (hidden.shape, R, V, D), reduction
+        out = torch.zeros(2, dtype=torch.float32, device=h.device)
+        if R == 0:
+            ctx.save_for_backward(h, w, b, tok, out, out)
+            return out.new_empty(targets.shape) if reduction == "none" else out[0].clone()
+        with _On(h) as st:
+            nll, lse = _xent_fwd(h, w, b, tok, R, V, D, _xent_work(w, h, R, V, D, False), st)
+            if reduction != "none":
+                _lib.call("svae_xent_reduce", nll.data_ptr(), tok.data_ptr(), _IDS[tok.dtype], R, V, int(reduction == "mean"), out.data_ptr(), st)
+        ctx.save_for_backward(h, w, b, tok, lse, out)
+        return nll.view(targets.shape) if reduction == "none" else out[0].clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        h, w, b, tok, lse, out = ctx.saved_tensors
+        shape, R, V, D = ctx.shapes
+        if R == 0:
+            return h.new_empty(shape), torch.zeros_like(w), None if b is None else torch.zeros_like(b), None, None
+        weight = dloss.reshape(-1).float().contiguous() if ctx.reduction == "none" else (dloss.float() * out[1]).expand(R).contiguous()
+        with _On(h) as st:
+            need = ctx.needs_input_grad[:3]
+            dh, dw, db = _xent_bwd(h, w, b, tok, R, V, D, lse, weight, need, _xent_work(w, h, R, V, D, True), st)
+        return None if dh is None else dh.view(shape), dw, db, None, None
+
+
+def linear_cross_entropy(hidden, weight, targets, bias=None, reduction="mean"):
+    """Softmax cross entropy of the logits ``hidden @ weight.T + bias`` without ever keeping them, fp32.
+
+    hidden [..., D], weight [V, D], bias [V] of one type (fp32, bf16, fp16); targets int32 / int64, shaped ``hidden.shape[:-1]``;
+    a target outside [0, V) leaves its row out.  reduction: "mean" over the rows with a target (0 if there are none), "sum" or
+    "none".  The backward pass makes the logits again in pieces of the vocabulary; gradients have the inputs' type."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be mean, sum or none, got %r" % (reduction,))
+    return _LinearCrossEntropy.apply(hidden, weight, bias, targets, reduction)

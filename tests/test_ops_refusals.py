@@ -61,3 +61,28 @@ def test_dropout_entry_point_refuses():
     refused("sizes", "svae_dropout", P, 7, P, 8, 0, 2, 8, 0.5, 1, 0, None, None, None)
     refused("type", "svae_dropout", P, 8, P, 8, 5, 2, 8, 0.5, 1, 0, None, None, None)
     refused("null", "svae_dropout", P, 8, None, 8, 0, 2, 8, 0.5, 1, 0, None, None, None)
+
+
+def test_xent_entry_points_refuse():
+    n = ctypes.c_longlong()
+    for bad in ((P, 8, 7, 4, 10, 8, 0), (P, 7, 1, 4, 10, 8, 0), (P, 8, 1, 0, 10, 8, 0), (P, 8, 1, 4, 0, 8, 1), (P, 8, 1, 4, 10, 0, 1),
+                (P, 1 << 21, 1, 4, 10, 8, 0), (P, 1 << 17, 1, 4, 10, (1 << 16) + 1, 0)):
+        refused("svae_xent: (type|sizes)", "svae_xent_bytes", *bad, ctypes.byref(n))
+    refused("null", "svae_xent_bytes", P, 8, 1, 4, 10, 8, 0, None)
+    refused("null", "svae_xent_fwd", None, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 1 << 30, None)
+    refused("ld", "svae_xent_fwd", P, 7, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 1 << 30, None)
+    refused("workspace", "svae_xent_fwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 100, None)
+    refused("aligned", "svae_xent_fwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, ctypes.c_void_p(264), 1 << 30, None)
+    refused("null", "svae_xent_fwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, None, P, P, 1 << 30, None)
+    refused("null", "svae_xent_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, None, P, P, 8, P, 8, None, P, 1 << 30, None)
+    refused("ld", "svae_xent_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 7, P, 8, None, P, 1 << 30, None)
+    refused("bias gradient", "svae_xent_bwd", P, 8, P, 8, P, P, 0, 1, 4, 10, 8, P, P, P, 8, None, 8, P, P, 1 << 30, None)
+    refused("bad arguments", "svae_xent_reduce", P, P, 0, 0, 10, 1, P, None)
+
+
+def test_xent_refuses_what_does_not_fit():
+    t = torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.linear_nll(t, t, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="reduction"):
+        ops.linear_cross_entropy(t, t, torch.zeros(4, dtype=torch.int64), reduction="max")
