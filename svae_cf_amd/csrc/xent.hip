@@ -8,9 +8,10 @@
 // piece is written to the workspace, then two products take it up.  Everything is bound by the matrix units (6 R V D flops for
 // loss and gradient and 2 R V D for making z again), except that few rows leave the loss bound by reading W.
 //
-// All products run on one core: 256 x 256 (or 256 x 64) outputs a workgroup, 8 waves, steps of 64 along the contraction, two
+// All products run on one core: 256 x 128 (or 256 x 64) outputs a workgroup of 4 waves, steps of 32 along the contraction, three
 // stages of LDS filled by LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from
-// writes to the other and does not wait for the prefetch), v_mfma_f32_16x16x32.
+// writes to the other and does not wait for the prefetch), v_mfma_f32_16x16x32.  Two workgroups share a CU: one multiplies
+// while the other waits at its barrier, reads fragments or works through an epilogue.
 //   z^T tile: A = W rows, B = H rows, both with the contraction contiguous.  C has the row of H in the lane and four vocabulary
 //     entries in registers, so a row's maximum and sum are mostly in-lane work.
 //   G is kept as blocks of 16 rows x 32 vocabulary entries, 1 KiB: a lane's 16 bytes are the 8 values that it made, which are a
@@ -32,7 +33,11 @@ typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 constexpr int BM = 256;                   // outputs of a workgroup along A
-constexpr int BK = 64;                    // contraction of a step
+constexpr int BK = 32;                    // contraction of a step
+constexpr int STAGES = 3;
+constexpr int WAVES = 4;
+constexpr int AHEAD = 4;                  // fragments of A that are read in front of their products
+constexpr int KPAD = 64;                  // the copies' row length is a multiple of this
 constexpr unsigned BUF_FLAGS = 0x00020000u;
 constexpr unsigned NOWHERE = 0xFFFFFFF0u; // past every buffer's end: such a lane loads zeros
 constexpr float LOG2E = 1.4426950408889634f;
@@ -48,10 +53,6 @@ __device__ __forceinline__ f32x4 mfma<_Float16>(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, long long bytes) {
-    const long long n = bytes < 0 ? 0 : bytes > 0xFFFFFF00ll ? 0xFFFFFF00ll : bytes;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (unsigned)n, BUF_FLAGS);
-}
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, char* lds, unsigned off) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)lds, 16, off, 0, 0, 0);
 }
@@ -61,50 +62,40 @@ __device__ __forceinline__ s16x4 tr16(const char* p) {
 __device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // the six leading products of two numbers in three parts each, smallest first: part of A, part of B
-__device__ __forceinline__ int part_a(int s) { return (0x001102 >> (4 * s)) & 15; }
-__device__ __forceinline__ int part_b(int s) { return (0x010120 >> (4 * s)) & 15; }
+__device__ __forceinline__ constexpr int part_a(int s) { return (0x001102 >> (4 * s)) & 15; }
+__device__ __forceinline__ constexpr int part_b(int s) { return (0x010120 >> (4 * s)) & 15; }
 
 // ------------------------------------------------------------------------------------------------
-// The core: acc[t][n] (16 x 16 each; A side t, B side n) += A B over `steps` steps of 64.
-//   AKIND 0: A [m][k], k contiguous (rows lda bytes apart)      LDS image [256 m][64 k]
-//   AKIND 1: A [k][m], m contiguous                             LDS image [64 k][256 m], read transposed
+// The core: acc[t][n] (16 x 16 each; A side t, B side n) += A B over `steps` steps of 32.
+//   AKIND 0: A [m][k], k contiguous (rows lda bytes apart)      LDS image [256 m][32 k]
+//   AKIND 1: A [k][m], m contiguous                             LDS image [32 k][256 m], read transposed
 //   BKIND 0: B [n][k] like A      BKIND 1: blocks of G, contraction over the vocabulary      BKIND 2: over the rows
 // LDS images hold 16-byte chunks; which chunk a lane fetches is permuted so that the 16 lanes that a read serves at a time
-// fall on different banks: [.][64] images: chunk c of row r at c ^ ((r / 2) % 8); [.][256]: pairs of chunks, c ^ 2 (r % 8).
-// PARTS 3: the step runs over the six pairs of parts; the parts of an operand lie apart by a_part / b_part bytes.
+// fall on different banks: [.][32] images: chunk c of row r at c ^ ((r / 4) % 4); [.][256]: pairs of chunks, c ^ 2 (r % 8).
+// PARTS 3: every step runs over the six pairs of parts; the parts of an operand lie apart by a_part / b_part bytes.
 // ------------------------------------------------------------------------------------------------
+// What LDS-DMA may read from an operand at contraction step k is [p + k step, + bytes).  Kind 1: whole steps all have `bytes`,
+// step `full` has `tail` (rows that end inside it), later ones nothing.  Kind 0 loses `step` bytes a step, as p moves along its rows.
 struct Operand {
-    const char* p;        // first row (contraction step 0) of the tile
-    long long left;       // bytes from p to the end of what may be read
+    const char* p;        // first row, contraction step 0 of the tile
     long long step;       // bytes from one step to the next
     long long part;       // bytes from one part to the next
-    unsigned ld;          // bytes between rows (BKIND 1, 2: between blocks of 16 rows)
-    int kmax;             // AKIND / BKIND 0: length of a row in elements; chunks behind it are loaded as zeros
+    unsigned bytes, tail;
+    int full;
+    unsigned ld;          // bytes between rows (BKIND 1, 2: between the blocks of one and the next 16 rows)
+    int kmax;             // AKIND 0: length of a row in elements; chunks behind it are loaded as zeros
 };
 
 template <int BN>
 struct Lay {
     static constexpr int WN = BN / 64;                  // waves along B, 64 outputs each
-    static constexpr int WM = 8 / WN;                   // waves along A
+    static constexpr int WM = WAVES / WN;               // waves along A
     static constexpr int MT = BM / WM / 16;             // 16-wide tiles of a wave along A
-    static constexpr int NB = BN / 64;                  // LDS-DMA instructions of a wave for B and step (4 for A)
+    static constexpr int NA = BM * BK * 2 / 1024 / WAVES, NB = BN * BK * 2 / 1024 / WAVES;     // LDS-DMA instructions of a wave and step
 };
 
-// lane offsets of the LDS-DMA instructions (global side)
-template <int KIND>
-__device__ __forceinline__ unsigned dma_off(int inst, int lane, unsigned ld) {
-    if (KIND == 0) {
-        const int row = inst * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-        return (unsigned)row * ld + (unsigned)c * 16u;
-    } else if (KIND == 1) {                              // [64 k][256 m]
-        const int row = inst * 2 + (lane >> 5), c = (lane & 31) ^ ((row & 7) << 1);
-        return (unsigned)row * ld + (unsigned)c * 16u;
-    }
-    return 0;
-}
-
 template <typename E, int BN, int AKIND, int BKIND, int PARTS, bool COLSUM>
-__device__ __forceinline__ void core(const Operand& A, const Operand& B, int steps, char* a0, char* a1, char* b0, char* b1,
+__device__ __forceinline__ void core(const Operand& A, const Operand& B, int steps, char* const (&sa)[STAGES], char* const (&sb)[STAGES],
                                      f32x4 (&acc)[Lay<BN>::MT][4], f32x4 (&cs)[4]) {
     typedef Lay<BN> L;
     const int lane = threadIdx.x & 63;
@@ -112,106 +103,136 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
     const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
     const int i16 = lane & 15, q = lane >> 4;
 
-    unsigned oa[4], ob[L::NB];
-    int ca[4], cb[L::NB];                                // first element of the chunk inside the step (kind 0)
+    // LDS-DMA: every instruction fills 1 KiB
+    //   kind 0: 16 rows of 4 chunks      kind 1: 2 rows of 32 chunks      blocks of G: one block
+    const int chunk = (lane & 3) ^ q;                    // kind 0: chunk (lane % 4) ^ ((row / 4) % 4), row = lane / 4
+    unsigned oa[L::NA], ob[L::NB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        oa[j] = dma_off<AKIND>(wave * 4 + j, lane, A.ld);
-        ca[j] = (int)((oa[j] - (unsigned)((wave * 4 + j) * 8 + (lane >> 3)) * A.ld) >> 1);
+    for (int j = 0; j < L::NA; ++j) {
+        const unsigned inst = (unsigned)(wave * L::NA + j);
+        if (AKIND == 0) oa[j] = (inst * 16u + (unsigned)(lane >> 2)) * A.ld + (unsigned)chunk * 16u;
+        else {
+            const unsigned row = inst * 2u + (unsigned)(lane >> 5);
+            oa[j] = row * A.ld + (((unsigned)lane & 31u) ^ ((row & 7u) << 1)) * 16u;
+        }
     }
 #pragma unroll
     for (int j = 0; j < L::NB; ++j) {
-        const int b = wave * L::NB + j;
-        if (BKIND == 0) {
-            ob[j] = dma_off<0>(b, lane, B.ld);
-            cb[j] = (int)((ob[j] - (unsigned)(b * 8 + (lane >> 3)) * B.ld) >> 1);
-        } else if (BKIND == 1) ob[j] = (unsigned)(b >> 1) * B.ld + (unsigned)(b & 1) * 1024u + (unsigned)lane * 16u;
-        else ob[j] = (unsigned)(b / (BN / 32)) * B.ld + (unsigned)(b % (BN / 32)) * 1024u + (unsigned)lane * 16u;
+        const unsigned inst = (unsigned)(wave * L::NB + j);
+        if (BKIND == 0) ob[j] = (inst * 16u + (unsigned)(lane >> 2)) * B.ld + (unsigned)chunk * 16u;
+        else if (BKIND == 1) ob[j] = inst * B.ld + (unsigned)lane * 16u;
+        else ob[j] = inst / (BN / 32) * B.ld + inst % (BN / 32) * 1024u + (unsigned)lane * 16u;
     }
     // fragment offsets inside a stage
-    unsigned fa[2], ft[L::MT], fb[2];
-    if (AKIND == 0) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) fa[kk] = (unsigned)(wm + i16) * 128u + (unsigned)((kk * 4 + q) ^ (i16 >> 1)) * 16u;
-    } else {
+    unsigned fa, fb;
+    if (AKIND == 0) fa = (unsigned)(wm + i16) * 64u + (unsigned)(q ^ (i16 >> 2)) * 16u;
+    else {
         const int row = 4 * q + (i16 >> 2);
-#pragma unroll
-        for (int t = 0; t < L::MT; ++t)
-            ft[t] = (unsigned)row * 512u + (unsigned)(((wm >> 4) + t) ^ (row & 7)) * 32u + (unsigned)(i16 & 3) * 8u;
+        fa = (unsigned)row * 512u + (unsigned)((wm >> 4) ^ (row & 7)) * 32u + (unsigned)(i16 & 3) * 8u;
     }
-    if (BKIND == 0) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) fb[kk] = (unsigned)(wn + i16) * 128u + (unsigned)((kk * 4 + q) ^ (i16 >> 1)) * 16u;
-    } else if (BKIND == 1) fb[0] = (unsigned)(wn >> 4) * 2048u + (unsigned)(q * 16 + (i16 ^ (4 * q))) * 16u;
+    if (BKIND == 0) fb = (unsigned)(wn + i16) * 64u + (unsigned)(q ^ (i16 >> 2)) * 16u;
+    else if (BKIND == 1) fb = (unsigned)(wn >> 4) * 1024u + (unsigned)(q * 16 + (i16 ^ (4 * q))) * 16u;
     else {
         const int r = 4 * q + (i16 >> 2), qq = i16 & 3;
-        fb[0] = (unsigned)(wn >> 5) * 1024u + (unsigned)(qq * 16 + (r ^ (4 * qq))) * 16u;
+        fb = (unsigned)(wn >> 5) * 1024u + (unsigned)(qq * 16 + (r ^ (4 * qq))) * 16u;
     }
 
-    auto fetch = [&](int it, char* sa, char* sb) {
-        const int k = PARTS == 1 ? it : it / 6, s = PARTS == 1 ? 0 : it % 6;
-        const long long pa = PARTS == 1 ? 0 : part_a(s) * A.part, pb = PARTS == 1 ? 0 : part_b(s) * B.part;
-        const __amdgpu_buffer_rsrc_t ra = buffer(A.p + pa + k * A.step, A.left - k * A.step);
-        const __amdgpu_buffer_rsrc_t rb = buffer(B.p + pb + k * B.step, B.left - k * B.step);
+    const char *pa = A.p, *pb = B.p;                     // of the next step to be fetched
+    unsigned na = A.bytes, nb = B.bytes;
+    int kf = 0;
+    auto fetch = [&](int s, char* da, char* db) {        // parts pair s (PARTS 3; a constant where it is called)
+        const char* qa = PARTS == 1 || part_a(s) == 0 ? pa : pa + part_a(s) * A.part;
+        const char* qb = PARTS == 1 || part_b(s) == 0 ? pb : pb + part_b(s) * B.part;
+        const bool past = kf >= steps;
+        unsigned ra = na, rb = nb;
+        if (AKIND == 1 && kf >= A.full) ra = kf == A.full ? A.tail : 0;      // nothing behind the last row
+        if (past) ra = rb = 0;
+        ra = (unsigned)__builtin_amdgcn_readfirstlane((int)ra);    // (uniform as it is; this keeps the selects on the scalar side)
+        rb = (unsigned)__builtin_amdgcn_readfirstlane((int)rb);
+        const __amdgpu_buffer_rsrc_t va = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qa), 0, ra, BUF_FLAGS);
+        const __amdgpu_buffer_rsrc_t vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qb), 0, rb, BUF_FLAGS);
+        const bool in = AKIND != 0 || chunk * 8 < A.kmax - kf * BK;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            dma16(ra, sa + (wave * 4 + j) * 1024, AKIND == 0 && ca[j] >= A.kmax - k * BK ? NOWHERE : oa[j]);
+        for (int j = 0; j < L::NA; ++j) dma16(va, da + (wave * L::NA + j) * 1024, in ? oa[j] : NOWHERE);
 #pragma unroll
-        for (int j = 0; j < L::NB; ++j)
-            dma16(rb, sb + (wave * L::NB + j) * 1024, BKIND == 0 && cb[j] >= B.kmax - k * BK ? NOWHERE : ob[j]);
-    };
-    auto multiply = [&](int it, const char* sa, const char* sb) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            s16x8 a[L::MT], b[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                if (BKIND == 0) b[n] = *reinterpret_cast<const s16x8*>(sb + fb[kk] + n * 2048);
-                else if (BKIND == 1) b[n] = *reinterpret_cast<const s16x8*>(sb + fb[0] + n * 2048 + kk * 1024);
-                else {
-                    const char* p = sb + fb[0] + (n >> 1) * 1024 + (n & 1) * 8 + kk * 2 * (BN / 32) * 1024;
-                    b[n] = join(tr16(p), tr16(p + (BN / 32) * 1024));
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < L::MT; ++t) {
-                if (AKIND == 0) a[t] = *reinterpret_cast<const s16x8*>(sa + fa[kk] + t * 2048);
-                else a[t] = join(tr16(sa + ft[t] + kk * 16384), tr16(sa + ft[t] + kk * 16384 + 8192));
-            }
-#pragma unroll
-            for (int t = 0; t < L::MT; ++t)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) acc[t][n] = mfma<E>(a[t], b[n], acc[t][n]);
-            if (COLSUM && (PARTS == 1 || part_a(it % 6) == 0)) {
-                const short one = __builtin_bit_cast(short, (E)1.0f);
-                const s16x8 ones = {one, one, one, one, one, one, one, one};
-#pragma unroll
-                for (int n = 0; n < 4; ++n) cs[n] = mfma<E>(ones, b[n], cs[n]);
-            }
-            __builtin_amdgcn_sched_barrier(0);           // fragments of one half step at a time: 128 sums leave room for no more
+        for (int j = 0; j < L::NB; ++j) dma16(vb, db + (wave * L::NB + j) * 1024, ob[j]);
+        if (PARTS == 1 || s == 5) {
+            ++kf;
+            pa += A.step;
+            pb += B.step;
+            if (AKIND == 0) na -= BK * 2;
+            if (BKIND == 0) nb -= BK * 2;
         }
     };
-    auto arrive = [&]() {                                // own loads landed, own reads done; then everyone's
+    auto multiply = [&](int s, const char* da, const char* db) {
+        s16x8 a[L::MT], b[4];
+        if (AKIND == 1) asm volatile("" : "+v"(fa));     // (offsets of the tiles are made again, not kept: registers are short)
+        auto read_a = [&](int t) {
+            if (AKIND == 0) return *reinterpret_cast<const s16x8*>(da + fa + t * 1024);
+            const char* p = da + (fa ^ (unsigned)(t << 5));
+            return join(tr16(p), tr16(p + 8192));
+        };
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (BKIND == 0 || BKIND == 1) b[n] = *reinterpret_cast<const s16x8*>(db + fb + n * 1024);
+            else {
+                const char* p = db + fb + (n >> 1) * 1024 + (n & 1) * 8;
+                b[n] = join(tr16(p), tr16(p + (BN / 32) * 1024));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < AHEAD && t < L::MT; ++t) a[t] = read_a(t);
+#pragma unroll
+        for (int t = 0; t < L::MT; ++t) {
+            __builtin_amdgcn_sched_barrier(0);           // reads stay AHEAD tiles in front of the products
+            if (t + AHEAD < L::MT) a[t + AHEAD] = read_a(t + AHEAD);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) acc[t][n] = mfma<E>(a[t], b[n], acc[t][n]);
+        }
+        if (COLSUM && (PARTS == 1 || part_a(s) == 0)) {
+            const short one = __builtin_bit_cast(short, (E)1.0f);
+            const s16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) cs[n] = mfma<E>(ones, b[n], cs[n]);
+        }
+    };
+    // step `it`: its stage has landed for every wave (own loads but the next step's, then the barrier), every wave has read the
+    // stage of step it - 1 (reads done before the barrier): that one is filled again.  Loads behind the last step are issued
+    // like the others, from an empty buffer, so that waits are counted the same everywhere.
+    auto step = [&](int s, int stage) {                  // s: pair of parts
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_waitcnt(0x0070 | (L::NA + L::NB));      // vmcnt(the next step's), lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        fetch((s + 2) % 6, sa[(stage + 2) % STAGES], sb[(stage + 2) % STAGES]);
+        multiply(s, sa[stage], sb[stage]);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    const int n = steps * (PARTS == 1 ? 1 : 6);
-    if (n > 0) fetch(0, a0, b0);
-    int it = 0;
-    for (; it + 2 <= n; it += 2) {
-        arrive();
-        fetch(it + 1, a1, b1);
-        multiply(it, a0, b0);
-        arrive();
-        if (it + 2 < n) fetch(it + 2, a0, b0);
-        multiply(it + 1, a1, b1);
+    static_assert(STAGES == 3 && L::NA + L::NB < 16, "waits are counted for three stages");
+    if (steps <= 0) return;
+    fetch(0, sa[0], sb[0]);
+    fetch(1, sa[1], sb[1]);
+    if (PARTS == 1) {
+        for (int it = 0;;) {
+            step(0, 0);
+            if (++it >= steps) break;
+            step(0, 1);
+            if (++it >= steps) break;
+            step(0, 2);
+            if (++it >= steps) break;
+        }
+    } else {
+        for (int it = 0; it < steps; ++it) {
+            step(0, 0);
+            step(1, 1);
+            step(2, 2);
+            step(3, 0);
+            step(4, 1);
+            step(5, 2);
+        }
     }
-    if (it < n) {
-        arrive();
-        multiply(it, a0, b0);
-    }
+    __builtin_amdgcn_s_waitcnt(0x0070);                  // no load may be on its way into LDS that the workgroup gives back
+    asm volatile("" ::: "memory");
 }
 
 // position in the launch -> tile: consecutive workgroups go to the 8 XCDs in turn; each gets a run of consecutive tiles, so
@@ -243,9 +264,11 @@ struct LogitArgs {
 };
 
 template <typename E, int BN, int PARTS, bool GRAD>
-__global__ __launch_bounds__(512, 2) void xent_logit_kernel(LogitArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) {
     typedef Lay<BN> L;
-    __shared__ __attribute__((aligned(1024))) char sa0[BM * BK * 2], sa1[BM * BK * 2], sb0[BN * BK * 2], sb1[BN * BK * 2];
+    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
+    char* const sa[STAGES] = {a0, a1, a2};
+    char* const sb[STAGES] = {b0, b1, b2};
     __shared__ float2 red[L::WM][BN];
     const int tile = tile_of(a.nvt * a.nrt);
     if (tile < 0) return;
@@ -258,10 +281,12 @@ __global__ __launch_bounds__(512, 2) void xent_logit_kernel(LogitArgs a) {
 
     Operand A, B;
     A.p = a.w + v0 * a.ldw;
-    A.left = ((a.V - v0 < BM ? a.V - v0 : BM) - 1) * a.ldw + a.D * 2ll;
+    A.bytes = (unsigned)(((a.V - v0 < BM ? a.V - v0 : BM) - 1) * a.ldw + a.D * 2ll);
+    A.tail = 0; A.full = 0;
     A.step = BK * 2; A.part = a.w_part; A.ld = a.ldw; A.kmax = a.D;
     B.p = a.h + r0 * a.Dp * 2;
-    B.left = (long long)BN * a.Dp * 2;
+    B.bytes = (unsigned)BN * a.Dp * 2u;
+    B.tail = 0; B.full = 0;
     B.step = BK * 2; B.part = a.h_part; B.ld = (unsigned)a.Dp * 2u; B.kmax = a.Dp;
 
     f32x4 acc[L::MT][4], none[4];
@@ -269,7 +294,7 @@ __global__ __launch_bounds__(512, 2) void xent_logit_kernel(LogitArgs a) {
     for (int t = 0; t < L::MT; ++t)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, 0, 0, PARTS, false>(A, B, a.Dp / BK, sa0, sa1, sb0, sb1, acc, none);
+    core<E, BN, 0, 0, PARTS, false>(A, B, a.Dp / BK, sa, sb, acc, none);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -383,15 +408,18 @@ struct ProductArgs {
     void* out;                // [rows][ld_out] of the caller's type
     void* bout;
     const float* scale;       // fp16: scale[1] takes the scale of G out again (written only with the final result)
-    long long x_part, g_part, x_bytes, ld_out, slab_stride;
+    long long x_part, g_part, ld_out, slab_stride;
     unsigned ldx;
+    int x_rows, x_cols;       // rows of x, and the elements of a row that may be read
     int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
 };
 
 template <typename E, typename T, int BN, int PARTS, bool OVER_V>
-__global__ __launch_bounds__(512, 2) void xent_product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs a) {
     typedef Lay<BN> L;
-    __shared__ __attribute__((aligned(1024))) char sa0[BM * BK * 2], sa1[BM * BK * 2], sb0[BN * BK * 2], sb1[BN * BK * 2];
+    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
+    char* const sa[STAGES] = {a0, a1, a2};
+    char* const sb[STAGES] = {b0, b1, b2};
     const int tile = tile_of(a.ndt * a.nnt * a.splits);
     if (tile < 0) return;
     const int dt = tile % a.ndt, nt = tile / a.ndt % a.nnt, split = tile / (a.ndt * a.nnt);
@@ -399,18 +427,20 @@ __global__ __launch_bounds__(512, 2) void xent_product_kernel(ProductArgs a) {
 
     Operand A, B;
     A.ld = a.ldx; A.part = a.x_part; A.step = (long long)BK * a.ldx; A.kmax = 0;
-    const long long aoff = k0 * A.step + (long long)dt * BM * 2;
-    A.p = a.x + aoff;
-    A.left = a.x_bytes - aoff;
-    B.kmax = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
+    // rows k0 BK ... of x, columns from dt BM: whole steps of BK rows, then what is left of x's rows
+    A.p = a.x + k0 * A.step + (long long)dt * BM * 2;
+    A.full = a.x_rows / BK - k0;
+    A.bytes = (unsigned)(BK - 1) * a.ldx + (unsigned)(a.x_cols - dt * BM) * 2u;
+    A.tail = a.x_rows % BK ? (unsigned)(a.x_rows % BK - 1) * a.ldx + (unsigned)(a.x_cols - dt * BM) * 2u : 0;
+    B.kmax = 0; B.tail = 0; B.full = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
     if (OVER_V) {
-        B.step = 2048;
+        B.step = 1024;
         B.p = a.g + (long long)nt * (BN / 16) * B.ld + k0 * B.step;
-        B.left = (long long)(BN / 16) * B.ld;
+        B.bytes = (unsigned)(BN / 16 - 1) * B.ld + 1024u;
     } else {
-        B.step = 4ll * B.ld;
+        B.step = 2ll * B.ld;
         B.p = a.g + (long long)nt * (BN / 32) * 1024 + k0 * B.step;
-        B.left = (long long)(a.steps - k0) * B.step;
+        B.bytes = B.ld + (BN / 32) * 1024u;
     }
     f32x4 acc[L::MT][4], cs[4];
 #pragma unroll
@@ -419,7 +449,7 @@ __global__ __launch_bounds__(512, 2) void xent_product_kernel(ProductArgs a) {
         for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 4; ++n) cs[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, 1, OVER_V ? 1 : 2, PARTS, !OVER_V>(A, B, k1 - k0, sa0, sa1, sb0, sb1, acc, cs);
+    core<E, BN, 1, OVER_V ? 1 : 2, PARTS, !OVER_V>(A, B, k1 - k0, sa, sb, acc, cs);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -635,7 +665,7 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restric
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 constexpr long long PIECE_BYTES = 512ll << 20;           // what G of one piece may take
-constexpr int CUS = 256;
+constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
     int parts, Rp, Vp, Dp, BN, nrt, nvt, copy_w, pieces, piece_tiles, dh_splits, dw_splits, ndt;
@@ -648,7 +678,7 @@ inline int pick_splits(long long tiles, int steps, long long slab_bytes) {
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
-        const double cost = (double)((tiles * s + CUS - 1) / CUS) * ((steps + s - 1) / s + 3) + (s > 1 ? 2.0 * s * slab_bytes / 4e6 + 4 : 0);
+        const double cost = (double)((tiles * s + SLOTS - 1) / SLOTS) * ((steps + s - 1) / s + 3) + (s > 1 ? 2.0 * s * slab_bytes / 4e6 + 4 : 0);
         if (cost < least * 0.98) { least = cost; best = s; }
     }
     return best;
@@ -659,10 +689,10 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     SV_CHECK_ARG(R > 0 && R <= 1 << 24 && V > 0 && V <= 1 << 28 && D > 0 && D <= 1 << 16 && ld_w >= D && ld_w <= 1 << 20,
                  "svae_xent: sizes R %lld, V %lld, D %lld, ld %lld", R, V, D, ld_w);
     s->parts = type == SV_F32 ? 3 : 1;
-    s->BN = R <= 64 ? 64 : 256;
+    s->BN = R <= 64 ? 64 : 128;
     s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
     s->Vp = (int)((V + BM - 1) / BM * BM);
-    s->Dp = (int)((D + BK - 1) / BK * BK);
+    s->Dp = (int)((D + KPAD - 1) / KPAD * KPAD);
     s->nrt = s->Rp / s->BN;
     s->nvt = s->Vp / BM;
     s->ndt = (s->Dp + BM - 1) / BM;
@@ -695,7 +725,7 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         s->g = take(s->g_part * s->parts);
         s->dh_splits = pick_splits((long long)s->ndt * s->nrt, s->piece_tiles * (BM / BK) * (s->parts == 1 ? 1 : 6), 4ll * s->Rp * s->Dp);
         s->dh_slab = take(4ll * s->Rp * s->Dp * s->dh_splits);
-        s->dw_splits = pick_splits((long long)s->ndt * s->piece_tiles, s->Rp / BK * (s->parts == 1 ? 1 : 6), 4ll * s->piece_tiles * BM * s->Dp);
+        s->dw_splits = pick_splits((long long)s->ndt * s->piece_tiles * (BM / 128), s->Rp / BK * (s->parts == 1 ? 1 : 6), 4ll * s->piece_tiles * BM * s->Dp);
         s->dw_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->Dp * s->dw_splits : 0);
         s->db_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->dw_splits : 0);
     }
@@ -757,8 +787,8 @@ inline void logits(const Call& c, const Shape& s, const LogitArgs& a) {
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
         const dim3 grid(launch_for((long long)a.nvt * a.nrt));
-        if (s.BN == 64) hipLaunchKernelGGL((xent_logit_kernel<E, 64, P, GRAD>), grid, dim3(512), 0, c.stream, a);
-        else hipLaunchKernelGGL((xent_logit_kernel<E, 256, P, GRAD>), grid, dim3(512), 0, c.stream, a);
+        if (s.BN == 64) hipLaunchKernelGGL((xent_logit_kernel<E, 64, P, GRAD>), grid, dim3(64 * WAVES), 0, c.stream, a);
+        else hipLaunchKernelGGL((xent_logit_kernel<E, 128, P, GRAD>), grid, dim3(64 * WAVES), 0, c.stream, a);
     });
 }
 
@@ -849,7 +879,7 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
         d.g = a.g; d.scale = scale; d.g_part = s.g_part; d.D = D; d.Dp = s.Dp; d.ndt = s.ndt; d.nv32 = nt * (BM / 32);
         if (dh) {
             d.x = a.w + v0 * s.ldw;
-            d.x_bytes = (rows_v - 1) * s.ldw + (s.copy_w ? s.Dp : D) * 2ll;
+            d.x_rows = rows_v; d.x_cols = s.copy_w ? s.Dp : D;
             d.x_part = s.w_part; d.ldx = (unsigned)s.ldw;
             d.slab = (float*)(c.work + s.dh_slab); d.slab_stride = (long long)s.Rp * s.Dp;
             d.rows = s.Rp; d.nnt = s.nrt; d.splits = s.dh_splits; d.steps = nt * (BM / BK); d.add = p > 0;
@@ -858,14 +888,14 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
                 typedef decltype(e) E;
                 constexpr int P = decltype(parts)::value;
                 const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
-                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(512), 0, c.stream, d);
-                else hipLaunchKernelGGL((xent_product_kernel<E, T, 256, P, true>), grid, dim3(512), 0, c.stream, d);
+                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(64 * WAVES), 0, c.stream, d);
+                else hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, true>), grid, dim3(64 * WAVES), 0, c.stream, d);
             });
             SV_LAUNCH_CHECK();
         }
         if (dw) {
-            d.x = a.h; d.x_bytes = s.h_part; d.x_part = s.h_part; d.ldx = (unsigned)s.Dp * 2u;
-            d.rows = rows_v; d.nnt = nt; d.splits = s.dw_splits; d.steps = s.Rp / BK; d.add = 0;
+            d.x = a.h; d.x_rows = s.Rp; d.x_cols = s.Dp; d.x_part = s.h_part; d.ldx = (unsigned)s.Dp * 2u;
+            d.rows = rows_v; d.nnt = nt * (BM / 128); d.splits = s.dw_splits; d.steps = s.Rp / BK; d.add = 0;
             d.out = (char*)dw + v0 * ld_dw * es; d.ld_out = ld_dw;
             d.bout = db ? (char*)db + v0 * es : nullptr;
             d.slab = s.dw_splits > 1 ? (float*)(c.work + s.dw_slab) : nullptr;
@@ -877,7 +907,7 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
                 typedef decltype(t) T;
                 typedef decltype(e) E;
                 constexpr int P = decltype(parts)::value;
-                hipLaunchKernelGGL((xent_product_kernel<E, T, 256, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(512), 0, c.stream, d);
+                hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(64 * WAVES), 0, c.stream, d);
                 if (d.slab != nullptr) {
                     const unsigned nmain = (unsigned)(((long long)rows_v * (s.Dp / 4) + 255) / 256), nbias = db ? (rows_v + 255) / 256 : 0;
                     hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain + nbias), dim3(256), 0, c.stream, d.slab, d.slab_stride, d.splits, rows_v, D,
