@@ -14,9 +14,9 @@
 // while the other waits at its barrier, reads fragments or works through an epilogue.
 //   z^T tile: A = W rows, B = H rows, both with the contraction contiguous.  C has the row of H in the lane and four vocabulary
 //     entries in registers, so a row's maximum and sum are mostly in-lane work.
-//   G is kept as blocks of 16 rows x 32 vocabulary entries, 1 KiB: a lane's 16 bytes are the 8 values that it made, which are a
-//     B fragment of G W as they stand if W's rows are taken in the same order (16 (j / 4) + 4 (lane / 16) + j % 4), and that is
-//     the order in which transposing LDS reads deliver W.  For G^T H the same blocks are read with transposing LDS reads.
+//   G is kept as blocks of 16 rows x 32 vocabulary entries, 1 KiB: the 8 values that a lane makes are its part of a B fragment
+//     of G W as they stand if W's rows are taken in the same order (16 (j / 4) + 4 (lane / 16) + j % 4), and that is the order in
+//     which transposing LDS reads deliver W.  For G^T H the same blocks are read with transposing LDS reads.
 //
 // Types: bf16 and fp16 go to the matrix units as they are; G is rounded to the inputs' type (relative 2^-8 / 2^-11 of each
 // term, as the inputs themselves are), for fp16 after scaling by a power of two that puts the largest row weight near 2^14, so
@@ -70,12 +70,19 @@ __device__ __forceinline__ constexpr int part_b(int s) { return (0x010120 >> (4 
 //   AKIND 0: A [m][k], k contiguous (rows lda bytes apart)      LDS image [256 m][32 k]
 //   AKIND 1: A [k][m], m contiguous                             LDS image [32 k][256 m], read transposed
 //   BKIND 0: B [n][k] like A      BKIND 1: blocks of G, contraction over the vocabulary      BKIND 2: over the rows
-// LDS images hold 16-byte chunks; which chunk a lane fetches is permuted so that the 16 lanes that a read serves at a time
-// fall on different banks: [.][32] images: chunk c of row r at c ^ ((r / 4) % 4); [.][256]: pairs of chunks, c ^ 2 (r % 8).
+// LDS images hold 16-byte chunks; which chunk a lane fetches is permuted so that the lanes that a read serves in one cycle fall
+// on different banks.  A 16-byte read serves lanes 0-3, 12-15, 20-27 together (then 4-11, 16-19, 28-31, and so on), an 8-byte
+// one 32 lanes in a row (measured: 4 and 2 cycles a wave without conflicts, twice that where only 16 lanes in a row are kept
+// apart).  [.][32] images: chunk c of row r at c ^ (-(r / 4) % 4); [.][256] images: pairs of chunks, c ^ 2 (r % 8).
 // PARTS 3: every step runs over the six pairs of parts; the parts of an operand lie apart by a_part / b_part bytes.
 // ------------------------------------------------------------------------------------------------
 // What LDS-DMA may read from an operand at contraction step k is [p + k step, + bytes).  Kind 1: whole steps all have `bytes`,
 // step `full` has `tail` (rows that end inside it), later ones nothing.  Kind 0 loses `step` bytes a step, as p moves along its rows.
+//
+// A block of G, 16 rows x 32 vocabulary entries: two halves of 16 entries, 512 bytes each, row r at 32 r, its four entries from
+// 4 q on at chunk q ^ 2 (r / 8) of 8 bytes: both ways of reading it take the 2 cycles.
+__device__ __forceinline__ unsigned g_offset(int r, int q) { return (unsigned)(r * 32 + (q ^ ((r >> 3) << 1)) * 8); }
+
 struct Operand {
     const char* p;        // first row, contraction step 0 of the tile
     long long step;       // bytes from one step to the next
@@ -105,7 +112,7 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
 
     // LDS-DMA: every instruction fills 1 KiB
     //   kind 0: 16 rows of 4 chunks      kind 1: 2 rows of 32 chunks      blocks of G: one block
-    const int chunk = (lane & 3) ^ q;                    // kind 0: chunk (lane % 4) ^ ((row / 4) % 4), row = lane / 4
+    const int chunk = (lane & 3) ^ (-q & 3);             // kind 0: chunk (lane % 4) ^ (-(row / 4) % 4), row = lane / 4
     unsigned oa[L::NA], ob[L::NB];
 #pragma unroll
     for (int j = 0; j < L::NA; ++j) {
@@ -125,16 +132,15 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
     }
     // fragment offsets inside a stage
     unsigned fa, fb;
-    if (AKIND == 0) fa = (unsigned)(wm + i16) * 64u + (unsigned)(q ^ (i16 >> 2)) * 16u;
+    if (AKIND == 0) fa = (unsigned)(wm + i16) * 64u + (unsigned)(q ^ (-(i16 >> 2) & 3)) * 16u;
     else {
         const int row = 4 * q + (i16 >> 2);
         fa = (unsigned)row * 512u + (unsigned)((wm >> 4) ^ (row & 7)) * 32u + (unsigned)(i16 & 3) * 8u;
     }
-    if (BKIND == 0) fb = (unsigned)(wn + i16) * 64u + (unsigned)(q ^ (i16 >> 2)) * 16u;
-    else if (BKIND == 1) fb = (unsigned)(wn >> 4) * 1024u + (unsigned)(q * 16 + (i16 ^ (4 * q))) * 16u;
+    if (BKIND == 0) fb = (unsigned)(wn + i16) * 64u + (unsigned)(q ^ (-(i16 >> 2) & 3)) * 16u;
+    else if (BKIND == 1) fb = (unsigned)(wn >> 4) * 1024u + g_offset(i16, q);
     else {
-        const int r = 4 * q + (i16 >> 2), qq = i16 & 3;
-        fb = (unsigned)(wn >> 5) * 1024u + (unsigned)(qq * 16 + (r ^ (4 * qq))) * 16u;
+        fb = (unsigned)(wn >> 5) * 1024u + g_offset(4 * q + (i16 >> 2), i16 & 3);
     }
 
     const char *pa = A.p, *pb = B.p;                     // of the next step to be fetched
@@ -174,9 +180,12 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
         };
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            if (BKIND == 0 || BKIND == 1) b[n] = *reinterpret_cast<const s16x8*>(db + fb + n * 1024);
-            else {
-                const char* p = db + fb + (n >> 1) * 1024 + (n & 1) * 8;
+            if (BKIND == 0) b[n] = *reinterpret_cast<const s16x8*>(db + fb + n * 1024);
+            else if (BKIND == 1) {
+                const char* p = db + fb + n * 1024;
+                b[n] = join(*reinterpret_cast<const s16x4*>(p), *reinterpret_cast<const s16x4*>(p + 512));
+            } else {
+                const char* p = db + fb + (n >> 1) * 1024 + (n & 1) * 512;
                 b[n] = join(tr16(p), tr16(p + (BN / 32) * 1024));
             }
         }
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
             const long long r = r0 + wn + 16 * n + i16;
             const float w = a.wrow[r] * up, lse = a.lse[r];
             const int tg = a.tgt[r];
-            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + (q * 16 + (i16 ^ (4 * q))) * 16;
+            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + g_offset(i16, q);
 #pragma unroll
             for (int t = 0; t < L::MT; t += 2) {
                 float g[8];
@@ -380,14 +389,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
                 char* to = dst + (t >> 1) * 1024;
 #pragma unroll
                 for (int s = 0; s < PARTS; ++s) {
-                    s16x8 out;
+                    s16x4 out[2];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const E e = (E)g[j];
-                        out[j] = __builtin_bit_cast(short, e);
+                        out[j >> 2][j & 3] = __builtin_bit_cast(short, e);
                         g[j] -= (float)e;
                     }
-                    *reinterpret_cast<s16x8*>(to + s * a.g_part) = out;
+                    *reinterpret_cast<s16x4*>(to + s * a.g_part) = out[0];
+                    *reinterpret_cast<s16x4*>(to + s * a.g_part + 512) = out[1];
                 }
             }
         }
