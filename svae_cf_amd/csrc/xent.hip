@@ -8,15 +8,16 @@
 // piece is written to the workspace, then two products take it up.  Everything is bound by the matrix units (6 R V D flops for
 // loss and gradient and 2 R V D for making z again), except that few rows leave the loss bound by reading W.
 //
-// All products run on one core: 256 x 128 (or 256 x 64) outputs a workgroup of 4 waves, steps of 32 along the contraction, three
-// stages of LDS filled by LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from
-// writes to the other and does not wait for the prefetch), v_mfma_f32_16x16x32.  Two workgroups share a CU: one multiplies
-// while the other waits at its barrier, reads fragments or works through an epilogue.
-//   z^T tile: A = W rows, B = H rows, both with the contraction contiguous.  C has the row of H in the lane and four vocabulary
-//     entries in registers, so a row's maximum and sum are mostly in-lane work.
-//   G is kept as blocks of 16 rows x 32 vocabulary entries, 1 KiB: the 8 values that a lane makes are its part of a B fragment
-//     of G W as they stand if W's rows are taken in the same order (16 (j / 4) + 4 (lane / 16) + j % 4), and that is the order in
-//     which transposing LDS reads deliver W.  For G^T H the same blocks are read with transposing LDS reads.
+// All products run on one core: 256 x BN outputs a workgroup, steps of 32 along the contraction, three stages of LDS filled by
+// LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from writes to the other and
+// does not wait for the prefetch), v_mfma_f32_16x16x32, a wave makes 128 x 64.
+//   H, W and G are kept as blocks of 16 rows x 32 columns, 1 KiB: LDS-DMA fetches whole blocks (of W's own rows it would fetch
+//     64-byte pieces, at half the rate), and a block can be the operand of a contraction along its columns as it stands or of one
+//     over its rows with transposing LDS reads, without bank conflicts either way.
+//   z^T tile: A = W, B = H, both along the columns.  C has the row of H in the lane and four vocabulary entries in registers, so
+//     a row's maximum and sum are mostly in-lane work, and the eight values of G that a lane makes are two pieces of a block.
+//   G W: A = W over its rows, B = G along its columns.  G^T H: A = H, B = G, both over their rows.
+// Few rows and no gradient: W is read once, as it lies (16-bit types, aligned rows); that is bound by HBM.
 //
 // Types: bf16 and fp16 go to the matrix units as they are; G is rounded to the inputs' type (relative 2^-8 / 2^-11 of each
 // term, as the inputs themselves are), for fp16 after scaling by a power of two that puts the largest row weight near 2^14, so
@@ -35,12 +36,10 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 constexpr int BM = 256;                   // outputs of a workgroup along A
 constexpr int BK = 32;                    // contraction of a step
 constexpr int STAGES = 3;
-constexpr int WAVES = 4;
 constexpr int AHEAD = 4;                  // fragments of A that are read in front of their products
-constexpr int KPAD = 64;                  // the copies' row length is a multiple of this
 constexpr unsigned BUF_FLAGS = 0x00020000u;
 constexpr unsigned NOWHERE = 0xFFFFFFF0u; // past every buffer's end: such a lane loads zeros
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 template <typename E>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c);
@@ -67,39 +66,75 @@ __device__ __forceinline__ constexpr int part_b(int s) { return (0x010120 >> (4 
 
 // ------------------------------------------------------------------------------------------------
 // The core: acc[t][n] (16 x 16 each; A side t, B side n) += A B over `steps` steps of 32.
-//   AKIND 0: A [m][k], k contiguous (rows lda bytes apart)      LDS image [256 m][32 k]
-//   AKIND 1: A [k][m], m contiguous                             LDS image [32 k][256 m], read transposed
-//   BKIND 0: B [n][k] like A      BKIND 1: blocks of G, contraction over the vocabulary      BKIND 2: over the rows
-// LDS images hold 16-byte chunks; which chunk a lane fetches is permuted so that the lanes that a read serves in one cycle fall
-// on different banks.  A 16-byte read serves lanes 0-3, 12-15, 20-27 together (then 4-11, 16-19, 28-31, and so on), an 8-byte
-// one 32 lanes in a row (measured: 4 and 2 cycles a wave without conflicts, twice that where only 16 lanes in a row are kept
-// apart).  [.][32] images: chunk c of row r at c ^ (-(r / 4) % 4); [.][256] images: pairs of chunks, c ^ 2 (r % 8).
-// PARTS 3: every step runs over the six pairs of parts; the parts of an operand lie apart by a_part / b_part bytes.
+//   PLAIN   rows as they lie, contraction along them; LDS image [rows][32], 16-byte chunk c of row r at c ^ (-(r / 4) % 4)
+//   ALONG   blocks, contraction along their columns      ACROSS   blocks, contraction over their rows
+// An 8-byte LDS read serves 32 lanes in a row in a cycle; the images keep those on different banks (a wave's read takes 2 cycles).
+// PARTS 3: every step runs over the six pairs of parts; the parts of an operand lie `part` bytes apart.
 // ------------------------------------------------------------------------------------------------
-// What LDS-DMA may read from an operand at contraction step k is [p + k step, + bytes).  Kind 1: whole steps all have `bytes`,
-// step `full` has `tail` (rows that end inside it), later ones nothing.  Kind 0 loses `step` bytes a step, as p moves along its rows.
-//
-// A block of G, 16 rows x 32 vocabulary entries: two halves of 16 entries, 512 bytes each, row r at 32 r, its four entries from
-// 4 q on at chunk q ^ 2 (r / 8) of 8 bytes: both ways of reading it take the 2 cycles.
-__device__ __forceinline__ unsigned g_offset(int r, int q) { return (unsigned)(r * 32 + (q ^ ((r >> 3) << 1)) * 8); }
+enum { PLAIN, ALONG, ACROSS };
+
+// A block of 16 rows x 32 columns: two halves of 16 columns, 512 bytes each; row r at 32 r, its four entries from column 4 q of
+// the half on at chunk q ^ 2 (r / 8) of 8 bytes.
+__device__ __forceinline__ unsigned in_block(int r, int q) { return (unsigned)(r * 32 + (q ^ ((r >> 3) << 1)) * 8); }
 
 struct Operand {
-    const char* p;        // first row, contraction step 0 of the tile
+    const char* p;        // step 0 of the tile
     long long step;       // bytes from one step to the next
     long long part;       // bytes from one part to the next
-    unsigned bytes, tail;
-    int full;
-    unsigned ld;          // bytes between rows (BKIND 1, 2: between the blocks of one and the next 16 rows)
-    int kmax;             // AKIND 0: length of a row in elements; chunks behind it are loaded as zeros
+    unsigned bytes;       // what a step may read, from its p on (PLAIN: from step 0's p on)
+    unsigned ld;          // bytes between rows (PLAIN) or between the blocks of one and the next 16 rows
+    int kmax;             // PLAIN: length of a row in elements; chunks behind it are loaded as zeros
 };
 
 template <int BN>
 struct Lay {
+    static constexpr int WAVES = BN == 256 ? 8 : 4;
     static constexpr int WN = BN / 64;                  // waves along B, 64 outputs each
     static constexpr int WM = WAVES / WN;               // waves along A
     static constexpr int MT = BM / WM / 16;             // 16-wide tiles of a wave along A
     static constexpr int NA = BM * BK * 2 / 1024 / WAVES, NB = BN * BK * 2 / 1024 / WAVES;     // LDS-DMA instructions of a wave and step
 };
+
+// lane offset of LDS-DMA instruction `inst` (it fills 1 KiB: 16 rows of 4 chunks, or one block) of a tile of W rows or columns
+template <int KIND, int W>
+__device__ __forceinline__ unsigned dma_offset(unsigned inst, int lane, unsigned ld) {
+    if (KIND == PLAIN) return (inst * 16u + (unsigned)(lane >> 2)) * ld + (unsigned)((lane & 3) ^ (-(lane >> 4) & 3)) * 16u;
+    if (KIND == ALONG) return inst * ld + (unsigned)lane * 16u;
+    return inst / (W / 32) * ld + inst % (W / 32) * 1024u + (unsigned)lane * 16u;
+}
+// fragment j (16 rows or columns from w0 + 16 j on) of a stage
+struct Frag {
+    unsigned lo, hi;
+};
+template <int KIND, int W>
+__device__ __forceinline__ Frag frag_offset(int w0, int lane) {
+    const int i16 = lane & 15, q = lane >> 4;
+    Frag f;
+    if (KIND == PLAIN) {
+        const unsigned row = (unsigned)(w0 + i16) * 64u, sw = (unsigned)(-(i16 >> 2) & 3), at = (unsigned)(q & 1) * 8u;
+        f.lo = row + ((unsigned)(q >> 1) ^ sw) * 16u + at;
+        f.hi = row + ((unsigned)(2 + (q >> 1)) ^ sw) * 16u + at;
+    } else if (KIND == ALONG) {
+        f.lo = (unsigned)(w0 >> 4) * 1024u + in_block(i16, q);
+        f.hi = f.lo + 512u;
+    } else {
+        f.lo = (unsigned)(w0 >> 5) * 1024u + in_block(4 * q + (i16 >> 2), i16 & 3);
+        f.hi = f.lo + (W / 32) * 1024u;
+    }
+    return f;
+}
+// entries 4 q ... and 16 + 4 q ... of the contraction's 32, whatever the kind
+template <int KIND>
+__device__ __forceinline__ s16x8 read_frag(const char* stage, const Frag& f, int j) {
+    if (KIND == ACROSS) {
+        const unsigned o = (unsigned)((j >> 1) * 1024 + (j & 1) * 512);
+        return join(tr16(stage + f.lo + o), tr16(stage + f.hi + o));
+    }
+    // (volatile: else the compiler makes one ds_read2_b64 of two reads, which takes 12 cycles instead of 2 x 2)
+    typedef const volatile __attribute__((address_space(3))) s16x4* P;
+    const s16x4 lo = *(P)(stage + f.lo + j * 1024), hi = *(P)(stage + f.hi + j * 1024);
+    return join(lo, hi);
+}
 
 template <typename E, int BN, int AKIND, int BKIND, int PARTS, bool COLSUM>
 __device__ __forceinline__ void core(const Operand& A, const Operand& B, int steps, char* const (&sa)[STAGES], char* const (&sb)[STAGES],
@@ -107,57 +142,26 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
     typedef Lay<BN> L;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
-    const int i16 = lane & 15, q = lane >> 4;
-
-    // LDS-DMA: every instruction fills 1 KiB
-    //   kind 0: 16 rows of 4 chunks      kind 1: 2 rows of 32 chunks      blocks of G: one block
-    const int chunk = (lane & 3) ^ (-q & 3);             // kind 0: chunk (lane % 4) ^ (-(row / 4) % 4), row = lane / 4
     unsigned oa[L::NA], ob[L::NB];
 #pragma unroll
-    for (int j = 0; j < L::NA; ++j) {
-        const unsigned inst = (unsigned)(wave * L::NA + j);
-        if (AKIND == 0) oa[j] = (inst * 16u + (unsigned)(lane >> 2)) * A.ld + (unsigned)chunk * 16u;
-        else {
-            const unsigned row = inst * 2u + (unsigned)(lane >> 5);
-            oa[j] = row * A.ld + (((unsigned)lane & 31u) ^ ((row & 7u) << 1)) * 16u;
-        }
-    }
+    for (int j = 0; j < L::NA; ++j) oa[j] = dma_offset<AKIND, BM>((unsigned)(wave * L::NA + j), lane, A.ld);
 #pragma unroll
-    for (int j = 0; j < L::NB; ++j) {
-        const unsigned inst = (unsigned)(wave * L::NB + j);
-        if (BKIND == 0) ob[j] = (inst * 16u + (unsigned)(lane >> 2)) * B.ld + (unsigned)chunk * 16u;
-        else if (BKIND == 1) ob[j] = inst * B.ld + (unsigned)lane * 16u;
-        else ob[j] = inst / (BN / 32) * B.ld + inst % (BN / 32) * 1024u + (unsigned)lane * 16u;
-    }
-    // fragment offsets inside a stage
-    unsigned fa, fb;
-    if (AKIND == 0) fa = (unsigned)(wm + i16) * 64u + (unsigned)(q ^ (-(i16 >> 2) & 3)) * 16u;
-    else {
-        const int row = 4 * q + (i16 >> 2);
-        fa = (unsigned)row * 512u + (unsigned)((wm >> 4) ^ (row & 7)) * 32u + (unsigned)(i16 & 3) * 8u;
-    }
-    if (BKIND == 0) fb = (unsigned)(wn + i16) * 64u + (unsigned)(q ^ (-(i16 >> 2) & 3)) * 16u;
-    else if (BKIND == 1) fb = (unsigned)(wn >> 4) * 1024u + g_offset(i16, q);
-    else {
-        fb = (unsigned)(wn >> 5) * 1024u + g_offset(4 * q + (i16 >> 2), i16 & 3);
-    }
+    for (int j = 0; j < L::NB; ++j) ob[j] = dma_offset<BKIND, BN>((unsigned)(wave * L::NB + j), lane, B.ld);
+    const Frag fa = frag_offset<AKIND, BM>((wave / L::WN) * (16 * L::MT), lane), fb = frag_offset<BKIND, BN>((wave % L::WN) * 64, lane);
+    const int chunk = ((lane & 3) ^ (-(lane >> 4) & 3)) * 8;         // PLAIN: first element of the lane's chunk
 
     const char *pa = A.p, *pb = B.p;                     // of the next step to be fetched
     unsigned na = A.bytes, nb = B.bytes;
     int kf = 0;
-    auto fetch = [&](int s, char* da, char* db) {        // parts pair s (PARTS 3; a constant where it is called)
+    auto fetch = [&](int s, char* da, char* db) {        // pair of parts s (PARTS 3; a constant where it is called)
         const char* qa = PARTS == 1 || part_a(s) == 0 ? pa : pa + part_a(s) * A.part;
         const char* qb = PARTS == 1 || part_b(s) == 0 ? pb : pb + part_b(s) * B.part;
-        const bool past = kf >= steps;
-        unsigned ra = na, rb = nb;
-        if (AKIND == 1 && kf >= A.full) ra = kf == A.full ? A.tail : 0;      // nothing behind the last row
-        if (past) ra = rb = 0;
-        ra = (unsigned)__builtin_amdgcn_readfirstlane((int)ra);    // (uniform as it is; this keeps the selects on the scalar side)
-        rb = (unsigned)__builtin_amdgcn_readfirstlane((int)rb);
+        // (uniform as they are; readfirstlane keeps the selects on the scalar side)
+        const unsigned ra = (unsigned)__builtin_amdgcn_readfirstlane((int)(kf >= steps ? 0u : na));
+        const unsigned rb = (unsigned)__builtin_amdgcn_readfirstlane((int)(kf >= steps ? 0u : nb));
         const __amdgpu_buffer_rsrc_t va = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qa), 0, ra, BUF_FLAGS);
         const __amdgpu_buffer_rsrc_t vb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qb), 0, rb, BUF_FLAGS);
-        const bool in = AKIND != 0 || chunk * 8 < A.kmax - kf * BK;
+        const bool in = AKIND != PLAIN || chunk < A.kmax - kf * BK;
 #pragma unroll
         for (int j = 0; j < L::NA; ++j) dma16(va, da + (wave * L::NA + j) * 1024, in ? oa[j] : NOWHERE);
 #pragma unroll
@@ -166,35 +170,20 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
             ++kf;
             pa += A.step;
             pb += B.step;
-            if (AKIND == 0) na -= BK * 2;
-            if (BKIND == 0) nb -= BK * 2;
+            if (AKIND == PLAIN) na -= BK * 2;
+            if (BKIND == PLAIN) nb -= BK * 2;
         }
     };
     auto multiply = [&](int s, const char* da, const char* db) {
         s16x8 a[L::MT], b[4];
-        if (AKIND == 1) asm volatile("" : "+v"(fa));     // (offsets of the tiles are made again, not kept: registers are short)
-        auto read_a = [&](int t) {
-            if (AKIND == 0) return *reinterpret_cast<const s16x8*>(da + fa + t * 1024);
-            const char* p = da + (fa ^ (unsigned)(t << 5));
-            return join(tr16(p), tr16(p + 8192));
-        };
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            if (BKIND == 0) b[n] = *reinterpret_cast<const s16x8*>(db + fb + n * 1024);
-            else if (BKIND == 1) {
-                const char* p = db + fb + n * 1024;
-                b[n] = join(*reinterpret_cast<const s16x4*>(p), *reinterpret_cast<const s16x4*>(p + 512));
-            } else {
-                const char* p = db + fb + (n >> 1) * 1024 + (n & 1) * 512;
-                b[n] = join(tr16(p), tr16(p + (BN / 32) * 1024));
-            }
-        }
+        for (int n = 0; n < 4; ++n) b[n] = read_frag<BKIND>(db, fb, n);
 #pragma unroll
-        for (int t = 0; t < AHEAD && t < L::MT; ++t) a[t] = read_a(t);
+        for (int t = 0; t < AHEAD && t < L::MT; ++t) a[t] = read_frag<AKIND>(da, fa, t);
 #pragma unroll
         for (int t = 0; t < L::MT; ++t) {
             __builtin_amdgcn_sched_barrier(0);           // reads stay AHEAD tiles in front of the products
-            if (t + AHEAD < L::MT) a[t + AHEAD] = read_a(t + AHEAD);
+            if (t + AHEAD < L::MT) a[t + AHEAD] = read_frag<AKIND>(da, fa, t + AHEAD);
 #pragma unroll
             for (int n = 0; n < 4; ++n) acc[t][n] = mfma<E>(a[t], b[n], acc[t][n]);
         }
@@ -205,8 +194,8 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
             for (int n = 0; n < 4; ++n) cs[n] = mfma<E>(ones, b[n], cs[n]);
         }
     };
-    // step `it`: its stage has landed for every wave (own loads but the next step's, then the barrier), every wave has read the
-    // stage of step it - 1 (reads done before the barrier): that one is filled again.  Loads behind the last step are issued
+    // A step: its stage has landed for every wave (own loads but the next step's, then the barrier), every wave has read the
+    // stage of the step before (reads done before the barrier): that one is filled again.  Loads behind the last step are issued
     // like the others, from an empty buffer, so that waits are counted the same everywhere.
     auto step = [&](int s, int stage) {                  // s: pair of parts
         asm volatile("" ::: "memory");
@@ -257,13 +246,13 @@ inline unsigned launch_for(long long tiles) { return (unsigned)((tiles + 7) / 8 
 // z^T tiles: loss statistics (GRAD = false) or blocks of G (GRAD = true)
 // ------------------------------------------------------------------------------------------------
 struct LogitArgs {
-    const char* w;            // W, ldw bytes a row, parts w_part bytes apart
-    const char* h;            // copy of H, [Rp][Dp], parts h_part bytes apart
-    const float* bias;        // [Vp], -inf behind V
+    const char* w;            // W: its rows, ldw bytes apart (PLAIN), or blocks
+    const char* h;            // copy of H: rows of Dp elements (PLAIN) or blocks
+    const float* bias;        // [Vp] in units of log 2, -inf behind V
     const int* tgt;           // [Rp], -1: left out
-    float2* part;             // loss: [vocabulary tiles][Rp] (maximum, sum of exponentials)
-    float* zt;                // loss: [Rp] the target's logit
-    const float* lse;         // gradient
+    float2* part;             // loss: [vocabulary tiles][Rp] (maximum in units of log 2, sum of exponentials)
+    float* zt;                // loss: [Rp] the target's logit in units of log 2
+    const float* lse;         // gradient: [Rp]
     const float* wrow;        // gradient: [Rp], 0 for rows without a part in it
     const float* scale;       // gradient, fp16: the scale of G, or NULL
     char* g;                  // gradient: blocks of G, [Rp / 16][vocabulary tiles * 8], parts g_part bytes apart
@@ -272,8 +261,8 @@ struct LogitArgs {
     int V, D, Dp, Rp, v_begin, nvt, nrt;      // vocabulary of this launch: tiles v_begin / 256 ..., nvt of them
 };
 
-template <typename E, int BN, int PARTS, bool GRAD>
-__global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) {
+template <typename E, int BN, int KIND, int PARTS, bool GRAD>
+__global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(LogitArgs a) {
     typedef Lay<BN> L;
     __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
     char* const sa[STAGES] = {a0, a1, a2};
@@ -289,21 +278,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
     const long long r0 = (long long)rt * BN;
 
     Operand A, B;
-    A.p = a.w + v0 * a.ldw;
-    A.bytes = (unsigned)(((a.V - v0 < BM ? a.V - v0 : BM) - 1) * a.ldw + a.D * 2ll);
-    A.tail = 0; A.full = 0;
-    A.step = BK * 2; A.part = a.w_part; A.ld = a.ldw; A.kmax = a.D;
-    B.p = a.h + r0 * a.Dp * 2;
-    B.bytes = (unsigned)BN * a.Dp * 2u;
-    B.tail = 0; B.full = 0;
-    B.step = BK * 2; B.part = a.h_part; B.ld = (unsigned)a.Dp * 2u; B.kmax = a.Dp;
+    if (KIND == PLAIN) {
+        A.p = a.w + v0 * a.ldw;
+        A.bytes = (unsigned)(((a.V - v0 < BM ? a.V - v0 : BM) - 1) * a.ldw + a.D * 2ll);
+        A.step = B.step = BK * 2;
+        A.ld = a.ldw;
+        A.kmax = a.D;
+        B.p = a.h + r0 * a.Dp * 2;
+        B.bytes = (unsigned)BN * a.Dp * 2u;
+        B.ld = (unsigned)a.Dp * 2u;
+    } else {
+        A.ld = B.ld = (unsigned)(a.Dp / 32) * 1024u;
+        A.p = a.w + (v0 >> 4) * A.ld;
+        B.p = a.h + (r0 >> 4) * B.ld;
+        A.bytes = (BM / 16 - 1) * A.ld + 1024u;
+        B.bytes = (BN / 16 - 1) * B.ld + 1024u;
+        A.step = B.step = 1024;
+        A.kmax = 0;
+    }
+    A.part = a.w_part; B.part = a.h_part; B.kmax = 0;
 
     f32x4 acc[L::MT][4], none[4];
 #pragma unroll
     for (int t = 0; t < L::MT; ++t)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, 0, 0, PARTS, false>(A, B, a.Dp / BK, sa, sb, acc, none);
+    core<E, BN, KIND, KIND, PARTS, false>(A, B, a.Dp / BK, sa, sb, acc, none);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -312,12 +312,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
     const float* bias = a.bias + v0 + wm + 4 * q;
     if (!GRAD) {
         float top[4], sum[4];
-        int tg[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            top[n] = -INFINITY;
-            tg[n] = a.tgt[r0 + wn + 16 * n + i16];
-        }
+        for (int n = 0; n < 4; ++n) top[n] = -INFINITY;
 #pragma unroll
         for (int t = 0; t < L::MT; ++t) {
             const f32x4 bv = *reinterpret_cast<const f32x4*>(bias + 16 * t);
@@ -325,21 +321,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    acc[t][n][i] += bv[i];
+                    acc[t][n][i] = fmaf(acc[t][n][i], LOG2E, bv[i]);
                     top[n] = fmaxf(top[n], acc[t][n][i]);
-                    if (tg[n] == (int)v0 + wm + 16 * t + 4 * q + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
                 }
         }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            // fmaxf leaves NaN out; the sum below brings it back (exp(NaN - top))
+            // the target's logit, where a lane has it: most tiles have none of a wave's 16 rows' targets
+            const int rel = a.tgt[r0 + wn + 16 * n + i16] - ((int)v0 + wm + 4 * q);
+            if (__any(rel >= 0 && rel < 16 * L::MT && (rel & 15) < 4)) {
+#pragma unroll
+                for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (rel == 16 * t + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
+            }
+            // fmaxf leaves NaN out; the sum brings it back (exp(NaN - top))
             const float m = top[n] == -INFINITY ? 0.f : top[n];
             float s = 0.f;
 #pragma unroll
             for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s += PARTS == 1 ? __builtin_amdgcn_exp2f((acc[t][n][i] - m) * LOG2E) : expf(acc[t][n][i] - m);
+                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(acc[t][n][i] - m);
             sum[n] = s;
         }
         // lanes 16 apart hold other vocabulary entries of the same row
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
             for (int n = 0; n < 4; ++n) {
                 const float m2 = __shfl_xor(top[n], o, 64), s2 = __shfl_xor(sum[n], o, 64);
                 const float m = fmaxf(top[n], m2), base = m == -INFINITY ? 0.f : m;
-                sum[n] = sum[n] * expf(top[n] - base) + s2 * expf(m2 - base);
+                sum[n] = sum[n] * __builtin_amdgcn_exp2f(top[n] - base) + s2 * __builtin_amdgcn_exp2f(m2 - base);
                 top[n] = m;
             }
         if (q == 0) {
@@ -363,41 +366,53 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
             for (int w = 0; w < L::WM; ++w) m = fmaxf(m, red[w][threadIdx.x].x);
             const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int w = 0; w < L::WM; ++w) s += red[w][threadIdx.x].y * expf(red[w][threadIdx.x].x - base);
+            for (int w = 0; w < L::WM; ++w) s += red[w][threadIdx.x].y * __builtin_amdgcn_exp2f(red[w][threadIdx.x].x - base);
             a.part[(long long)vt * a.Rp + r0 + threadIdx.x] = make_float2(m, s);
         }
     } else {
         const float up = a.scale != nullptr ? a.scale[0] : 1.f;
         const long long nv32 = (long long)a.nvt * (BM / 32);
+        f32x4 bv[L::MT];
+#pragma unroll
+        for (int t = 0; t < L::MT; ++t) bv[t] = *reinterpret_cast<const f32x4*>(bias + 16 * t);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const long long r = r0 + wn + 16 * n + i16;
-            const float w = a.wrow[r] * up, lse = a.lse[r];
-            const int tg = a.tgt[r];
-            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + g_offset(i16, q);
+            const float w = a.wrow[r] * up, lse = a.lse[r] * LOG2E;
+            const int rel = a.tgt[r] - ((int)v0 + wm + 4 * q);
 #pragma unroll
-            for (int t = 0; t < L::MT; t += 2) {
-                float g[8];
+            for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int tt = t + (j >> 2), i = j & 3;
-                    const float x = acc[tt][n][i] + bias[16 * tt + i] - lse;
-                    float p = PARTS == 1 ? __builtin_amdgcn_exp2f(x * LOG2E) : expf(x);
-                    if (tg == (int)v0 + wm + 16 * tt + 4 * q + i) p -= 1.f;
-                    g[j] = w == 0.f ? 0.f : p * w;
-                }
-                char* to = dst + (t >> 1) * 1024;
+                for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_amdgcn_exp2f(fmaf(acc[t][n][i], LOG2E, bv[t][i] - lse));
+            if (__any(rel >= 0 && rel < 16 * L::MT && (rel & 15) < 4)) {
+#pragma unroll
+                for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (rel == 16 * t + i) acc[t][n][i] -= 1.f;
+            }
+            if (__any(w == 0.f)) {                       // no part in the gradient, whatever W makes of such a row's zeros
+#pragma unroll
+                for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][n][i] = w == 0.f ? 0.f : acc[t][n][i];
+            }
+            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + in_block(i16, q);
+#pragma unroll
+            for (int t = 0; t < L::MT; ++t) {
+                float g[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) g[i] = acc[t][n][i] * w;
 #pragma unroll
                 for (int s = 0; s < PARTS; ++s) {
-                    s16x4 out[2];
+                    s16x4 out;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const E e = (E)g[j];
-                        out[j >> 2][j & 3] = __builtin_bit_cast(short, e);
-                        g[j] -= (float)e;
+                    for (int i = 0; i < 4; ++i) {
+                        const E e = (E)g[i];
+                        out[i] = __builtin_bit_cast(short, e);
+                        g[i] -= (float)e;
                     }
-                    *reinterpret_cast<s16x4*>(to + s * a.g_part) = out[0];
-                    *reinterpret_cast<s16x4*>(to + s * a.g_part + 512) = out[1];
+                    *reinterpret_cast<s16x4*>(dst + s * a.g_part + (t >> 1) * 1024 + (t & 1) * 512) = out;
                 }
             }
         }
@@ -405,27 +420,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
 }
 
 // ------------------------------------------------------------------------------------------------
-// The two gradient products.  A = W or H with the width as its rows (256 of them a tile), read transposed; B = G.
+// The two gradient products.  A = W or H, 256 columns of it a tile; B = G.
 //   OVER_V true:  out[r][d] = sum over v of G[r][v] W[v][d]       rows of out: rows of H
 //   OVER_V false: out[v][d] = sum over r of G[r][v] H[r][d]       rows of out: the piece's vocabulary; bias gradient too
 // The contraction is cut into `splits` parts when there are too few tiles for the chip; each leaves fp32 sums in a slab.
 // ------------------------------------------------------------------------------------------------
 struct ProductArgs {
-    const char* x;            // W (from the piece's first row on) or the copy of H
-    const char* g;
+    const char* x;            // blocks of W (from the piece's first row on) or of H
+    const char* g;            // blocks of G
     float* slab;              // [splits][rows][Dp], added to when add != 0; NULL: out is written
     float* bslab;             // [splits][rows] bias gradient, or NULL
     void* out;                // [rows][ld_out] of the caller's type
     void* bout;
     const float* scale;       // fp16: scale[1] takes the scale of G out again (written only with the final result)
     long long x_part, g_part, ld_out, slab_stride;
-    unsigned ldx;
-    int x_rows, x_cols;       // rows of x, and the elements of a row that may be read
     int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
 };
 
 template <typename E, typename T, int BN, int PARTS, bool OVER_V>
-__global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(ProductArgs a) {
     typedef Lay<BN> L;
     __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
     char* const sa[STAGES] = {a0, a1, a2};
@@ -436,13 +449,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs
     const int k0 = (int)((long long)a.steps * split / a.splits), k1 = (int)((long long)a.steps * (split + 1) / a.splits);
 
     Operand A, B;
-    A.ld = a.ldx; A.part = a.x_part; A.step = (long long)BK * a.ldx; A.kmax = 0;
-    // rows k0 BK ... of x, columns from dt BM: whole steps of BK rows, then what is left of x's rows
-    A.p = a.x + k0 * A.step + (long long)dt * BM * 2;
-    A.full = a.x_rows / BK - k0;
-    A.bytes = (unsigned)(BK - 1) * a.ldx + (unsigned)(a.x_cols - dt * BM) * 2u;
-    A.tail = a.x_rows % BK ? (unsigned)(a.x_rows % BK - 1) * a.ldx + (unsigned)(a.x_cols - dt * BM) * 2u : 0;
-    B.kmax = 0; B.tail = 0; B.full = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
+    A.ld = (unsigned)(a.Dp / 32) * 1024u;
+    A.part = a.x_part; A.step = 2ll * A.ld; A.kmax = 0;
+    A.p = a.x + k0 * A.step + (long long)dt * (BM / 32) * 1024;
+    A.bytes = 2 * A.ld - (unsigned)dt * (BM / 32) * 1024u;          // columns behind Dp: blocks of the next rows, or nothing
+    B.kmax = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
     if (OVER_V) {
         B.step = 1024;
         B.p = a.g + (long long)nt * (BN / 16) * B.ld + k0 * B.step;
@@ -459,7 +470,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs
         for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 4; ++n) cs[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, 1, OVER_V ? 1 : 2, PARTS, !OVER_V>(A, B, k1 - k0, sa, sb, acc, cs);
+    core<E, BN, ACROSS, OVER_V ? ALONG : ACROSS, PARTS, !OVER_V>(A, B, k1 - k0, sa, sb, acc, cs);
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -527,26 +538,33 @@ __global__ __launch_bounds__(256) void xent_slab_sum_kernel(const float* __restr
 }
 
 // ------------------------------------------------------------------------------------------------
-// Copies: rows of H that take part, padded with zeros to [Rp][Dp] (a row that does not is zeros, whatever it holds); targets
-// and weights of the rows; the bias in fp32 with -inf behind the vocabulary; W where it cannot be loaded as it stands (fp32, or
-// rows that are no multiples of 16 bytes).  One launch, workgroup ranges.
+// Copies: rows of H that take part, as blocks (or as rows), padded with zeros to [Rp][Dp] (a row that does not take part is zeros,
+// whatever it holds); targets, weights and lse of the rows; the bias in fp32 and units of log 2, -inf behind the vocabulary; W as
+// blocks, zeros behind the vocabulary.  fp32 in three bf16 parts.  One launch, workgroup ranges.
 // ------------------------------------------------------------------------------------------------
 struct PrepArgs {
     const void *h, *w, *bias, *tok;
     const float *row_weight, *lse;        // NULL: loss only
-    char *hc, *wc;                        // wc NULL: W is not copied
+    char *hc, *wc;                        // wc NULL: W is not copied, and hc has rows
     float *biasf, *wrow, *lsec;
     int* tgt;
     long long ldh, ldw, h_part, w_part;
-    int tok64, R, Rp, V, Vp, D, Dp, nh, nb;
+    int tok64, R, Rp, V, Vp, D, Dp, nh, nb, wide_h, wide_w;
 };
 
 // eight columns of one row: from T to E, in PARTS parts
 template <typename T, typename E, int PARTS>
-__device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool live, char* dst, long long part) {
+__device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool live, bool wide, char* dst, long long part) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = live && j < left ? (float)src[j] : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if (live && wide) {                                  // rows of whole aligned vectors: left is at least 8, or nothing
+        if (left > 0) sv_load<8>(src, v);
+    } else if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) v[j] = (float)src[j];
+    }
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
         s16x8 out;
@@ -558,6 +576,10 @@ __device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool 
         }
         *reinterpret_cast<s16x8*>(dst + s * part) = out;
     }
+}
+// where eight columns from c on of row r are in blocks of a matrix of Dp columns
+__device__ __forceinline__ long long block_at(long long r, int c, int Dp) {
+    return ((r >> 4) * (Dp >> 5) + (c >> 5)) * 1024 + ((c >> 4) & 1) * 512 + in_block((int)(r & 15), (c & 15) >> 2);
 }
 
 template <typename T, typename E, int PARTS>
@@ -583,15 +605,16 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
                 a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
             }
         }
-        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.h) + (live ? r : 0) * a.ldh + c, a.D - c, live, a.hc + (r * a.Dp + c) * 2, a.h_part);
+        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.h) + (live ? r : 0) * a.ldh + c, a.D - c, live, a.wide_h,
+                           a.hc + (a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2), a.h_part);
     } else if ((int)blockIdx.x < a.nh + a.nb) {
         const long long v = i - (long long)a.nh * 256;
-        if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
+        if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] * LOG2E : 0.f;
     } else {
         const long long j = i - (long long)(a.nh + a.nb) * 256, r = j / per;
         const int c = (int)(j - r * per) * 8;
-        if (r >= a.V) return;
-        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + r * a.ldw + c, a.D - c, true, a.wc + (r * a.Dp + c) * 2, a.w_part);
+        if (r >= a.Vp) return;
+        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + (r < a.V ? r : 0) * a.ldw + c, a.D - c, r < a.V, a.wide_w, a.wc + block_at(r, c, a.Dp), a.w_part);
     }
 }
 
@@ -606,7 +629,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float2* __restric
     for (int v = s; v < nvt; v += 64) {
         const float2 p = part[(long long)v * Rp + r];
         const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
-        sum = sum * expf(m - base) + p.y * expf(p.x - base);
+        sum = sum * exp2f(m - base) + p.y * exp2f(p.x - base);
         m = m2;
     }
     red[s][i] = make_float2(m, sum);
@@ -615,13 +638,13 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float2* __restric
     for (int k = 1; k < 64; ++k) {
         const float2 p = red[k][i];
         const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
-        sum = sum * expf(m - base) + p.y * expf(p.x - base);
+        sum = sum * exp2f(m - base) + p.y * exp2f(p.x - base);
         m = m2;
     }
     const bool here = tgt[r] >= 0;
-    const float l = m + logf(sum);
-    lse[r] = here ? l : 0.f;
-    nll[r] = here ? l - zt[r] : 0.f;
+    const float l = m + log2f(sum);                          // (units of log 2)
+    lse[r] = here ? l * LN2 : 0.f;
+    nll[r] = here ? (l - zt[r]) * LN2 : 0.f;
 }
 
 // sum of the losses and number of rows with a target; in a fixed order, in 64 bits (a mean over no rows is 0)
@@ -674,11 +697,12 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restric
 // ------------------------------------------------------------------------------------------------
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
+constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
 constexpr long long PIECE_BYTES = 512ll << 20;           // what G of one piece may take
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
-    int parts, Rp, Vp, Dp, BN, nrt, nvt, copy_w, pieces, piece_tiles, dh_splits, dw_splits, ndt;
+    int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, dh_splits, dw_splits, ndt;
     long long h, h_part, w, w_part, ldw, bias, tgt, wrow, zt, part, scale, g, g_part, dh_slab, dw_slab, db_slab, total;
 };
 
@@ -699,14 +723,14 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     SV_CHECK_ARG(R > 0 && R <= 1 << 24 && V > 0 && V <= 1 << 28 && D > 0 && D <= 1 << 16 && ld_w >= D && ld_w <= 1 << 20,
                  "svae_xent: sizes R %lld, V %lld, D %lld, ld %lld", R, V, D, ld_w);
     s->parts = type == SV_F32 ? 3 : 1;
+    s->direct = !grad && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
     s->BN = R <= 64 ? 64 : 128;
     s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
     s->Vp = (int)((V + BM - 1) / BM * BM);
-    s->Dp = (int)((D + KPAD - 1) / KPAD * KPAD);
+    s->Dp = (int)((D + BK - 1) / BK * BK);
     s->nrt = s->Rp / s->BN;
     s->nvt = s->Vp / BM;
     s->ndt = (s->Dp + BM - 1) / BM;
-    s->copy_w = type == SV_F32 || D % 8 != 0 || ld_w % 8 != 0 || (unsigned long long)weight % 16 != 0;
     SV_CHECK_ARG((long long)s->nvt * s->nrt < 0x7ffffff0ll, "svae_xent: R %lld and V %lld need too many workgroups", R, V);
     long long at = 0;
     auto take = [&](long long bytes) {
@@ -716,8 +740,8 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     };
     s->h_part = (long long)s->Rp * s->Dp * 2;
     s->h = take(s->h_part * s->parts);
-    s->w_part = s->copy_w ? V * s->Dp * 2 : 0;
-    s->ldw = (s->copy_w ? s->Dp : ld_w) * 2;
+    s->w_part = s->direct ? 0 : (long long)s->Vp * s->Dp * 2;
+    s->ldw = ld_w * 2;
     s->w = take(s->w_part * s->parts);
     s->bias = take(4ll * s->Vp);
     s->tgt = take(4ll * s->Rp);
@@ -765,14 +789,17 @@ inline int prepare(const Call& c, const Shape& s, const float* row_weight, const
     p.lsec = (float*)(c.work + s.zt);
     p.h = c.hidden; p.w = c.weight; p.bias = c.bias; p.tok = c.targets; p.row_weight = row_weight;
     p.hc = c.work + s.h;
-    p.wc = s.copy_w ? c.work + s.w : nullptr;
+    p.wc = s.direct ? nullptr : c.work + s.w;
     p.biasf = (float*)(c.work + s.bias); p.wrow = (float*)(c.work + s.wrow); p.tgt = (int*)(c.work + s.tgt);
     p.ldh = c.ld_h; p.ldw = c.ld_w; p.h_part = s.h_part; p.w_part = s.w_part;
     p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.Vp = s.Vp; p.D = c.D; p.Dp = s.Dp;
     const long long nh = ((long long)s.Rp * (s.Dp / 8) + 255) / 256, nb = (s.Vp + 255) / 256,
-                    nw = s.copy_w ? ((long long)c.V * (s.Dp / 8) + 255) / 256 : 0;
+                    nw = s.direct ? 0 : ((long long)s.Vp * (s.Dp / 8) + 255) / 256;
     SV_CHECK_ARG(nh + nb + nw < 0x7ffffff0ll, "svae_xent: too large");
     p.nh = (int)nh; p.nb = (int)nb;
+    const int es = sv_elem_size(c.type);
+    p.wide_h = sv_vec_for(8, c.D, c.hidden, c.ld_h, es, c.hidden, c.ld_h, es) == 8;
+    p.wide_w = sv_vec_for(8, c.D, c.weight, c.ld_w, es, c.weight, c.ld_w, es) == 8;
     by_type(c.type, [&](auto t, auto e, auto parts) {
         hipLaunchKernelGGL((xent_prep_kernel<decltype(t), decltype(e), decltype(parts)::value>), dim3((unsigned)(nh + nb + nw)), dim3(256), 0, c.stream, p);
     });
@@ -782,12 +809,12 @@ inline int prepare(const Call& c, const Shape& s, const float* row_weight, const
 
 inline LogitArgs logit_args(const Call& c, const Shape& s) {
     LogitArgs a{};
-    a.w = s.copy_w ? c.work + s.w : (const char*)c.weight;
+    a.w = s.direct ? (const char*)c.weight : c.work + s.w;
     a.h = c.work + s.h;
     a.bias = (const float*)(c.work + s.bias); a.tgt = (const int*)(c.work + s.tgt);
     a.w_part = s.w_part; a.h_part = s.h_part; a.g_part = s.g_part;
     a.ldw = (unsigned)s.ldw;
-    a.V = c.V; a.D = s.copy_w ? s.Dp : c.D; a.Dp = s.Dp; a.Rp = s.Rp; a.nrt = s.nrt;
+    a.V = c.V; a.D = c.D; a.Dp = s.Dp; a.Rp = s.Rp; a.nrt = s.nrt;
     return a;
 }
 
@@ -797,8 +824,16 @@ inline void logits(const Call& c, const Shape& s, const LogitArgs& a) {
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
         const dim3 grid(launch_for((long long)a.nvt * a.nrt));
-        if (s.BN == 64) hipLaunchKernelGGL((xent_logit_kernel<E, 64, P, GRAD>), grid, dim3(64 * WAVES), 0, c.stream, a);
-        else hipLaunchKernelGGL((xent_logit_kernel<E, 128, P, GRAD>), grid, dim3(64 * WAVES), 0, c.stream, a);
+        auto go = [&](auto kernel, int bn) { hipLaunchKernelGGL(kernel, grid, dim3(bn == 256 ? 512 : 256), 0, c.stream, a); };
+        if constexpr (!GRAD && P == 1) {
+            if (s.direct) {
+                if (s.BN == 64) go(xent_logit_kernel<E, 64, PLAIN, P, GRAD>, 64);
+                else go(xent_logit_kernel<E, 128, PLAIN, P, GRAD>, 128);
+                return;
+            }
+        }
+        if (s.BN == 64) go(xent_logit_kernel<E, 64, ALONG, P, GRAD>, 64);
+        else go(xent_logit_kernel<E, 128, ALONG, P, GRAD>, 128);
     });
 }
 
@@ -888,9 +923,8 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
         ProductArgs d{};
         d.g = a.g; d.scale = scale; d.g_part = s.g_part; d.D = D; d.Dp = s.Dp; d.ndt = s.ndt; d.nv32 = nt * (BM / 32);
         if (dh) {
-            d.x = a.w + v0 * s.ldw;
-            d.x_rows = rows_v; d.x_cols = s.copy_w ? s.Dp : D;
-            d.x_part = s.w_part; d.ldx = (unsigned)s.ldw;
+            d.x = a.w + v0 * s.Dp * 2;
+            d.x_part = s.w_part;
             d.slab = (float*)(c.work + s.dh_slab); d.slab_stride = (long long)s.Rp * s.Dp;
             d.rows = s.Rp; d.nnt = s.nrt; d.splits = s.dh_splits; d.steps = nt * (BM / BK); d.add = p > 0;
             by_type(type, [&](auto t, auto e, auto parts) {
@@ -898,13 +932,13 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
                 typedef decltype(e) E;
                 constexpr int P = decltype(parts)::value;
                 const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
-                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(64 * WAVES), 0, c.stream, d);
-                else hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, true>), grid, dim3(64 * WAVES), 0, c.stream, d);
+                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(256), 0, c.stream, d);
+                else hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, true>), grid, dim3(256), 0, c.stream, d);
             });
             SV_LAUNCH_CHECK();
         }
         if (dw) {
-            d.x = a.h; d.x_rows = s.Rp; d.x_cols = s.Dp; d.x_part = s.h_part; d.ldx = (unsigned)s.Dp * 2u;
+            d.x = a.h; d.x_part = s.h_part;
             d.rows = rows_v; d.nnt = nt * (BM / 128); d.splits = s.dw_splits; d.steps = s.Rp / BK; d.add = 0;
             d.out = (char*)dw + v0 * ld_dw * es; d.ld_out = ld_dw;
             d.bout = db ? (char*)db + v0 * es : nullptr;
@@ -917,7 +951,7 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
                 typedef decltype(t) T;
                 typedef decltype(e) E;
                 constexpr int P = decltype(parts)::value;
-                hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(64 * WAVES), 0, c.stream, d);
+                hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(256), 0, c.stream, d);
                 if (d.slab != nullptr) {
                     const unsigned nmain = (unsigned)(((long long)rows_v * (s.Dp / 4) + 255) / 256), nbias = db ? (rows_v + 255) / 256 : 0;
                     hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain + nbias), dim3(256), 0, c.stream, d.slab, d.slab_stride, d.splits, rows_v, D,
