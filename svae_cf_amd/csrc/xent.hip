@@ -36,10 +36,11 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 constexpr int BM = 256;                   // outputs of a workgroup along A
 constexpr int BK = 32;                    // contraction of a step
 constexpr int STAGES = 3;
+constexpr int WAVES = 4;
 constexpr int AHEAD = 4;                  // fragments of A that are read in front of their products
 constexpr unsigned BUF_FLAGS = 0x00020000u;
 constexpr unsigned NOWHERE = 0xFFFFFFF0u; // past every buffer's end: such a lane loads zeros
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
 template <typename E>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c);
@@ -88,10 +89,9 @@ struct Operand {
 
 template <int BN>
 struct Lay {
-    static constexpr int WAVES = BN == 256 ? 8 : 4;
     static constexpr int WN = BN / 64;                  // waves along B, 64 outputs each
     static constexpr int WM = WAVES / WN;               // waves along A
-    static constexpr int MT = BM / WM / 16;             // 16-wide tiles of a wave along A
+    static constexpr int MT = BM / WM / 16;             // 16-wide tiles of a wave along A, at most; tile t of wave w is number WM t + w
     static constexpr int NA = BM * BK * 2 / 1024 / WAVES, NB = BN * BK * 2 / 1024 / WAVES;     // LDS-DMA instructions of a wave and step
 };
 
@@ -102,43 +102,40 @@ __device__ __forceinline__ unsigned dma_offset(unsigned inst, int lane, unsigned
     if (KIND == ALONG) return inst * ld + (unsigned)lane * 16u;
     return inst / (W / 32) * ld + inst % (W / 32) * 1024u + (unsigned)lane * 16u;
 }
-// fragment j (16 rows or columns from w0 + 16 j on) of a stage
+// Fragments of a stage: number `first` + EVERY j (16 rows or columns each; EVERY: 1, 2 or 4)
 struct Frag {
     unsigned lo, hi;
 };
 template <int KIND, int W>
-__device__ __forceinline__ Frag frag_offset(int w0, int lane) {
+__device__ __forceinline__ Frag frag_offset(int first, int lane) {
     const int i16 = lane & 15, q = lane >> 4;
     Frag f;
     if (KIND == PLAIN) {
-        const unsigned row = (unsigned)(w0 + i16) * 64u, sw = (unsigned)(-(i16 >> 2) & 3), at = (unsigned)(q & 1) * 8u;
+        const unsigned row = (unsigned)(first * 16 + i16) * 64u, sw = (unsigned)(-(i16 >> 2) & 3), at = (unsigned)(q & 1) * 8u;
         f.lo = row + ((unsigned)(q >> 1) ^ sw) * 16u + at;
         f.hi = row + ((unsigned)(2 + (q >> 1)) ^ sw) * 16u + at;
     } else if (KIND == ALONG) {
-        f.lo = (unsigned)(w0 >> 4) * 1024u + in_block(i16, q);
+        f.lo = (unsigned)first * 1024u + in_block(i16, q);
         f.hi = f.lo + 512u;
     } else {
-        f.lo = (unsigned)(w0 >> 5) * 1024u + in_block(4 * q + (i16 >> 2), i16 & 3);
+        f.lo = (unsigned)first * 512u + in_block(4 * q + (i16 >> 2), i16 & 3);      // (a block has two of them)
         f.hi = f.lo + (W / 32) * 1024u;
     }
     return f;
 }
 // entries 4 q ... and 16 + 4 q ... of the contraction's 32, whatever the kind
-template <int KIND>
+template <int KIND, int EVERY>
 __device__ __forceinline__ s16x8 read_frag(const char* stage, const Frag& f, int j) {
-    if (KIND == ACROSS) {
-        const unsigned o = (unsigned)((j >> 1) * 1024 + (j & 1) * 512);
-        return join(tr16(stage + f.lo + o), tr16(stage + f.hi + o));
-    }
+    if (KIND == ACROSS) return join(tr16(stage + f.lo + j * EVERY * 512), tr16(stage + f.hi + j * EVERY * 512));
     // (volatile: else the compiler makes one ds_read2_b64 of two reads, which takes 12 cycles instead of 2 x 2)
     typedef const volatile __attribute__((address_space(3))) s16x4* P;
-    const s16x4 lo = *(P)(stage + f.lo + j * 1024), hi = *(P)(stage + f.hi + j * 1024);
+    const s16x4 lo = *(P)(stage + f.lo + j * EVERY * 1024), hi = *(P)(stage + f.hi + j * EVERY * 1024);
     return join(lo, hi);
 }
 
-template <typename E, int BN, int AKIND, int BKIND, int PARTS, bool COLSUM>
+template <typename E, int BN, int MT, int AKIND, int BKIND, int PARTS, bool COLSUM>
 __device__ __forceinline__ void core(const Operand& A, const Operand& B, int steps, char* const (&sa)[STAGES], char* const (&sb)[STAGES],
-                                     f32x4 (&acc)[Lay<BN>::MT][4], f32x4 (&cs)[4]) {
+                                     f32x4 (&acc)[MT][4], f32x4 (&cs)[4]) {
     typedef Lay<BN> L;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -147,7 +144,7 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
     for (int j = 0; j < L::NA; ++j) oa[j] = dma_offset<AKIND, BM>((unsigned)(wave * L::NA + j), lane, A.ld);
 #pragma unroll
     for (int j = 0; j < L::NB; ++j) ob[j] = dma_offset<BKIND, BN>((unsigned)(wave * L::NB + j), lane, B.ld);
-    const Frag fa = frag_offset<AKIND, BM>((wave / L::WN) * (16 * L::MT), lane), fb = frag_offset<BKIND, BN>((wave % L::WN) * 64, lane);
+    const Frag fa = frag_offset<AKIND, BM>(wave / L::WN, lane), fb = frag_offset<BKIND, BN>((wave % L::WN) * 4, lane);
     const int chunk = ((lane & 3) ^ (-(lane >> 4) & 3)) * 8;         // PLAIN: first element of the lane's chunk
 
     const char *pa = A.p, *pb = B.p;                     // of the next step to be fetched
@@ -175,15 +172,15 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
         }
     };
     auto multiply = [&](int s, const char* da, const char* db) {
-        s16x8 a[L::MT], b[4];
+        s16x8 a[MT], b[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) b[n] = read_frag<BKIND>(db, fb, n);
+        for (int n = 0; n < 4; ++n) b[n] = read_frag<BKIND, 1>(db, fb, n);
 #pragma unroll
-        for (int t = 0; t < AHEAD && t < L::MT; ++t) a[t] = read_frag<AKIND>(da, fa, t);
+        for (int t = 0; t < AHEAD && t < MT; ++t) a[t] = read_frag<AKIND, L::WM>(da, fa, t);
 #pragma unroll
-        for (int t = 0; t < L::MT; ++t) {
+        for (int t = 0; t < MT; ++t) {
             __builtin_amdgcn_sched_barrier(0);           // reads stay AHEAD tiles in front of the products
-            if (t + AHEAD < L::MT) a[t + AHEAD] = read_frag<AKIND>(da, fa, t + AHEAD);
+            if (t + AHEAD < MT) a[t + AHEAD] = read_frag<AKIND, L::WM>(da, fa, t + AHEAD);
 #pragma unroll
             for (int n = 0; n < 4; ++n) acc[t][n] = mfma<E>(a[t], b[n], acc[t][n]);
         }
@@ -242,16 +239,23 @@ __device__ __forceinline__ int tile_of(int total) {
 }
 inline unsigned launch_for(long long tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
 
+// (maximum, sum of exponentials above it) of two sets of logits
+__device__ __forceinline__ void join_sums(float& m, float& s, float m2, float s2) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    s = s * __builtin_amdgcn_exp2f((m - base) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - base) * LOG2E);
+    m = top;
+}
+
 // ------------------------------------------------------------------------------------------------
 // z^T tiles: loss statistics (GRAD = false) or blocks of G (GRAD = true)
 // ------------------------------------------------------------------------------------------------
 struct LogitArgs {
     const char* w;            // W: its rows, ldw bytes apart (PLAIN), or blocks
     const char* h;            // copy of H: rows of Dp elements (PLAIN) or blocks
-    const float* bias;        // [Vp] in units of log 2, -inf behind V
+    const float* bias;        // [Vp], -inf behind V
     const int* tgt;           // [Rp], -1: left out
-    float2* part;             // loss: [vocabulary tiles][Rp] (maximum in units of log 2, sum of exponentials)
-    float* zt;                // loss: [Rp] the target's logit in units of log 2
+    float2* part;             // loss: [vocabulary tiles][Rp] (maximum, sum of exponentials)
+    float* zt;                // loss: [Rp] the target's logit
     const float* lse;         // gradient: [Rp]
     const float* wrow;        // gradient: [Rp], 0 for rows without a part in it
     const float* scale;       // gradient, fp16: the scale of G, or NULL
@@ -262,7 +266,7 @@ struct LogitArgs {
 };
 
 template <typename E, int BN, int KIND, int PARTS, bool GRAD>
-__global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(LogitArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) {
     typedef Lay<BN> L;
     __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
     char* const sa[STAGES] = {a0, a1, a2};
@@ -298,51 +302,50 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
     }
     A.part = a.w_part; B.part = a.h_part; B.kmax = 0;
 
-    f32x4 acc[L::MT][4], none[4];
-#pragma unroll
-    for (int t = 0; t < L::MT; ++t)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, KIND, KIND, PARTS, false>(A, B, a.Dp / BK, sa, sb, acc, none);
-
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
+    const int w0 = 16 * (wave / L::WN), wn = (wave % L::WN) * 64;        // tile t: vocabulary entries from w0 + 16 WM t on
     const int i16 = lane & 15, q = lane >> 4;
-    const float* bias = a.bias + v0 + wm + 4 * q;
+    constexpr int EVERY = 16 * L::WM;
+    const float* bias = a.bias + v0 + w0 + 4 * q;
+    // the sums start from the bias; loss and gradient make the same bits of z, so that errors of z cancel against those of lse
+    f32x4 acc[L::MT][4], none[4];
+#pragma unroll
+    for (int t = 0; t < L::MT; ++t) {
+        const f32x4 bv = *reinterpret_cast<const f32x4*>(bias + EVERY * t);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[t][n] = bv;
+    }
+    core<E, BN, L::MT, KIND, KIND, PARTS, false>(A, B, a.Dp / BK, sa, sb, acc, none);
+
+    // where a lane has the logit of a row's target: most tiles have none of a wave's 16 rows' targets
+    auto mine = [&](int n) { return a.tgt[r0 + wn + 16 * n + i16] - ((int)v0 + w0 + 4 * q); };
+    auto some = [&](int rel) { return __any(rel >= 0 && rel < EVERY * L::MT && rel % EVERY < 4); };
     if (!GRAD) {
         float top[4], sum[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) top[n] = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < L::MT; ++t) {
-            const f32x4 bv = *reinterpret_cast<const f32x4*>(bias + 16 * t);
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[t][n][i] = fmaf(acc[t][n][i], LOG2E, bv[i]);
-                    top[n] = fmaxf(top[n], acc[t][n][i]);
-                }
-        }
-#pragma unroll
         for (int n = 0; n < 4; ++n) {
-            // the target's logit, where a lane has it: most tiles have none of a wave's 16 rows' targets
-            const int rel = a.tgt[r0 + wn + 16 * n + i16] - ((int)v0 + wm + 4 * q);
-            if (__any(rel >= 0 && rel < 16 * L::MT && (rel & 15) < 4)) {
+            const int rel = mine(n);
+            if (some(rel)) {
 #pragma unroll
                 for (int t = 0; t < L::MT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (rel == 16 * t + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
+                        if (rel == EVERY * t + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
             }
+            float m = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < L::MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m = fmaxf(m, acc[t][n][i]);
+            top[n] = m;
             // fmaxf leaves NaN out; the sum brings it back (exp(NaN - top))
-            const float m = top[n] == -INFINITY ? 0.f : top[n];
+            const float base = m == -INFINITY ? 0.f : m * -LOG2E;
             float s = 0.f;
 #pragma unroll
             for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(acc[t][n][i] - m);
+                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(fmaf(acc[t][n][i], LOG2E, base));
             sum[n] = s;
         }
         // lanes 16 apart hold other vocabulary entries of the same row
@@ -351,9 +354,7 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const float m2 = __shfl_xor(top[n], o, 64), s2 = __shfl_xor(sum[n], o, 64);
-                const float m = fmaxf(top[n], m2), base = m == -INFINITY ? 0.f : m;
-                sum[n] = sum[n] * __builtin_amdgcn_exp2f(top[n] - base) + s2 * __builtin_amdgcn_exp2f(m2 - base);
-                top[n] = m;
+                join_sums(top[n], sum[n], m2, s2);
             }
         if (q == 0) {
 #pragma unroll
@@ -361,35 +362,30 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
         }
         __syncthreads();
         if ((int)threadIdx.x < BN) {
-            float m = -INFINITY, s = 0.f;
+            float m = red[0][threadIdx.x].x, s = red[0][threadIdx.x].y;
 #pragma unroll
-            for (int w = 0; w < L::WM; ++w) m = fmaxf(m, red[w][threadIdx.x].x);
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int w = 0; w < L::WM; ++w) s += red[w][threadIdx.x].y * __builtin_amdgcn_exp2f(red[w][threadIdx.x].x - base);
+            for (int w = 1; w < L::WM; ++w) join_sums(m, s, red[w][threadIdx.x].x, red[w][threadIdx.x].y);
             a.part[(long long)vt * a.Rp + r0 + threadIdx.x] = make_float2(m, s);
         }
     } else {
         const float up = a.scale != nullptr ? a.scale[0] : 1.f;
         const long long nv32 = (long long)a.nvt * (BM / 32);
-        f32x4 bv[L::MT];
-#pragma unroll
-        for (int t = 0; t < L::MT; ++t) bv[t] = *reinterpret_cast<const f32x4*>(bias + 16 * t);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const long long r = r0 + wn + 16 * n + i16;
-            const float w = a.wrow[r] * up, lse = a.lse[r] * LOG2E;
-            const int rel = a.tgt[r] - ((int)v0 + wm + 4 * q);
+            const float w = a.wrow[r] * up, lse = a.lse[r], low = -lse * LOG2E;
 #pragma unroll
             for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_amdgcn_exp2f(fmaf(acc[t][n][i], LOG2E, bv[t][i] - lse));
-            if (__any(rel >= 0 && rel < 16 * L::MT && (rel & 15) < 4)) {
+                for (int i = 0; i < 4; ++i)              // (one operation where 2^-24 |lse| in p does not matter)
+                    acc[t][n][i] = __builtin_amdgcn_exp2f(PARTS == 1 ? fmaf(acc[t][n][i], LOG2E, low) : (acc[t][n][i] - lse) * LOG2E);
+            const int rel = mine(n);
+            if (some(rel)) {
 #pragma unroll
                 for (int t = 0; t < L::MT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (rel == 16 * t + i) acc[t][n][i] -= 1.f;
+                        if (rel == EVERY * t + i) acc[t][n][i] -= 1.f;
             }
             if (__any(w == 0.f)) {                       // no part in the gradient, whatever W makes of such a row's zeros
 #pragma unroll
@@ -397,9 +393,10 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[t][n][i] = w == 0.f ? 0.f : acc[t][n][i];
             }
-            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32) + (wm >> 5)) * 1024 + in_block(i16, q);
+            char* dst = a.g + ((r >> 4) * nv32 + (long long)vt * (BM / 32)) * 1024 + in_block(i16, q);
 #pragma unroll
             for (int t = 0; t < L::MT; ++t) {
+                const int half = L::WM * t + (w0 >> 4);  // 16 columns: half a block
                 float g[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) g[i] = acc[t][n][i] * w;
@@ -412,7 +409,7 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
                         out[i] = __builtin_bit_cast(short, e);
                         g[i] -= (float)e;
                     }
-                    *reinterpret_cast<s16x4*>(dst + s * a.g_part + (t >> 1) * 1024 + (t & 1) * 512) = out;
+                    *reinterpret_cast<s16x4*>(dst + s * a.g_part + half * 512) = out;
                 }
             }
         }
@@ -420,7 +417,8 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_logit_kernel(Logi
 }
 
 // ------------------------------------------------------------------------------------------------
-// The two gradient products.  A = W or H, 256 columns of it a tile; B = G.
+// The two gradient products.  A = W or H, up to 256 columns of it a tile (in steps of 32, so that the tiles of a width are alike
+// and nearly full); B = G.
 //   OVER_V true:  out[r][d] = sum over v of G[r][v] W[v][d]       rows of out: rows of H
 //   OVER_V false: out[v][d] = sum over r of G[r][v] H[r][d]       rows of out: the piece's vocabulary; bias gradient too
 // The contraction is cut into `splits` parts when there are too few tiles for the chip; each leaves fp32 sums in a slab.
@@ -437,8 +435,8 @@ struct ProductArgs {
     int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
 };
 
-template <typename E, typename T, int BN, int PARTS, bool OVER_V>
-__global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(ProductArgs a) {
+template <typename E, typename T, int BN, int MT, int PARTS, bool OVER_V>
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs a) {
     typedef Lay<BN> L;
     __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
     char* const sa[STAGES] = {a0, a1, a2};
@@ -451,8 +449,9 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(Pr
     Operand A, B;
     A.ld = (unsigned)(a.Dp / 32) * 1024u;
     A.part = a.x_part; A.step = 2ll * A.ld; A.kmax = 0;
-    A.p = a.x + k0 * A.step + (long long)dt * (BM / 32) * 1024;
-    A.bytes = 2 * A.ld - (unsigned)dt * (BM / 32) * 1024u;          // columns behind Dp: blocks of the next rows, or nothing
+    constexpr int WIDE = 16 * L::WM * MT;                // columns of x that this workgroup makes
+    A.p = a.x + k0 * A.step + (long long)dt * (WIDE / 32) * 1024;
+    A.bytes = 2 * A.ld - (unsigned)dt * (WIDE / 32) * 1024u;        // columns behind Dp: blocks of the next rows, or nothing
     B.kmax = 0; B.part = a.g_part; B.ld = (unsigned)a.nv32 * 1024u;
     if (OVER_V) {
         B.step = 1024;
@@ -463,18 +462,19 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(Pr
         B.p = a.g + (long long)nt * (BN / 32) * 1024 + k0 * B.step;
         B.bytes = B.ld + (BN / 32) * 1024u;
     }
-    f32x4 acc[L::MT][4], cs[4];
+    f32x4 acc[MT][4], cs[4];
 #pragma unroll
-    for (int t = 0; t < L::MT; ++t)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 4; ++n) cs[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    core<E, BN, ACROSS, OVER_V ? ALONG : ACROSS, PARTS, !OVER_V>(A, B, k1 - k0, sa, sb, acc, cs);
+    core<E, BN, MT, ACROSS, OVER_V ? ALONG : ACROSS, PARTS, !OVER_V>(A, B, k1 - k0, sa, sb, acc, cs);
 
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));                       // (addresses of the results are not made, and kept, in front of the products)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = (wave / L::WN) * (16 * L::MT), wn = (wave % L::WN) * 64;
+    const int w0 = 16 * (wave / L::WN), wn = (wave % L::WN) * 64;
     const int i16 = lane & 15, q = lane >> 4;
     const float down = a.scale != nullptr ? a.scale[1] : 1.f;
 #pragma unroll
@@ -482,8 +482,8 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(Pr
         const int r = nt * BN + wn + 16 * n + i16;
         if (r >= a.rows) continue;
 #pragma unroll
-        for (int t = 0; t < L::MT; ++t) {
-            const int d = dt * BM + wm + 16 * t + 4 * q;
+        for (int t = 0; t < MT; ++t) {
+            const int d = dt * WIDE + w0 + 16 * L::WM * t + 4 * q;
             if (a.slab != nullptr) {
                 if (d < a.Dp) {
                     f32x4* s = reinterpret_cast<f32x4*>(a.slab + split * a.slab_stride + (long long)r * a.Dp + d);
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(64 * Lay<BN>::WAVES, 2) void xent_product_kernel(Pr
                 }
             }
         }
-        if (!OVER_V && dt == 0 && wm == 0 && q == 0) {
+        if (!OVER_V && dt == 0 && w0 == 0 && q == 0) {
             if (a.bslab != nullptr) a.bslab[(long long)split * a.rows + r] = cs[n][0];
             else if (a.bout != nullptr) reinterpret_cast<T*>(a.bout)[r] = (T)(cs[n][0] * down);
         }
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256) void xent_slab_sum_kernel(const float* __restr
 
 // ------------------------------------------------------------------------------------------------
 // Copies: rows of H that take part, as blocks (or as rows), padded with zeros to [Rp][Dp] (a row that does not take part is zeros,
-// whatever it holds); targets, weights and lse of the rows; the bias in fp32 and units of log 2, -inf behind the vocabulary; W as
+// whatever it holds); targets, weights and lse of the rows; the bias in fp32, -inf behind the vocabulary; W as
 // blocks, zeros behind the vocabulary.  fp32 in three bf16 parts.  One launch, workgroup ranges.
 // ------------------------------------------------------------------------------------------------
 struct PrepArgs {
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
                            a.hc + (a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2), a.h_part);
     } else if ((int)blockIdx.x < a.nh + a.nb) {
         const long long v = i - (long long)a.nh * 256;
-        if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] * LOG2E : 0.f;
+        if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
     } else {
         const long long j = i - (long long)(a.nh + a.nb) * 256, r = j / per;
         const int c = (int)(j - r * per) * 8;
@@ -618,33 +618,32 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
     }
 }
 
-// lse and loss of 16 rows a workgroup from the tiles' statistics
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
-                                                         const int* __restrict__ tgt, int R, int Rp, int nvt,
-                                                         float* __restrict__ nll, float* __restrict__ lse) {
-    __shared__ float2 red[64][17];
-    const int i = threadIdx.x & 15, s = threadIdx.x >> 4;
-    const long long r = (long long)blockIdx.x * 16 + i;
+// lse and loss from the tiles' statistics: a workgroup takes 256 / SLICES rows, SLICES threads share the tiles of one
+template <int SLICES>
+__global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
+                                                        const int* __restrict__ tgt, int R, int Rp, int nvt,
+                                                        float* __restrict__ nll, float* __restrict__ lse) {
+    constexpr int ROWS = 256 / SLICES;
+    __shared__ float2 red[SLICES][ROWS + 1];
+    const int i = threadIdx.x % ROWS, s = threadIdx.x / ROWS;
+    const long long r = (long long)blockIdx.x * ROWS + i;
     float m = -INFINITY, sum = 0.f;
-    for (int v = s; v < nvt; v += 64) {
-        const float2 p = part[(long long)v * Rp + r];
-        const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
-        sum = sum * exp2f(m - base) + p.y * exp2f(p.x - base);
-        m = m2;
+    for (int v = s; v < nvt; v += 4 * SLICES) {          // four tiles at a time: their loads do not wait for each other
+        float2 p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            p[k] = v + k * SLICES < nvt ? part[(long long)(v + k * SLICES) * Rp + r] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) join_sums(m, sum, p[k].x, p[k].y);
     }
     red[s][i] = make_float2(m, sum);
     __syncthreads();
-    if (threadIdx.x >= 16 || r >= R) return;
-    for (int k = 1; k < 64; ++k) {
-        const float2 p = red[k][i];
-        const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.f : m2;
-        sum = sum * exp2f(m - base) + p.y * exp2f(p.x - base);
-        m = m2;
-    }
+    if ((int)threadIdx.x >= ROWS || r >= R) return;
+    for (int k = 1; k < SLICES; ++k) join_sums(m, sum, red[k][i].x, red[k][i].y);
     const bool here = tgt[r] >= 0;
-    const float l = m + log2f(sum);                          // (units of log 2)
-    lse[r] = here ? l * LN2 : 0.f;
-    nll[r] = here ? (l - zt[r]) * LN2 : 0.f;
+    const float l = m + logf(sum);
+    lse[r] = here ? l : 0.f;
+    nll[r] = here ? l - zt[r] : 0.f;
 }
 
 // sum of the losses and number of rows with a target; in a fixed order, in 64 bits (a mean over no rows is 0)
@@ -698,11 +697,11 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restric
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
-constexpr long long PIECE_BYTES = 512ll << 20;           // what G of one piece may take
+constexpr long long PIECE_BYTES = 1ll << 30;             // what G of one piece may take
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
-    int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, dh_splits, dw_splits, ndt;
+    int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, dh_splits, dw_splits, ndt, dblocks;
     long long h, h_part, w, w_part, ldw, bias, tgt, wrow, zt, part, scale, g, g_part, dh_slab, dw_slab, db_slab, total;
 };
 
@@ -730,7 +729,10 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->Dp = (int)((D + BK - 1) / BK * BK);
     s->nrt = s->Rp / s->BN;
     s->nvt = s->Vp / BM;
+    // tiles of the width: as few as 256 columns a tile allow, of equal numbers of 32-column blocks
     s->ndt = (s->Dp + BM - 1) / BM;
+    s->dblocks = (s->Dp / 32 + s->ndt - 1) / s->ndt;
+    s->dblocks = s->BN == 64 ? 8 : s->dblocks <= 2 ? 2 : s->dblocks <= 4 ? 4 : s->dblocks;
     SV_CHECK_ARG((long long)s->nvt * s->nrt < 0x7ffffff0ll, "svae_xent: R %lld and V %lld need too many workgroups", R, V);
     long long at = 0;
     auto take = [&](long long bytes) {
@@ -824,16 +826,41 @@ inline void logits(const Call& c, const Shape& s, const LogitArgs& a) {
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
         const dim3 grid(launch_for((long long)a.nvt * a.nrt));
-        auto go = [&](auto kernel, int bn) { hipLaunchKernelGGL(kernel, grid, dim3(bn == 256 ? 512 : 256), 0, c.stream, a); };
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, a); };
         if constexpr (!GRAD && P == 1) {
             if (s.direct) {
-                if (s.BN == 64) go(xent_logit_kernel<E, 64, PLAIN, P, GRAD>, 64);
-                else go(xent_logit_kernel<E, 128, PLAIN, P, GRAD>, 128);
+                if (s.BN == 64) go(xent_logit_kernel<E, 64, PLAIN, P, GRAD>);
+                else go(xent_logit_kernel<E, 128, PLAIN, P, GRAD>);
                 return;
             }
         }
-        if (s.BN == 64) go(xent_logit_kernel<E, 64, ALONG, P, GRAD>, 64);
-        else go(xent_logit_kernel<E, 128, ALONG, P, GRAD>, 128);
+        if (s.BN == 64) go(xent_logit_kernel<E, 64, ALONG, P, GRAD>);
+        else go(xent_logit_kernel<E, 128, ALONG, P, GRAD>);
+    });
+}
+
+template <bool OVER_V>
+inline void products(const Call& c, const Shape& s, const ProductArgs& d) {
+    by_type(c.type, [&](auto t, auto e, auto parts) {
+        typedef decltype(t) T;
+        typedef decltype(e) E;
+        constexpr int P = decltype(parts)::value;
+        const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, d); };
+        if (s.dblocks == 2) go(xent_product_kernel<E, T, 128, 2, P, OVER_V>);
+        else if (s.dblocks == 4) go(xent_product_kernel<E, T, 128, 4, P, OVER_V>);
+        else if (s.dblocks == 5) go(xent_product_kernel<E, T, 128, 5, P, OVER_V>);
+        else if (s.dblocks == 6) go(xent_product_kernel<E, T, 128, 6, P, OVER_V>);
+        else if (s.dblocks == 7) go(xent_product_kernel<E, T, 128, 7, P, OVER_V>);
+        else {
+            if constexpr (OVER_V) {
+                if (s.BN == 64) {
+                    go(xent_product_kernel<E, T, 64, 4, P, true>);
+                    return;
+                }
+            }
+            go(xent_product_kernel<E, T, 128, 8, P, OVER_V>);
+        }
     });
 }
 
@@ -874,7 +901,11 @@ extern "C" int svae_xent_fwd(const void* hidden, long long ld_h, const void* wei
     a.v_begin = 0; a.nvt = s.nvt;
     logits<false>(c, s, a);
     SV_LAUNCH_CHECK();
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(s.Rp / 16), dim3(1024), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
+    // few rows and many tiles: more threads a row
+    if ((long long)s.Rp * 8 < s.nvt * 64ll)
+        hipLaunchKernelGGL(xent_rows_kernel<64>, dim3(s.Rp / 4), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
+    else
+        hipLaunchKernelGGL(xent_rows_kernel<8>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
     SV_LAUNCH_CHECK();
     return 0;
 }
@@ -927,14 +958,7 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
             d.x_part = s.w_part;
             d.slab = (float*)(c.work + s.dh_slab); d.slab_stride = (long long)s.Rp * s.Dp;
             d.rows = s.Rp; d.nnt = s.nrt; d.splits = s.dh_splits; d.steps = nt * (BM / BK); d.add = p > 0;
-            by_type(type, [&](auto t, auto e, auto parts) {
-                typedef decltype(t) T;
-                typedef decltype(e) E;
-                constexpr int P = decltype(parts)::value;
-                const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
-                if (s.BN == 64) hipLaunchKernelGGL((xent_product_kernel<E, T, 64, P, true>), grid, dim3(256), 0, c.stream, d);
-                else hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, true>), grid, dim3(256), 0, c.stream, d);
-            });
+            products<true>(c, s, d);
             SV_LAUNCH_CHECK();
         }
         if (dw) {
@@ -947,18 +971,17 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
             d.slab_stride = (long long)s.piece_tiles * BM * s.Dp;
             const int wide = es * 4 < 16 ? es * 4 : 16;
             d.out_vec = D % 4 == 0 && ld_dw * es % wide == 0 && (unsigned long long)d.out % wide == 0;
-            by_type(type, [&](auto t, auto e, auto parts) {
-                typedef decltype(t) T;
-                typedef decltype(e) E;
-                constexpr int P = decltype(parts)::value;
-                hipLaunchKernelGGL((xent_product_kernel<E, T, 128, P, false>), dim3(launch_for((long long)d.ndt * d.nnt * d.splits)), dim3(256), 0, c.stream, d);
-                if (d.slab != nullptr) {
+            products<false>(c, s, d);
+            SV_LAUNCH_CHECK();
+            if (d.slab != nullptr) {
+                by_type(type, [&](auto t, auto, auto) {
+                    typedef decltype(t) T;
                     const unsigned nmain = (unsigned)(((long long)rows_v * (s.Dp / 4) + 255) / 256), nbias = db ? (rows_v + 255) / 256 : 0;
                     hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain + nbias), dim3(256), 0, c.stream, d.slab, d.slab_stride, d.splits, rows_v, D,
                                        s.Dp, (T*)d.out, ld_dw, d.bslab, (T*)d.bout, scale, nmain);
-                }
-            });
-            SV_LAUNCH_CHECK();
+                });
+                SV_LAUNCH_CHECK();
+            }
         }
     }
     if (dh) {
