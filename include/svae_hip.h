@@ -435,11 +435,13 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
  *   svae_xent_reduce  out[0] = the sum of nll or (mean != 0) its mean over the rows with a target (0 over none), out[1] = the
  *                     weight of a row in it
  *   svae_xent_bwd     gradients of sum_r row_weight[r] nll[r], given fwd's lse: dh [R][D], dw [V][D], db [V] in the inputs'
- *                     type; dh or dw may be NULL (db comes with dw).  Made in pieces of the vocabulary, sized by the workspace.
- *                     A row of weight 0 takes no part, whatever it holds.
- * Workspace (aligned to 256 bytes): svae_xent_bytes(weight, ld_w, type, R, V, D, grad, &bytes), grad != 0 for svae_xent_bwd; the
- * size depends on whether weight's rows can be loaded as they stand (16-bit types, address and row length multiples of 16 bytes). */
-int svae_xent_bytes(const void* weight, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes);
+ *                     type; dh or dw may be NULL (db comes with dw).  Made in pieces of the vocabulary.  A row of weight 0
+ *                     takes no part, whatever it holds.
+ *   svae_xent_fwd_bwd both in one call, for programs that know the rows' weights beforehand (copies of the inputs are made once)
+ * Workspace, aligned to 256 bytes: svae_xent_bytes(address of weight modulo 16, ld_w, type, R, V, D, grad, &bytes), grad != 0 for
+ * the gradients.  The loss of up to 512 rows in a 16-bit type reads weight as it lies if address and rows are multiples of 16
+ * bytes; else the workspace holds a copy of weight; gradients have two pieces of up to 512 MiB in it. */
+int svae_xent_bytes(int weight_align, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes);
 int svae_xent_fwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                   const void* targets, int tok64, int type, int R, int V, int D, float* nll, float* lse, void* work,
                   long long work_bytes, void* stream);
@@ -448,6 +450,11 @@ int svae_xent_bwd(const void* hidden, long long ld_h, const void* weight, long l
                   const void* targets, int tok64, int type, int R, int V, int D, const float* lse, const float* row_weight,
                   void* dh, long long ld_dh, void* dw, long long ld_dw, void* db, void* work, long long work_bytes,
                   void* stream);
+
+int svae_xent_fwd_bwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                      const void* targets, int tok64, int type, int R, int V, int D, const float* row_weight, float* nll,
+                      float* lse, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db, void* work,
+                      long long work_bytes, void* stream);
 
 /* ---- dropout from a counter-based generator ------------------------------------------------------------------
  * No counterpart in the reference.  y[r][c] = x[r][c] * 65536 / (65536 - k) where the 16 random bits of (r, c) are at least

@@ -99,8 +99,9 @@ SIGNATURES = {
     "svae_lookup_bwd_bytes": [_I, _I, _P],
     "svae_lookup_bwd": [_P, _I, _LL, _P, _P, _I, _I, _I, _F, _P, _I, _LL, _I, _P, _LL, _P],
     "svae_dropout": [_P, _LL, _P, _LL, _I, _I, _I, _c.c_double, _ULL, _U, _P, _P, _P],
-    "svae_xent_bytes": [_P, _LL, _I, _I, _I, _I, _I, _P],
+    "svae_xent_bytes": [_I, _LL, _I, _I, _I, _I, _I, _P],
     "svae_xent_fwd": [_P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _LL, _P],
+    "svae_xent_fwd_bwd": [_P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _LL, _P, _LL, _P, _P, _LL, _P],
     "svae_xent_reduce": [_P, _P, _I, _I, _I, _I, _P, _P],
     "svae_xent_bwd": [_P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _LL, _P, _LL, _P, _P, _LL, _P],
     # split instantiations (prec 2) of the fused kernels

@@ -41,12 +41,15 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const T* __restrict__ t
 }
 
 // ------------------------------------------------------------------------------------------------
-// Stable radix sort of (token, place) by token.  Least significant digit first, the fewest passes of at most 11 bits, equal
-// digits; two launches a pass: digit counts per workgroup, then every workgroup adds up the counts in front of it (there are
-// at most 256 workgroups, so that is a few microseconds from the L2 and saves a launch for the scan) and places its keys.
-// Places outside [0, V) and the padding token get the key V and end up behind all others.
+// Stable radix sort of (token, place) by token, least significant digit first.  Places outside [0, V) and the padding token get
+// the key V and end up behind all others.
+//   up to SMALL places: one workgroup, digits of 8 bits, keys and places in LDS (20 000 tokens, 256 places: 9 us for the launch
+//   instead of 4 x 4);
+//   more: the fewest passes of at most 11 bits, equal digits; two launches a pass: digit counts per workgroup, then every
+//   workgroup adds up the counts in front of it (there are at most 256 workgroups, so that is a few microseconds from the L2 and
+//   saves a launch for the scan) and places its keys.  21 800 places: 1024 a workgroup, 22 workgroups; bound by latency.
 // ------------------------------------------------------------------------------------------------
-constexpr int SORT_MAX_BITS = 11, SORT_MAX_WG = 256, SORT_MIN_TILE = 4096;
+constexpr int SORT_MAX_BITS = 11, SORT_MAX_WG = 256, SORT_MIN_TILE = 1024, SMALL = 4096, SMALL_BITS = 8;
 
 struct SortShape {
     int passes, bits, nwg, tile;          // digits, bits of a digit, workgroups, keys of a workgroup (a multiple of 1024)
@@ -55,8 +58,9 @@ inline SortShape sort_shape(int R, int V) {
     SortShape s;
     int bits = 1;
     while (((long long)V >> bits) != 0) ++bits;              // keys 0 .. V
-    s.passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
-    s.bits = (bits + s.passes - 1) / s.passes;
+    const int most = R <= SMALL ? SMALL_BITS : SORT_MAX_BITS;
+    s.passes = (bits + most - 1) / most;
+    s.bits = R <= SMALL ? SMALL_BITS : (bits + s.passes - 1) / s.passes;
     long long tile = ((long long)R + SORT_MAX_WG - 1) / SORT_MAX_WG;
     tile = (tile + 1023) / 1024 * 1024;
     s.tile = (int)(tile < SORT_MIN_TILE ? SORT_MIN_TILE : tile);
@@ -77,6 +81,30 @@ __device__ __forceinline__ unsigned sort_key(const SortArgs& a, long long i) {
     const long long t = token_at(a.tok, a.tok64, i);
     return t < 0 || t >= a.V || t == a.pad ? (unsigned)a.V : (unsigned)t;
 }
+// lanes of the wave that are `live` and have this lane's digit
+__device__ __forceinline__ unsigned long long same_digit(bool live, unsigned digit, int bits) {
+    unsigned long long same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long one = __ballot((digit >> b) & 1u);
+        same &= (digit >> b) & 1u ? one : ~one;
+    }
+    return same;
+}
+// exclusive sum over the 1024 threads of a workgroup; wtot: 16 words of LDS; ends behind a barrier
+__device__ __forceinline__ unsigned scan1024(unsigned v, unsigned* wtot) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    unsigned scan = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned up = __shfl_up(scan, o, 64);
+        if (lane >= o) scan += up;
+    }
+    if (lane == 63) wtot[wave] = scan;
+    __syncthreads();
+    unsigned first = scan - v;
+    for (int w = 0; w < wave; ++w) first += wtot[w];
+    return first;
+}
 
 __global__ __launch_bounds__(1024) void sort_count_kernel(SortArgs a) {
     __shared__ unsigned hist[1 << SORT_MAX_BITS];
@@ -91,46 +119,44 @@ __global__ __launch_bounds__(1024) void sort_count_kernel(SortArgs a) {
 }
 
 __global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a) {
-    extern __shared__ unsigned lds[];                        // [16 waves][1 << bits], then 16 wave totals
+    extern __shared__ unsigned lds[];                        // [16 waves][1 << bits] counts, [1 << bits] x 2 sums, 16 wave totals
     const int nb = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned* mine = lds + wave * nb;
-    unsigned* wtot = lds + 16 * nb;
-    for (int d = tid; d < 16 * nb; d += 1024) lds[d] = 0;
-    __syncthreads();
+    unsigned *before = lds + 16 * nb, *total = before + nb, *wtot = total + nb;
+    for (int d = tid; d < 18 * nb; d += 1024) lds[d] = 0;
     // each wave owns a run of consecutive keys, so that waves in order and rounds in order are the keys' order
     const int run = a.tile / 16;
     const long long base = (long long)blockIdx.x * a.tile + (long long)wave * run;
-    for (int j = lane; j < run; j += 64)
-        if (base + j < a.R) atomicAdd(&mine[(sort_key(a, base + j) >> a.shift) & (nb - 1)], 1u);
-    // digits 2 tid and 2 tid + 1: keys of this digit in the workgroups in front, and in all
-    unsigned before[2] = {0, 0}, total[2] = {0, 0};
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int d = 2 * tid + q;
-        if (d < nb) {
-#pragma unroll 8
-            for (int b = 0; b < (int)gridDim.x; ++b) {
-                const unsigned n = a.cnt[(size_t)b * nb + d];
-                total[q] += n;
-                before[q] += b < (int)blockIdx.x ? n : 0u;
-            }
-        }
-    }
-    unsigned scan = total[0] + total[1];                     // inclusive scan over the workgroup's threads
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned up = __shfl_up(scan, o, 64);
-        if (lane >= o) scan += up;
-    }
-    if (lane == 63) wtot[wave] = scan;
+    const unsigned key0 = base + lane < a.R ? sort_key(a, base + lane) : 0u;
     __syncthreads();
-    unsigned first = scan - total[0] - total[1];
-    for (int w = 0; w < wave; ++w) first += wtot[w];
+    for (int j = 0; j < run; j += 64) {
+        const long long i = base + j + lane;
+        if (i < a.R) atomicAdd(&mine[((j == 0 ? key0 : sort_key(a, i)) >> a.shift) & (nb - 1)], 1u);
+    }
+    // keys of each digit in the workgroups in front, and in all: the rows of counts are dealt to the threads of a digit
+    const int per = nb < 1024 ? 1024 >> a.bits : 1;
+    for (int d = tid & (nb - 1), row = tid >> a.bits; d < nb; d += 1024) {
+        unsigned b = 0, t = 0;
+#pragma unroll 8
+        for (int w = nb < 1024 ? row : 0; w < (int)gridDim.x; w += per) {
+            const unsigned n = a.cnt[(size_t)w * nb + d];
+            t += n;
+            b += w < (int)blockIdx.x ? n : 0u;
+        }
+        if (b) atomicAdd(&before[d], b);
+        if (t) atomicAdd(&total[d], t);
+    }
+    __syncthreads();
+    unsigned mine2[2] = {0, 0};                              // digits 2 tid and 2 tid + 1
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        if (2 * tid + q < nb) mine2[q] = total[2 * tid + q];
+    const unsigned first = scan1024(mine2[0] + mine2[1], wtot);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int d = 2 * tid + q;
         if (d < nb) {
-            unsigned at = first + (q ? total[0] : 0u) + before[q];
+            unsigned at = first + (q ? mine2[0] : 0u) + before[d];
             for (int w = 0; w < 16; ++w) {
                 const unsigned n = lds[w * nb + d];
                 lds[w * nb + d] = at;
@@ -143,13 +169,9 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a) {
     for (int j = 0; j < run; j += 64) {
         const long long i = base + j + lane;
         const bool live = i < a.R;
-        const unsigned key = live ? sort_key(a, i) : 0u;
+        const unsigned key = j == 0 ? key0 : live ? sort_key(a, i) : 0u;
         const unsigned digit = (key >> a.shift) & (nb - 1);
-        unsigned long long same = __ballot(live);            // the lanes of this round with the same digit
-        for (int b = 0; b < a.bits; ++b) {
-            const unsigned long long one = __ballot((digit >> b) & 1u);
-            same &= (digit >> b) & 1u ? one : ~one;
-        }
+        const unsigned long long same = same_digit(live, digit, a.bits);
         const unsigned rank = __popcll(same & ((1ull << lane) - 1ull));
         if (live) {
             const unsigned at = next[digit];
@@ -162,37 +184,102 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a) {
     }
 }
 
-// ------------------------------------------------------------------------------------------------
-// The gradient over sorted tokens.  A wave owns GROUP table rows and finds their segments of the sorted list by bisection;
-// a segment of up to LONG rows is added by that wave, an empty one is written as zeros.  Popular tokens have longer segments:
-// those are added in pieces of CHUNK sorted places by workgroups of their own into fp32 partial sums (first workgroups of the
-// same launch), which a second launch adds up in order.  A chunk meets at most two long segments, the one at its first place
-// (slot 0) and the one at its last (slot 1): anything between is shorter than the chunk.
-// ------------------------------------------------------------------------------------------------
-constexpr int CHUNK = 64, LONG = 64, GROUP = 4;
-static_assert(LONG >= CHUNK, "a chunk could meet a third long segment");
-
-// first place whose key is not below k
-__device__ __forceinline__ int lower_bound(const int* __restrict__ keys, int R, long long k) {
-    int lo = 0, hi = R;
-    while (lo < hi) {
-        const int mid = lo + ((hi - lo) >> 1);
-        if (keys[mid] < k) lo = mid + 1;
-        else hi = mid;
+__global__ __launch_bounds__(1024) void sort_small_kernel(SortArgs a, int passes) {
+    constexpr int NB = 1 << SMALL_BITS;
+    __shared__ unsigned key[2][SMALL];
+    __shared__ unsigned short place[2][SMALL];
+    __shared__ unsigned hist[16][NB];
+    __shared__ unsigned wtot[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int run = (a.R + 1023) / 1024 * 64;                // keys of a wave
+    for (int i = tid; i < a.R; i += 1024) {
+        key[0][i] = sort_key(a, i);
+        place[0][i] = (unsigned short)i;
     }
-    return lo;
+    for (int p = 0; p < passes; ++p) {
+        const int from = p & 1, shift = p * SMALL_BITS;
+        for (int d = lane; d < NB; d += 64) hist[wave][d] = 0;
+        __syncthreads();
+        volatile unsigned* next = hist[wave];
+        for (int i = wave * run + lane; i < (wave + 1) * run; i += 64) {
+            const bool live = i < a.R;
+            const unsigned digit = live ? (key[from][i] >> shift) & (NB - 1) : 0u;
+            const unsigned long long same = same_digit(live, digit, SMALL_BITS);
+            if (live && (same & ((1ull << lane) - 1ull)) == 0) next[digit] += (unsigned)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        unsigned n = 0;
+        if (tid < NB)
+            for (int w = 0; w < 16; ++w) n += hist[w][tid];
+        unsigned at = scan1024(n, wtot);
+        if (tid < NB)
+            for (int w = 0; w < 16; ++w) {
+                const unsigned c = hist[w][tid];
+                hist[w][tid] = at;
+                at += c;
+            }
+        __syncthreads();
+        for (int i = wave * run + lane; i < (wave + 1) * run; i += 64) {
+            const bool live = i < a.R;
+            const unsigned k = live ? key[from][i] : 0u, digit = (k >> shift) & (NB - 1);
+            const unsigned long long same = same_digit(live, digit, SMALL_BITS);
+            const unsigned rank = __popcll(same & ((1ull << lane) - 1ull));
+            if (live) {
+                const unsigned to = next[digit];
+                __builtin_amdgcn_wave_barrier();
+                if (rank == 0) next[digit] = to + (unsigned)__popcll(same);
+                key[from ^ 1][to + rank] = k;
+                place[from ^ 1][to + rank] = place[from][i];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < a.R; i += 1024) {
+        a.kout[i] = (int)key[passes & 1][i];
+        a.pout[i] = place[passes & 1][i];
+    }
 }
 
-// acc += sum of dy[perm[i]][c .. c + VEC) over i = b, b + step, .. < e, eight rows in flight
-template <int VEC, typename T>
-__device__ __forceinline__ void sum_rows(const T* __restrict__ dy, long long ldd, const int* __restrict__ perm, int b, int e,
-                                         int step, int c, float* acc) {
+// ------------------------------------------------------------------------------------------------
+// The gradient over sorted tokens.  A wave owns `group` table rows and finds their segments of the sorted list; a segment of up
+// to LONG rows is added by that wave, an empty one is written as zeros.  Popular tokens have longer segments: those are added in
+// pieces of CHUNK sorted places by workgroups of their own into fp32 partial sums (first workgroups of the same launch), which a
+// second launch adds up in order.  A chunk meets at most two long segments, the one at its first place (slot 0) and the one at
+// its last (slot 1): anything between is shorter than the chunk.
+// ------------------------------------------------------------------------------------------------
+constexpr int CHUNK = 64, LONG = 64, MOST_GROUP = 16;
+static_assert(CHUNK == 64 && LONG == CHUNK, "a lane has one place of a chunk, and a chunk meets no third long segment");
+
+// first place in [lo, R) whose key is not below k: 64 ways at a time, so a few loads in a row instead of log2 R
+__device__ __forceinline__ int lower_bound(const int* __restrict__ keys, int lo, int R, long long k, int lane) {
+    int hi = R;
+    while (hi - lo > 64) {
+        const long long n = hi - lo;
+        const bool below = keys[lo + (int)(n * lane >> 6)] < k;                        // places spread over [lo, hi)
+        const int c = __popcll(__ballot(below));                                       // lanes 0 .. c - 1 are below
+        hi = c == 64 ? hi : lo + (int)(n * c >> 6) + (c == 0 ? 0 : 1);
+        lo = c == 0 ? lo : lo + (int)(n * (c - 1) >> 6) + 1;
+        if (c == 0) return lo;
+    }
+    const bool below = lo + lane < hi && keys[lo + lane < hi ? lo + lane : lo] < k;
+    return lo + __popcll(__ballot(below));
+}
+// the end of the segment of key k that has place i
+__device__ __forceinline__ int segment_end(const int* __restrict__ keys, int i, int R, int k, int lane) {
+    return lower_bound(keys, i, R, (long long)k + 1, lane);
+}
+
+// acc += sum of dy[place(i)][c .. c + VEC) over i = b, b + step, .. < e, eight rows in flight
+template <int VEC, typename T, typename P>
+__device__ __forceinline__ void sum_rows(const T* __restrict__ dy, long long ldd, P place, int b, int e, int step, int c, float* acc) {
     for (int i = b; i < e; i += 8 * step) {
         float v[8][VEC];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const bool in = i + j * step < e;
-            if (in) sv_load<VEC>(dy + (long long)perm[i + j * step] * ldd + c, v[j]);
+            if (in) sv_load<VEC>(dy + (long long)place(i + j * step) * ldd + c, v[j]);
             else {
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) v[j][q] = 0.f;
@@ -221,58 +308,70 @@ __device__ __forceinline__ void put_row(G* __restrict__ dst, float* acc, float s
 template <int VEC, typename T, typename G>
 __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ dy, long long ldd, const int* __restrict__ keys,
                                                          const int* __restrict__ perm, int R, int V, int D, float scale,
-                                                         G* __restrict__ grad, long long ldg, int accumulate, int nchunk,
+                                                         G* __restrict__ grad, long long ldg, int accumulate, int nchunk, int group,
                                                          float* __restrict__ part) {
     __shared__ float red[4][64 * VEC];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if ((int)blockIdx.x < nchunk) {
-        const long long p0 = (long long)blockIdx.x * CHUNK;
-        const int p1 = (int)(p0 + CHUNK < R ? p0 + CHUNK : R);
-        const int kf = keys[p0], kl = keys[p1 - 1];
+        const int p0 = (int)blockIdx.x * CHUNK, p1 = R - p0 < CHUNK ? R : p0 + CHUNK;
+        // the chunk's keys and those of 64 places on either side: enough to tell which runs are long
+        const int kin = p0 + lane < p1 ? keys[p0 + lane] : -1;
+        const int kf = __builtin_amdgcn_readfirstlane(kin), kl = __builtin_amdgcn_readlane(kin, p1 - p0 - 1);
+        const int kb = p0 > lane ? keys[p0 - 1 - lane] : -1, ka = p1 + lane < R ? keys[p1 + lane] : -1;
+        const unsigned long long all = ~0ull;
+        auto run = [&](unsigned long long m) { return m == all ? 64 : __builtin_ctzll(~m); };      // lanes from 0 on
+        const unsigned long long mf = __ballot(kin == kf), ml = __ballot(kin == kl);
 #pragma unroll 1
         for (int slot = 0; slot < (kf == kl ? 1 : 2); ++slot) {
-            const int k = slot == 0 ? kf : kl;
-            if (k >= V) continue;
-            const int s = lower_bound(keys, R, k), e = lower_bound(keys, R, (long long)k + 1);
-            if (e - s <= LONG) continue;
-            const int b = s > (int)p0 ? s : (int)p0, z = e < p1 ? e : p1;
+            if ((slot == 0 ? kf : kl) >= V) continue;
+            const int b = slot == 0 ? p0 : p0 + __builtin_ctzll(ml), z = slot == 0 ? p0 + __popcll(mf) : p1;
+            const int length = z - b + (slot == 0 ? run(__ballot(kb == kf)) : 0) + (z == p1 ? run(__ballot(ka == kl)) : 0);
+            if (length <= LONG) continue;
             for (int c0 = 0; c0 < D; c0 += 64 * VEC) {
                 const int c = c0 + lane * VEC;
                 float acc[VEC];
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-                if (c < D) sum_rows<VEC>(dy, ldd, perm, b + wave, z, 4, c, acc);
+                if (c < D) sum_rows<VEC>(dy, ldd, [&](int i) { return perm[i]; }, b + wave, z, 4, c, acc);
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
                 __syncthreads();
                 if (wave == 0 && c < D) {
 #pragma unroll
                     for (int q = 0; q < VEC; ++q)
-                        part[((size_t)blockIdx.x * 2 + slot) * D + c + q] =
-                            (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
+                        acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
+                    sv_store<VEC>(part + ((size_t)blockIdx.x * 2 + slot) * D + c, acc);
                 }
                 __syncthreads();
             }
         }
         return;
     }
-    const long long v0 = ((long long)((int)blockIdx.x - nchunk) * 4 + wave) * GROUP;
+    const long long v0 = ((long long)((int)blockIdx.x - nchunk) * 4 + wave) * group;
     if (v0 >= V) return;
-    const int mine = lower_bound(keys, R, v0 + (lane < GROUP ? lane : GROUP));
+    const int s0 = lower_bound(keys, 0, R, v0, lane);
+    // the keys from there on tell the other bounds, unless there are more than 64 of them
+    const int near = s0 + lane < R ? keys[s0 + lane] : 0x7fffffff;
+    const int place = s0 + lane < R ? perm[s0 + lane] : 0;
+    int s = s0;
 #pragma unroll 1
-    for (int g = 0; g < GROUP; ++g) {
-        if (v0 + g >= V) return;
-        const int s = __builtin_amdgcn_readlane(mine, g), e = __builtin_amdgcn_readlane(mine, g + 1);
-        if (e - s > LONG || (accumulate && e == s)) continue;
+    for (int g = 0; g < group && v0 + g < V; ++g) {
+        int e = s0 + __popcll(__ballot((long long)near <= v0 + g));
+        const bool far = e == s0 + 64;
+        if (far) e = segment_end(keys, s > e ? s : e, R, (int)(v0 + g), lane);
         G* dst = grad + (v0 + g) * ldg;
-        for (int c = lane * VEC; c < D; c += 64 * VEC) {
-            float acc[VEC];
+        if (e - s <= LONG && !(accumulate && e == s)) {
+            for (int c = lane * VEC; c < D; c += 64 * VEC) {
+                float acc[VEC];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-            sum_rows<VEC>(dy, ldd, perm, s, e, 1, c, acc);
-            put_row<VEC>(dst + c, acc, scale, accumulate);
+                for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+                if (far) sum_rows<VEC>(dy, ldd, [&](int i) { return perm[i]; }, s, e, 1, c, acc);
+                else if (e > s) sum_rows<VEC>(dy, ldd, [&](int i) { return __builtin_amdgcn_readlane(place, i - s0); }, s, e, 1, c, acc);
+                put_row<VEC>(dst + c, acc, scale, accumulate);
+            }
         }
+        s = e;
     }
 }
 
@@ -284,27 +383,40 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
     __shared__ float red[4][64 * VEC];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long p0 = (long long)blockIdx.x * CHUNK;
-    const int p1 = (int)(p0 + CHUNK < R ? p0 + CHUNK : R);
-    const int k = keys[p1 - 1];
-    if (k >= V) return;
-    const int s = lower_bound(keys, R, k);
-    if (s < (int)p0) return;
-    const int e = lower_bound(keys, R, (long long)k + 1);
-    if (e - s <= LONG) return;
+    const int p0 = (int)blockIdx.x * CHUNK;
+    if (R - p0 <= CHUNK) return;                             // no segment of more than LONG starts in the last places
+    const int kin = keys[p0 + lane];
+    const int k = __builtin_amdgcn_readlane(kin, 63);
+    const int ahead = p0 + CHUNK + lane < R ? keys[p0 + CHUNK + lane] : -1;
+    const int back = p0 > 0 ? keys[p0 - 1] : -1;
+    const unsigned long long here = __ballot(kin == k);
+    const int s = p0 + __builtin_ctzll(here);
+    const unsigned long long on = __ballot(ahead == k);
+    if (k >= V || (s == p0 && back == k) || __popcll(here) + __popcll(on) <= LONG) return;
+    const int e = segment_end(keys, p0 + CHUNK, R, k, lane);
     const int last = (e - 1) / CHUNK;
-    const int slot0 = s == (int)p0 ? 0 : 1;                  // in chunk p; the following ones have it at their first place
+    const int slot0 = s == p0 ? 0 : 1;                       // in chunk p; the following ones have it at their first place
     for (int c0 = 0; c0 < D; c0 += 64 * VEC) {
         const int c = c0 + lane * VEC;
         float acc[VEC];
 #pragma unroll
         for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
         if (c < D) {
-#pragma unroll 4
-            for (int j = (int)blockIdx.x + wave; j <= last; j += 4) {
-                const int slot = j == (int)blockIdx.x ? slot0 : 0;
+            for (int j = (int)blockIdx.x + wave; j <= last; j += 32) {       // eight partial sums in flight
+                float v[8][VEC];
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) acc[q] += part[((size_t)j * 2 + slot) * D + c + q];
+                for (int u = 0; u < 8; ++u) {
+                    const int jj = j + 4 * u;
+                    if (jj <= last) sv_load<VEC>(part + ((size_t)jj * 2 + (jj == (int)blockIdx.x ? slot0 : 0)) * D + c, v[u]);
+                    else {
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) v[u][q] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) acc[q] += v[u][q];
             }
         }
 #pragma unroll
@@ -356,6 +468,10 @@ extern "C" int svae_lookup_fwd(const void* table, int table_type, long long ld_t
 extern "C" int svae_token_sort_bytes(int R, int V, long long* bytes) {
     SV_CHECK_ARG(bytes && R >= 0 && V > 0 && V < 0x7fffffff, "svae_token_sort_bytes: bad arguments");
     const SortShape s = sort_shape(R, V);
+    if (R <= SMALL) {
+        *bytes = 0;
+        return 0;
+    }
     *bytes = align256(4ll * s.nwg << s.bits) + (s.passes > 1 ? 2 * align256(4ll * R) : 0);
     return 0;
 }
@@ -366,17 +482,23 @@ extern "C" int svae_token_sort(const void* tokens, int tok64, int R, int V, int 
     if (R == 0) return 0;
     long long need = 0;
     svae_token_sort_bytes(R, V, &need);
-    SV_CHECK_ARG(tokens && keys && perm && work, "svae_token_sort: null pointer");
+    SV_CHECK_ARG(tokens && keys && perm && (work || need == 0), "svae_token_sort: null pointer");
     SV_CHECK_ARG(work_bytes >= need, "svae_token_sort: workspace of %lld bytes, %lld needed", work_bytes, need);
     const SortShape s = sort_shape(R, V);
     char* w = (char*)work;
     SortArgs a;
     a.tok = tokens; a.tok64 = tok64; a.R = R; a.V = V; a.pad = pad; a.bits = s.bits; a.tile = s.tile;
     a.cnt = (unsigned*)w;
+    a.kin = a.pin = nullptr; a.kout = keys; a.pout = perm; a.shift = 0;
+    if (R <= SMALL) {
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a, s.passes);
+        SV_LAUNCH_CHECK();
+        return 0;
+    }
     w += align256(4ll * s.nwg << s.bits);
     int* k2 = (int*)w;
     int* p2 = (int*)(w + align256(4ll * R));
-    const size_t lds = ((size_t)16 << s.bits) * 4 + 64;
+    const size_t lds = ((size_t)18 << s.bits) * 4 + 64;
     const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (attr != hipSuccess) return svae_fail((int)attr, "svae_token_sort: %s", hipGetErrorString(attr));
     for (int p = 0; p < s.passes; ++p) {
@@ -411,7 +533,9 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
     SV_CHECK_ARG(work_bytes >= need, "svae_lookup_bwd: workspace of %lld bytes, %lld needed", work_bytes, need);
     if (R == 0 && accumulate) return 0;
     const int nchunk = (int)chunks_of(R);
-    const long long nrow = ((long long)V + 4 * GROUP - 1) / (4 * GROUP);
+    // rows of a wave: many where most rows are empty (they are only written), few where most have tokens to wait for
+    const int group = (long long)V >= 8ll * R ? MOST_GROUP : 4;
+    const long long nrow = ((long long)V + 4 * group - 1) / (4 * group);
     SV_CHECK_ARG(nchunk + nrow < 0x7fffffffll, "svae_lookup_bwd: R %d and V %d need too many workgroups", R, V);
     int vec = sv_vec_for(8, D, R ? dy : grad, R ? ld_dy : ld_grad, sv_elem_size(dy_type), grad, ld_grad, sv_elem_size(grad_type));
     while (vec > 2 && 32 * vec >= D) vec >>= 1;              // rather all 64 lanes with shorter vectors
@@ -421,7 +545,7 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
             typedef decltype(o) G;
             auto go = [&](auto kernel, auto join) {
                 hipLaunchKernelGGL(kernel, dim3((unsigned)(nchunk + nrow)), dim3(256), 0, (hipStream_t)stream, (const T*)dy, ld_dy, keys,
-                                   perm, R, V, D, scale, (G*)grad, ld_grad, accumulate, nchunk, (float*)work);
+                                   perm, R, V, D, scale, (G*)grad, ld_grad, accumulate, nchunk, group, (float*)work);
                 if (R > LONG)
                     hipLaunchKernelGGL(join, dim3((unsigned)nchunk), dim3(256), 0, (hipStream_t)stream, keys, R, V, D, scale, (G*)grad,
                                        ld_grad, accumulate, (const float*)work);

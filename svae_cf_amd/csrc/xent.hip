@@ -232,12 +232,12 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
 
 // position in the launch -> tile: consecutive workgroups go to the 8 XCDs in turn; each gets a run of consecutive tiles, so
 // that what they share is fetched into one L2
-__device__ __forceinline__ int tile_of(int total) {
+__device__ __forceinline__ int tile_of(unsigned block, int total) {
     const int per = (total + 7) / 8;
-    const int t = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    return (int)(blockIdx.x >> 3) < per && t < total ? t : -1;
+    const int t = (int)(block & 7) * per + (int)(block >> 3);
+    return (int)(block >> 3) < per && t < total ? t : -1;
 }
-inline unsigned launch_for(long long tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
+inline unsigned blocks_for(long long tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
 
 // (maximum, sum of exponentials above it) of two sets of logits
 __device__ __forceinline__ void join_sums(float& m, float& s, float m2, float s2) {
@@ -265,15 +265,10 @@ struct LogitArgs {
     int V, D, Dp, Rp, v_begin, nvt, nrt;      // vocabulary of this launch: tiles v_begin / 256 ..., nvt of them
 };
 
+// red: [waves along A][BN], for the loss
 template <typename E, int BN, int KIND, int PARTS, bool GRAD>
-__global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) {
+__device__ __forceinline__ void logit_tile(const LogitArgs& a, int tile, char* const (&sa)[STAGES], char* const (&sb)[STAGES], float2 (*red)[BN]) {
     typedef Lay<BN> L;
-    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
-    char* const sa[STAGES] = {a0, a1, a2};
-    char* const sb[STAGES] = {b0, b1, b2};
-    __shared__ float2 red[L::WM][BN];
-    const int tile = tile_of(a.nvt * a.nrt);
-    if (tile < 0) return;
     // bands of 8 row tiles, vocabulary tiles outside: the workgroups of an XCD share a few vocabulary and 8 row tiles
     const int band = tile / (8 * a.nvt), in = tile - band * 8 * a.nvt;
     const int wide = a.nrt - band * 8 < 8 ? a.nrt - band * 8 : 8;
@@ -416,6 +411,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
     }
 }
 
+template <typename E, int BN, int KIND, int PARTS>
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_loss_kernel(LogitArgs a) {
+    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
+    char* const sa[STAGES] = {a0, a1, a2};
+    char* const sb[STAGES] = {b0, b1, b2};
+    __shared__ float2 red[Lay<BN>::WM][BN];
+    const int tile = tile_of(blockIdx.x, a.nvt * a.nrt);
+    if (tile >= 0) logit_tile<E, BN, KIND, PARTS, false>(a, tile, sa, sb, red);
+}
+
 // ------------------------------------------------------------------------------------------------
 // The two gradient products.  A = W or H, up to 256 columns of it a tile (in steps of 32, so that the tiles of a width are alike
 // and nearly full); B = G.
@@ -426,23 +431,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_logit_kernel(LogitArgs a) 
 struct ProductArgs {
     const char* x;            // blocks of W (from the piece's first row on) or of H
     const char* g;            // blocks of G
-    float* slab;              // [splits][rows][Dp], added to when add != 0; NULL: out is written
-    float* bslab;             // [splits][rows] bias gradient, or NULL
+    float* slab;              // [splits][...][Dp] at the first row of this launch, added to when add != 0; NULL: out is written
+    float* bslab;             // [splits][...] bias gradient, or NULL
     void* out;                // [rows][ld_out] of the caller's type
     void* bout;
     const float* scale;       // fp16: scale[1] takes the scale of G out again (written only with the final result)
-    long long x_part, g_part, ld_out, slab_stride;
+    long long x_part, g_part, ld_out, slab_stride, bslab_stride;
     int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
 };
 
 template <typename E, typename T, int BN, int MT, int PARTS, bool OVER_V>
-__global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs a) {
+__device__ __forceinline__ void product_tile(const ProductArgs& a, int tile, char* const (&sa)[STAGES], char* const (&sb)[STAGES]) {
     typedef Lay<BN> L;
-    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[BN * BK * 2], b1[BN * BK * 2], b2[BN * BK * 2];
-    char* const sa[STAGES] = {a0, a1, a2};
-    char* const sb[STAGES] = {b0, b1, b2};
-    const int tile = tile_of(a.ndt * a.nnt * a.splits);
-    if (tile < 0) return;
     const int dt = tile % a.ndt, nt = tile / a.ndt % a.nnt, split = tile / (a.ndt * a.nnt);
     const int k0 = (int)((long long)a.steps * split / a.splits), k1 = (int)((long long)a.steps * (split + 1) / a.splits);
 
@@ -503,38 +503,74 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_product_kernel(ProductArgs
             }
         }
         if (!OVER_V && dt == 0 && w0 == 0 && q == 0) {
-            if (a.bslab != nullptr) a.bslab[(long long)split * a.rows + r] = cs[n][0];
+            if (a.bslab != nullptr) a.bslab[split * a.bslab_stride + r] = cs[n][0];
             else if (a.bout != nullptr) reinterpret_cast<T*>(a.bout)[r] = (T)(cs[n][0] * down);
         }
     }
 }
 
-// out[r][d] = sum of the slabs, in order; also the bias gradient's (bslabs [splits][rows]; the last workgroups)
-template <typename T>
-__global__ __launch_bounds__(256) void xent_slab_sum_kernel(const float* __restrict__ slab, long long slab_stride, int splits, int rows,
-                                                            int D, int Dp, T* __restrict__ out, long long ld_out,
-                                                            const float* __restrict__ bslab, T* __restrict__ bout,
-                                                            const float* __restrict__ scale, unsigned nmain) {
-    const float down = scale != nullptr ? scale[1] : 1.f;
-    if (blockIdx.x < nmain) {
-        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-        const int per = Dp / 4;
-        const long long r = i / per;
-        const int d = (int)(i - r * per) * 4;
-        if (r >= rows || d >= D) return;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(slab + k * slab_stride + r * Dp + d);
-        T* o = out + r * ld_out + d;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (d + j < D) o[j] = (T)(s[j] * down);
+// One launch of the gradient: G of one piece of the vocabulary, and the products of the piece before (its G is in the other of
+// two buffers).  The long workgroups come first, the short tiles of G fill what they leave.
+struct PieceArgs {
+    LogitArgs z;
+    ProductArgs h, w;
+    unsigned nh, nw;          // workgroups of dH and of dW, multiples of 8; the rest make G
+};
+
+template <typename E, typename T, int BN, int MT, int PARTS>
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_piece_kernel(PieceArgs a) {
+    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[128 * BK * 2], b1[128 * BK * 2], b2[128 * BK * 2];
+    char* const sa[STAGES] = {a0, a1, a2};
+    char* const sb[STAGES] = {b0, b1, b2};
+    if (blockIdx.x < a.nw) {
+        const int tile = tile_of(blockIdx.x, a.w.ndt * a.w.nnt * a.w.splits);
+        if (tile >= 0) product_tile<E, T, 128, MT, PARTS, false>(a.w, tile, sa, sb);
+    } else if (blockIdx.x < a.nw + a.nh) {
+        const int tile = tile_of(blockIdx.x - a.nw, a.h.ndt * a.h.nnt * a.h.splits);
+        if (tile >= 0) product_tile<E, T, BN, BN == 64 ? MT / 2 : MT, PARTS, true>(a.h, tile, sa, sb);
     } else {
-        const long long r = (long long)(blockIdx.x - nmain) * 256 + threadIdx.x;
-        if (r >= rows) return;
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += bslab[(long long)k * rows + r];
-        bout[r] = (T)(s * down);
+        const int tile = tile_of(blockIdx.x - a.nw - a.nh, a.z.nvt * a.z.nrt);
+        if (tile >= 0) logit_tile<E, BN, ALONG, PARTS, true>(a.z, tile, sa, sb, (float2(*)[BN])nullptr);
     }
+}
+
+// out[r][d] = sum of the slabs, in order; the slabs of dH, of dW and of the bias gradient in one launch
+struct SumArgs {
+    const float* slab;
+    void* out;
+    const float* scale;
+    long long slab_stride, ld_out;
+    int splits, rows, D, Dp;              // (the bias gradient: one column, Dp = 1)
+    unsigned blocks;
+};
+template <typename T>
+__device__ __forceinline__ void sum_slabs(const SumArgs& a, unsigned block) {
+    const float down = a.scale != nullptr ? a.scale[1] : 1.f;
+    const long long i = (long long)block * 256 + threadIdx.x;
+    if (a.Dp == 1) {
+        if (i >= a.rows) return;
+        float s = 0.f;
+        for (int k = 0; k < a.splits; ++k) s += a.slab[k * a.slab_stride + i];
+        reinterpret_cast<T*>(a.out)[i] = (T)(s * down);
+        return;
+    }
+    const int per = a.Dp / 4;
+    const long long r = i / per;
+    const int d = (int)(i - r * per) * 4;
+    if (r >= a.rows || d >= a.D) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < a.splits; ++k) s += *reinterpret_cast<const f32x4*>(a.slab + k * a.slab_stride + r * a.Dp + d);
+    T* o = reinterpret_cast<T*>(a.out) + r * a.ld_out + d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (d + j < a.D) o[j] = (T)(s[j] * down);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void xent_slab_sum_kernel(SumArgs h, SumArgs w, SumArgs b) {
+    if (blockIdx.x < h.blocks) sum_slabs<T>(h, blockIdx.x);
+    else if (blockIdx.x < h.blocks + w.blocks) sum_slabs<T>(w, blockIdx.x - h.blocks);
+    else sum_slabs<T>(b, blockIdx.x - h.blocks - w.blocks);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -545,8 +581,8 @@ __global__ __launch_bounds__(256) void xent_slab_sum_kernel(const float* __restr
 struct PrepArgs {
     const void *h, *w, *bias, *tok;
     const float *row_weight, *lse;        // NULL: loss only
-    char *hc, *wc;                        // wc NULL: W is not copied, and hc has rows
-    float *biasf, *wrow, *lsec;
+    char *hc, *hg, *wc;                   // hg (or NULL): without the rows of weight 0; wc NULL: W is not copied, and hc has rows
+    float *biasf, *wrow, *lsec;           // lsec: a copy of lse, where it is given
     int* tgt;
     long long ldh, ldw, h_part, w_part;
     int tok64, R, Rp, V, Vp, D, Dp, nh, nb, wide_h, wide_w;
@@ -597,16 +633,15 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
             if (t >= 0 && t < a.V) tg = (int)t;
             if (tg >= 0 && a.row_weight != nullptr) w = a.row_weight[r];
         }
-        const bool live = tg >= 0 && (a.row_weight == nullptr || w != 0.f);
         if (c == 0) {
             a.tgt[r] = tg;
-            if (a.row_weight != nullptr) {
-                a.wrow[r] = w;
-                a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
-            }
+            if (a.row_weight != nullptr) a.wrow[r] = w;
+            if (a.lse != nullptr) a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
         }
-        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.h) + (live ? r : 0) * a.ldh + c, a.D - c, live, a.wide_h,
-                           a.hc + (a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2), a.h_part);
+        const T* src = reinterpret_cast<const T*>(a.h) + (tg >= 0 ? r : 0) * a.ldh + c;
+        const long long to = a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2;
+        if (a.hc != nullptr) copy8<T, E, PARTS>(src, a.D - c, tg >= 0, a.wide_h, a.hc + to, a.h_part);
+        if (a.hg != nullptr) copy8<T, E, PARTS>(src, a.D - c, w != 0.f, a.wide_h, a.hg + to, a.h_part);
     } else if ((int)blockIdx.x < a.nh + a.nb) {
         const long long v = i - (long long)a.nh * 256;
         if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
@@ -622,7 +657,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
 template <int SLICES>
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
                                                         const int* __restrict__ tgt, int R, int Rp, int nvt,
-                                                        float* __restrict__ nll, float* __restrict__ lse) {
+                                                        float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ lsec) {
     constexpr int ROWS = 256 / SLICES;
     __shared__ float2 red[SLICES][ROWS + 1];
     const int i = threadIdx.x % ROWS, s = threadIdx.x / ROWS;
@@ -638,10 +673,12 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
     }
     red[s][i] = make_float2(m, sum);
     __syncthreads();
-    if ((int)threadIdx.x >= ROWS || r >= R) return;
+    if ((int)threadIdx.x >= ROWS) return;
     for (int k = 1; k < SLICES; ++k) join_sums(m, sum, red[k][i].x, red[k][i].y);
     const bool here = tgt[r] >= 0;
     const float l = m + logf(sum);
+    if (lsec != nullptr) lsec[r] = here ? l : 0.f;
+    if (r >= R) return;
     lse[r] = here ? l : 0.f;
     nll[r] = here ? l - zt[r] : 0.f;
 }
@@ -697,32 +734,28 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restric
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
-constexpr long long PIECE_BYTES = 1ll << 30;             // what G of one piece may take
+constexpr long long PIECE_LEAST = 128ll << 20, PIECE_MOST = 512ll << 20;     // what G of a piece may take; there are two
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
-    int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, dh_splits, dw_splits, ndt, dblocks;
-    long long h, h_part, w, w_part, ldw, bias, tgt, wrow, zt, part, scale, g, g_part, dh_slab, dw_slab, db_slab, total;
+    int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, h_splits, w_splits, ndt, dblocks;
+    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab, b_slab, total;
 };
 
-// parts of the contraction: least (rounds of workgroups) x (steps of each + what a workgroup costs beside them), plus the slabs'
-// traffic, in steps of about a microsecond
-inline int pick_splits(long long tiles, int steps, long long slab_bytes) {
-    int best = 1;
-    double least = 1e30;
-    for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
-        const double cost = (double)((tiles * s + SLOTS - 1) / SLOTS) * ((steps + s - 1) / s + 3) + (s > 1 ? 2.0 * s * slab_bytes / 4e6 + 4 : 0);
-        if (cost < least * 0.98) { least = cost; best = s; }
-    }
-    return best;
+// parts of a product's contraction: no workgroup should work longer than a slot's share of the launch
+inline int splits_for(double unit, double whole) {
+    const double s = unit * SLOTS / whole;
+    return s <= 1.0 ? 1 : s >= 32.0 ? 32 : (int)(s + 0.999);
 }
+
+enum { LOSS = 0, GRADIENT = 1 };
 
 inline int shape_of(const void* weight, long long ld_w, int type, long long R, long long V, long long D, int grad, Shape* s) {
     SV_CHECK_ARG(type >= 0 && type <= 2, "svae_xent: type %d", type);
     SV_CHECK_ARG(R > 0 && R <= 1 << 24 && V > 0 && V <= 1 << 28 && D > 0 && D <= 1 << 16 && ld_w >= D && ld_w <= 1 << 20,
                  "svae_xent: sizes R %lld, V %lld, D %lld, ld %lld", R, V, D, ld_w);
     s->parts = type == SV_F32 ? 3 : 1;
-    s->direct = !grad && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
+    s->direct = grad == LOSS && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
     s->BN = R <= 64 ? 64 : 128;
     s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
     s->Vp = (int)((V + BM - 1) / BM * BM);
@@ -742,28 +775,42 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     };
     s->h_part = (long long)s->Rp * s->Dp * 2;
     s->h = take(s->h_part * s->parts);
+    s->hg = grad == LOSS ? 0 : take(s->h_part * s->parts);
     s->w_part = s->direct ? 0 : (long long)s->Vp * s->Dp * 2;
     s->ldw = ld_w * 2;
     s->w = take(s->w_part * s->parts);
     s->bias = take(4ll * s->Vp);
     s->tgt = take(4ll * s->Rp);
     s->wrow = take(4ll * s->Rp);
+    s->lse = take(4ll * s->Rp);
     s->zt = take(4ll * s->Rp);
     s->scale = take(8);
-    s->g = s->part = at;                                   // the loss's statistics and the gradient's pieces share the rest
-    long long end = at + 8ll * s->nvt * s->Rp;
-    if (grad) {
-        long long tiles = PIECE_BYTES / (2ll * s->parts * s->Rp * BM);
+    s->part = s->g[0] = at;                                // the loss's statistics are done with when G is made
+    const long long end = at + 8ll * s->nvt * s->Rp;
+    if (grad != LOSS) {
+        // A piece's G is written and read twice: small pieces stay near the chip (21800 x 20000 x 200, bf16: G from HBM takes
+        // longer than its products).  Every piece adds to all of dH, so that a piece is at least 16 times dH's sums.
+        long long bytes = 64ll * s->Rp * s->Dp;
+        bytes = bytes < PIECE_LEAST ? PIECE_LEAST : bytes > PIECE_MOST ? PIECE_MOST : bytes;
+        long long tiles = bytes / (2ll * s->parts * s->Rp * BM);
         tiles = tiles < 1 ? 1 : tiles > s->nvt ? s->nvt : tiles;
         s->pieces = (int)((s->nvt + tiles - 1) / tiles);
         s->piece_tiles = (s->nvt + s->pieces - 1) / s->pieces;
+        s->pieces = (s->nvt + s->piece_tiles - 1) / s->piece_tiles;
         s->g_part = 2ll * s->Rp * s->piece_tiles * BM;
-        s->g = take(s->g_part * s->parts);
-        s->dh_splits = pick_splits((long long)s->ndt * s->nrt, s->piece_tiles * (BM / BK) * (s->parts == 1 ? 1 : 6), 4ll * s->Rp * s->Dp);
-        s->dh_slab = take(4ll * s->Rp * s->Dp * s->dh_splits);
-        s->dw_splits = pick_splits((long long)s->ndt * s->piece_tiles * (BM / 128), s->Rp / BK * (s->parts == 1 ? 1 : 6), 4ll * s->piece_tiles * BM * s->Dp);
-        s->dw_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->Dp * s->dw_splits : 0);
-        s->db_slab = take(s->dw_splits > 1 ? 4ll * s->piece_tiles * BM * s->dw_splits : 0);
+        s->g[0] = take(s->g_part * s->parts);
+        s->g[1] = s->pieces > 1 ? take(s->g_part * s->parts) : s->g[0];
+        // steps of 32 in a launch (a tile of G: as many as its epilogue takes, about ten, beside its own)
+        const double k = s->parts == 1 ? 1 : 6, h_unit = k * s->piece_tiles * (BM / BK), w_unit = k * (s->Rp / BK);
+        const double h_all = h_unit * s->ndt * s->nrt, w_all = w_unit * s->ndt * s->piece_tiles * (BM / 128);
+        const double z_all = s->pieces > 1 ? (k * (s->Dp / BK) + 10) * s->piece_tiles * s->nrt : 0;
+        s->h_splits = splits_for(h_unit, h_all + w_all + z_all);
+        s->w_splits = splits_for(w_unit, h_all + w_all + z_all);
+        if (s->h_splits > s->piece_tiles * (BM / BK) / 4) s->h_splits = s->piece_tiles * (BM / BK) / 4;
+        if (s->w_splits > s->Rp / BK / 2) s->w_splits = s->Rp / BK / 2;
+        s->h_slab = take(4ll * s->Rp * s->Dp * s->h_splits);
+        s->w_slab = take(s->w_splits > 1 ? 4ll * s->Vp * s->Dp * s->w_splits : 0);
+        s->b_slab = take(s->w_splits > 1 ? 4ll * s->Vp * s->w_splits : 0);
     }
     s->total = at > end ? at : end;
     return 0;
@@ -785,14 +832,14 @@ inline void by_type(int type, F f) {
     else f(_Float16{}, _Float16{}, std::integral_constant<int, 1>{});
 }
 
-inline int prepare(const Call& c, const Shape& s, const float* row_weight, const float* lse) {
+// loss: whether the rows with a target are wanted; row_weight: the rows of the gradient are; lse: fwd's, where it is not to be made
+inline int prepare(const Call& c, const Shape& s, bool loss, const float* row_weight, const float* lse) {
     PrepArgs p;
-    p.lse = lse;
-    p.lsec = (float*)(c.work + s.zt);
-    p.h = c.hidden; p.w = c.weight; p.bias = c.bias; p.tok = c.targets; p.row_weight = row_weight;
-    p.hc = c.work + s.h;
+    p.h = c.hidden; p.w = c.weight; p.bias = c.bias; p.tok = c.targets; p.row_weight = row_weight; p.lse = lse;
+    p.hc = loss ? c.work + s.h : nullptr;
+    p.hg = row_weight != nullptr ? c.work + s.hg : nullptr;
     p.wc = s.direct ? nullptr : c.work + s.w;
-    p.biasf = (float*)(c.work + s.bias); p.wrow = (float*)(c.work + s.wrow); p.tgt = (int*)(c.work + s.tgt);
+    p.biasf = (float*)(c.work + s.bias); p.wrow = (float*)(c.work + s.wrow); p.tgt = (int*)(c.work + s.tgt); p.lsec = (float*)(c.work + s.lse);
     p.ldh = c.ld_h; p.ldw = c.ld_w; p.h_part = s.h_part; p.w_part = s.w_part;
     p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.Vp = s.Vp; p.D = c.D; p.Dp = s.Dp;
     const long long nh = ((long long)s.Rp * (s.Dp / 8) + 255) / 256, nb = (s.Vp + 255) / 256,
@@ -820,48 +867,130 @@ inline LogitArgs logit_args(const Call& c, const Shape& s) {
     return a;
 }
 
-template <bool GRAD>
-inline void logits(const Call& c, const Shape& s, const LogitArgs& a) {
+inline int loss(const Call& c, const Shape& s, float* nll, float* lse, float* lsec) {
+    LogitArgs a = logit_args(c, s);
+    a.part = (float2*)(c.work + s.part);
+    a.zt = (float*)(c.work + s.zt);
+    a.v_begin = 0; a.nvt = s.nvt;
     by_type(c.type, [&](auto, auto e, auto parts) {
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
-        const dim3 grid(launch_for((long long)a.nvt * a.nrt));
+        const dim3 grid(blocks_for((long long)a.nvt * a.nrt));
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, a); };
-        if constexpr (!GRAD && P == 1) {
+        if constexpr (P == 1) {
             if (s.direct) {
-                if (s.BN == 64) go(xent_logit_kernel<E, 64, PLAIN, P, GRAD>);
-                else go(xent_logit_kernel<E, 128, PLAIN, P, GRAD>);
+                if (s.BN == 64) go(xent_loss_kernel<E, 64, PLAIN, P>);
+                else go(xent_loss_kernel<E, 128, PLAIN, P>);
                 return;
             }
         }
-        if (s.BN == 64) go(xent_logit_kernel<E, 64, ALONG, P, GRAD>);
-        else go(xent_logit_kernel<E, 128, ALONG, P, GRAD>);
+        if (s.BN == 64) go(xent_loss_kernel<E, 64, ALONG, P>);
+        else go(xent_loss_kernel<E, 128, ALONG, P>);
     });
+    SV_LAUNCH_CHECK();
+    // few rows and many tiles: more threads a row
+    if ((long long)s.Rp * 8 < s.nvt * 64ll)
+        hipLaunchKernelGGL(xent_rows_kernel<64>, dim3(s.Rp / 4), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
+    else
+        hipLaunchKernelGGL(xent_rows_kernel<8>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
+    SV_LAUNCH_CHECK();
+    return 0;
 }
 
-template <bool OVER_V>
-inline void products(const Call& c, const Shape& s, const ProductArgs& d) {
+inline void piece(const Call& c, const Shape& s, const PieceArgs& a, unsigned blocks) {
     by_type(c.type, [&](auto t, auto e, auto parts) {
         typedef decltype(t) T;
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
-        const dim3 grid(launch_for((long long)d.ndt * d.nnt * d.splits));
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, d); };
-        if (s.dblocks == 2) go(xent_product_kernel<E, T, 128, 2, P, OVER_V>);
-        else if (s.dblocks == 4) go(xent_product_kernel<E, T, 128, 4, P, OVER_V>);
-        else if (s.dblocks == 5) go(xent_product_kernel<E, T, 128, 5, P, OVER_V>);
-        else if (s.dblocks == 6) go(xent_product_kernel<E, T, 128, 6, P, OVER_V>);
-        else if (s.dblocks == 7) go(xent_product_kernel<E, T, 128, 7, P, OVER_V>);
-        else {
-            if constexpr (OVER_V) {
-                if (s.BN == 64) {
-                    go(xent_product_kernel<E, T, 64, 4, P, true>);
-                    return;
-                }
-            }
-            go(xent_product_kernel<E, T, 128, 8, P, OVER_V>);
-        }
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, c.stream, a); };
+        if (s.BN == 64) go(xent_piece_kernel<E, T, 64, 8, P>);
+        else if (s.dblocks == 2) go(xent_piece_kernel<E, T, 128, 2, P>);
+        else if (s.dblocks == 4) go(xent_piece_kernel<E, T, 128, 4, P>);
+        else if (s.dblocks == 5) go(xent_piece_kernel<E, T, 128, 5, P>);
+        else if (s.dblocks == 6) go(xent_piece_kernel<E, T, 128, 6, P>);
+        else if (s.dblocks == 7) go(xent_piece_kernel<E, T, 128, 7, P>);
+        else go(xent_piece_kernel<E, T, 128, 8, P>);
     });
+}
+
+// h: the rows of H that tiles of z are made from (the loss's or the gradient's copy; rows of weight 0 come to nothing either way)
+inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db) {
+    const float* scale = nullptr;
+    if (c.type == SV_F16) {
+        scale = (const float*)(c.work + s.scale);
+        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, c.stream, (const float*)(c.work + s.wrow), s.Rp, (float*)(c.work + s.scale));
+        SV_LAUNCH_CHECK();
+    }
+    const int es = sv_elem_size(c.type);
+    LogitArgs z = logit_args(c, s);
+    z.h = c.work + h;
+    z.lse = (const float*)(c.work + s.lse); z.wrow = (const float*)(c.work + s.wrow); z.scale = scale;
+    ProductArgs d{};
+    d.scale = scale; d.g_part = s.g_part; d.D = c.D; d.Dp = s.Dp; d.ndt = s.ndt;
+    float* const wslab = s.w_splits > 1 ? (float*)(c.work + s.w_slab) : nullptr;
+    float* const bslab = s.w_splits > 1 && db ? (float*)(c.work + s.b_slab) : nullptr;
+    for (int p = 0; p <= s.pieces; ++p) {                  // launch p: G of piece p, products of piece p - 1
+        PieceArgs a{};
+        unsigned nz = 0;
+        if (p < s.pieces) {
+            const int t0 = p * s.piece_tiles;
+            a.z = z;
+            a.z.v_begin = t0 * BM;
+            a.z.nvt = s.nvt - t0 < s.piece_tiles ? s.nvt - t0 : s.piece_tiles;
+            a.z.g = c.work + s.g[p & 1];
+            nz = blocks_for((long long)a.z.nvt * a.z.nrt);
+        }
+        if (p > 0) {
+            const int t0 = (p - 1) * s.piece_tiles, nt = s.nvt - t0 < s.piece_tiles ? s.nvt - t0 : s.piece_tiles;
+            const long long v0 = (long long)t0 * BM;
+            d.g = c.work + s.g[(p - 1) & 1];
+            d.nv32 = nt * (BM / 32);
+            if (dh) {
+                a.h = d;
+                a.h.x = c.work + s.w + v0 * s.Dp * 2; a.h.x_part = s.w_part;
+                a.h.slab = (float*)(c.work + s.h_slab); a.h.slab_stride = (long long)s.Rp * s.Dp;
+                a.h.rows = s.Rp; a.h.nnt = s.nrt; a.h.splits = s.h_splits; a.h.steps = nt * (BM / BK); a.h.add = p > 1;
+                a.nh = blocks_for((long long)a.h.ndt * a.h.nnt * a.h.splits);
+            }
+            if (dw) {
+                a.w = d;
+                a.w.x = c.work + s.hg; a.w.x_part = s.h_part;
+                a.w.rows = (int)(c.V - v0 < (long long)nt * BM ? c.V - v0 : (long long)nt * BM);
+                a.w.nnt = nt * (BM / 128); a.w.splits = s.w_splits; a.w.steps = s.Rp / BK; a.w.add = 0;
+                a.w.out = (char*)dw + v0 * ld_dw * es; a.w.ld_out = ld_dw;
+                a.w.bout = db ? (char*)db + v0 * es : nullptr;
+                a.w.slab = wslab ? wslab + v0 * s.Dp : nullptr; a.w.slab_stride = (long long)s.Vp * s.Dp;
+                a.w.bslab = bslab ? bslab + v0 : nullptr; a.w.bslab_stride = s.Vp;
+                const int wide = es * 4 < 16 ? es * 4 : 16;
+                a.w.out_vec = c.D % 4 == 0 && ld_dw * es % wide == 0 && (unsigned long long)a.w.out % wide == 0;
+                a.nw = blocks_for((long long)a.w.ndt * a.w.nnt * a.w.splits);
+            }
+        }
+        piece(c, s, a, nz + a.nh + a.nw);
+        SV_LAUNCH_CHECK();
+    }
+    SumArgs h1{}, w1{}, b1{};
+    if (dh) {
+        h1.slab = (const float*)(c.work + s.h_slab); h1.slab_stride = (long long)s.Rp * s.Dp; h1.out = dh; h1.ld_out = ld_dh;
+        h1.scale = scale; h1.splits = s.h_splits; h1.rows = c.R; h1.D = c.D; h1.Dp = s.Dp;
+        h1.blocks = (unsigned)(((long long)c.R * (s.Dp / 4) + 255) / 256);
+    }
+    if (dw && wslab) {
+        w1.slab = wslab; w1.slab_stride = (long long)s.Vp * s.Dp; w1.out = dw; w1.ld_out = ld_dw;
+        w1.scale = scale; w1.splits = s.w_splits; w1.rows = c.V; w1.D = c.D; w1.Dp = s.Dp;
+        w1.blocks = (unsigned)(((long long)c.V * (s.Dp / 4) + 255) / 256);
+    }
+    if (db && bslab) {
+        b1.slab = bslab; b1.slab_stride = s.Vp; b1.out = db; b1.scale = scale; b1.splits = s.w_splits; b1.rows = c.V; b1.D = b1.Dp = 1;
+        b1.blocks = (unsigned)((c.V + 255) / 256);
+    }
+    if (h1.blocks + w1.blocks + b1.blocks > 0) {
+        by_type(c.type, [&](auto t, auto, auto) {
+            hipLaunchKernelGGL(xent_slab_sum_kernel<decltype(t)>, dim3(h1.blocks + w1.blocks + b1.blocks), dim3(256), 0, c.stream, h1, w1, b1);
+        });
+        SV_LAUNCH_CHECK();
+    }
+    return 0;
 }
 
 inline int check_call(const char* name, const Call& c, const void* work, long long work_bytes, int grad, Shape* s) {
@@ -873,13 +1002,19 @@ inline int check_call(const char* name, const Call& c, const void* work, long lo
     SV_CHECK_ARG(work_bytes >= s->total, "%s: workspace of %lld bytes, %lld needed", name, work_bytes, s->total);
     return 0;
 }
+inline int check_gradients(const char* name, int D, const float* row_weight, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db) {
+    SV_CHECK_ARG(row_weight, "%s: null pointer", name);
+    SV_CHECK_ARG((!dh || ld_dh >= D) && (!dw || ld_dw >= D), "%s: ld %lld, %lld below D %d", name, ld_dh, ld_dw, D);
+    SV_CHECK_ARG(!db || dw, "%s: the bias gradient comes with the weight gradient", name);
+    return 0;
+}
 
 }  // namespace
 
-extern "C" int svae_xent_bytes(const void* weight, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes) {
+extern "C" int svae_xent_bytes(int weight_align, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes) {
     SV_CHECK_ARG(bytes != nullptr, "svae_xent_bytes: null pointer");
     Shape s{};
-    const int rc = shape_of(weight, ld_w, type, R, V, D, grad, &s);
+    const int rc = shape_of((const void*)(size_t)(weight_align & 15), ld_w, type, R, V, D, grad ? GRADIENT : LOSS, &s);
     if (rc != 0) return rc;
     *bytes = s.total;
     return 0;
@@ -890,24 +1025,12 @@ extern "C" int svae_xent_fwd(const void* hidden, long long ld_h, const void* wei
                              long long work_bytes, void* stream) {
     Call c{hidden, weight, bias, targets, ld_h, ld_w, tok64, type, R, V, D, (char*)work, (hipStream_t)stream};
     Shape s{};
-    int rc = check_call("svae_xent_fwd", c, work, work_bytes, 0, &s);
+    int rc = check_call("svae_xent_fwd", c, work, work_bytes, LOSS, &s);
     if (rc != 0) return rc;
     SV_CHECK_ARG(nll && lse, "svae_xent_fwd: null pointer");
-    rc = prepare(c, s, nullptr, nullptr);
+    rc = prepare(c, s, true, nullptr, nullptr);
     if (rc != 0) return rc;
-    LogitArgs a = logit_args(c, s);
-    a.part = (float2*)(c.work + s.part);
-    a.zt = (float*)(c.work + s.zt);
-    a.v_begin = 0; a.nvt = s.nvt;
-    logits<false>(c, s, a);
-    SV_LAUNCH_CHECK();
-    // few rows and many tiles: more threads a row
-    if ((long long)s.Rp * 8 < s.nvt * 64ll)
-        hipLaunchKernelGGL(xent_rows_kernel<64>, dim3(s.Rp / 4), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
-    else
-        hipLaunchKernelGGL(xent_rows_kernel<8>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, R, s.Rp, s.nvt, nll, lse);
-    SV_LAUNCH_CHECK();
-    return 0;
+    return loss(c, s, nll, lse, nullptr);
 }
 
 extern "C" int svae_xent_reduce(const float* nll, const void* targets, int tok64, int R, int V, int mean, float* out, void* stream) {
@@ -923,75 +1046,28 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
                              long long work_bytes, void* stream) {
     Call c{hidden, weight, bias, targets, ld_h, ld_w, tok64, type, R, V, D, (char*)work, (hipStream_t)stream};
     Shape s{};
-    int rc = check_call("svae_xent_bwd", c, work, work_bytes, 1, &s);
+    int rc = check_call("svae_xent_bwd", c, work, work_bytes, GRADIENT, &s);
+    if (rc == 0) rc = check_gradients("svae_xent_bwd", D, row_weight, dh, ld_dh, dw, ld_dw, db);
     if (rc != 0) return rc;
-    SV_CHECK_ARG(lse && row_weight, "svae_xent_bwd: null pointer");
-    SV_CHECK_ARG((!dh || ld_dh >= D) && (!dw || ld_dw >= D), "svae_xent_bwd: ld %lld, %lld below D %d", ld_dh, ld_dw, D);
-    SV_CHECK_ARG(!db || dw, "svae_xent_bwd: the bias gradient comes with the weight gradient");
+    SV_CHECK_ARG(lse, "svae_xent_bwd: null pointer");
     if (!dh && !dw) return 0;
-    rc = prepare(c, s, row_weight, lse);
+    rc = prepare(c, s, false, row_weight, lse);
     if (rc != 0) return rc;
-    LogitArgs a = logit_args(c, s);
-    a.lse = (const float*)(c.work + s.zt);
-    a.wrow = (const float*)(c.work + s.wrow);
-    a.g = c.work + s.g;
-    const float* scale = nullptr;
-    if (type == SV_F16) {
-        scale = (const float*)(c.work + s.scale);
-        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, c.stream, a.wrow, s.Rp, (float*)(c.work + s.scale));
-        SV_LAUNCH_CHECK();
-    }
-    a.scale = scale;
-    const int es = sv_elem_size(type);
-    for (int p = 0; p < s.pieces; ++p) {
-        const int t0 = p * s.piece_tiles, nt = s.nvt - t0 < s.piece_tiles ? s.nvt - t0 : s.piece_tiles;
-        if (nt <= 0) break;
-        const long long v0 = (long long)t0 * BM;
-        const int rows_v = (int)(V - v0 < (long long)nt * BM ? V - v0 : (long long)nt * BM);
-        a.v_begin = (int)v0; a.nvt = nt;
-        logits<true>(c, s, a);
-        SV_LAUNCH_CHECK();
-        ProductArgs d{};
-        d.g = a.g; d.scale = scale; d.g_part = s.g_part; d.D = D; d.Dp = s.Dp; d.ndt = s.ndt; d.nv32 = nt * (BM / 32);
-        if (dh) {
-            d.x = a.w + v0 * s.Dp * 2;
-            d.x_part = s.w_part;
-            d.slab = (float*)(c.work + s.dh_slab); d.slab_stride = (long long)s.Rp * s.Dp;
-            d.rows = s.Rp; d.nnt = s.nrt; d.splits = s.dh_splits; d.steps = nt * (BM / BK); d.add = p > 0;
-            products<true>(c, s, d);
-            SV_LAUNCH_CHECK();
-        }
-        if (dw) {
-            d.x = a.h; d.x_part = s.h_part;
-            d.rows = rows_v; d.nnt = nt * (BM / 128); d.splits = s.dw_splits; d.steps = s.Rp / BK; d.add = 0;
-            d.out = (char*)dw + v0 * ld_dw * es; d.ld_out = ld_dw;
-            d.bout = db ? (char*)db + v0 * es : nullptr;
-            d.slab = s.dw_splits > 1 ? (float*)(c.work + s.dw_slab) : nullptr;
-            d.bslab = s.dw_splits > 1 && db ? (float*)(c.work + s.db_slab) : nullptr;
-            d.slab_stride = (long long)s.piece_tiles * BM * s.Dp;
-            const int wide = es * 4 < 16 ? es * 4 : 16;
-            d.out_vec = D % 4 == 0 && ld_dw * es % wide == 0 && (unsigned long long)d.out % wide == 0;
-            products<false>(c, s, d);
-            SV_LAUNCH_CHECK();
-            if (d.slab != nullptr) {
-                by_type(type, [&](auto t, auto, auto) {
-                    typedef decltype(t) T;
-                    const unsigned nmain = (unsigned)(((long long)rows_v * (s.Dp / 4) + 255) / 256), nbias = db ? (rows_v + 255) / 256 : 0;
-                    hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain + nbias), dim3(256), 0, c.stream, d.slab, d.slab_stride, d.splits, rows_v, D,
-                                       s.Dp, (T*)d.out, ld_dw, d.bslab, (T*)d.bout, scale, nmain);
-                });
-                SV_LAUNCH_CHECK();
-            }
-        }
-    }
-    if (dh) {
-        by_type(type, [&](auto t, auto, auto) {
-            typedef decltype(t) T;
-            const unsigned nmain = (unsigned)(((long long)R * (s.Dp / 4) + 255) / 256);
-            hipLaunchKernelGGL(xent_slab_sum_kernel<T>, dim3(nmain), dim3(256), 0, c.stream, (const float*)(c.work + s.dh_slab), (long long)s.Rp * s.Dp,
-                               s.dh_splits, R, D, s.Dp, (T*)dh, ld_dh, (const float*)nullptr, (T*)nullptr, scale, nmain);
-        });
-        SV_LAUNCH_CHECK();
-    }
-    return 0;
+    return gradients(c, s, s.hg, dh, ld_dh, dw, ld_dw, db);
+}
+
+extern "C" int svae_xent_fwd_bwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                                 const void* targets, int tok64, int type, int R, int V, int D, const float* row_weight, float* nll,
+                                 float* lse, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db, void* work,
+                                 long long work_bytes, void* stream) {
+    Call c{hidden, weight, bias, targets, ld_h, ld_w, tok64, type, R, V, D, (char*)work, (hipStream_t)stream};
+    Shape s{};
+    int rc = check_call("svae_xent_fwd_bwd", c, work, work_bytes, GRADIENT, &s);
+    if (rc == 0) rc = check_gradients("svae_xent_fwd_bwd", D, row_weight, dh, ld_dh, dw, ld_dw, db);
+    if (rc != 0) return rc;
+    SV_CHECK_ARG(nll && lse, "svae_xent_fwd_bwd: null pointer");
+    rc = prepare(c, s, true, row_weight, nullptr);
+    if (rc == 0) rc = loss(c, s, nll, lse, (float*)(c.work + s.lse));
+    if (rc != 0 || (!dh && !dw)) return rc;
+    return gradients(c, s, s.h, dh, ld_dh, dw, ld_dw, db);
 }

@@ -13,6 +13,7 @@ Conventions
 ``linear_nll_grad`` are the same kernels for programs that run their own backward pass (and for graph capture).
 """
 import ctypes
+import functools
 
 import torch
 
@@ -21,18 +22,21 @@ from . import _lib
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 class _On:
-    """The device of a tensor as the current one, for the time of a call."""
+    """The device of a tensor as the current one, for the time of a call; gives that device's current stream."""
     __slots__ = ("index", "back")
 
     def __init__(self, t):
-        self.index = t.device.index
+        self.index = t.get_device()
 
     def __enter__(self):
         self.back = torch.cuda.current_device()
         if self.back != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.back != self.index:
@@ -40,31 +44,41 @@ class _On:
 
 
 def _check(t, what, types=_TYPES, device=None):
+    """Type code of a tensor that has one of `types` and is on the GPU (the one of `device`, a number, if given)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor, got %s" % (what, type(t).__name__))
-    if t.dtype not in types:
+    code = types.get(t.dtype)
+    if code is None:
         raise TypeError("%s has type %s: %s are supported" % (what, t.dtype, ", ".join(str(k)[6:] for k in types)))
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError("%s is on %s: the HIP path has no CPU fallback" % (what, t.device))
-    if device is not None and t.device != device:
-        raise ValueError("%s is on %s, the other tensors on %s" % (what, t.device, device))
-    return t
+    if device is not None and t.get_device() != device:
+        raise ValueError("%s is on %s, the other tensors on cuda:%d" % (what, t.device, device))
+    return code
 
 
 _IDS = {torch.int32: 0, torch.int64: 1}
+_INT64 = {torch.int64: 0}
+_FLOAT = {torch.float32: 0}
 
 
 def _rows(t):
-    """A 2-D tensor whose rows can be addressed (unit stride inside a row, rows that do not overlap): itself or a copy."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
-        return t
-    return t.contiguous()
+    """(t, distance of its rows in elements) for a 2-D tensor, a copy if its rows cannot be addressed (unit stride inside a row,
+    rows that do not overlap)."""
+    n, c = t.shape
+    ld, inner = t.stride()
+    if n <= 1:
+        ld = c
+    if (inner != 1 and c != 1) or ld < c:
+        t, ld = t.contiguous(), c
+    return t, ld
 
 
-def _ld(t):
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _flat(t):
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
 def _bytes(name, *args):
     n = ctypes.c_longlong()
     _lib.call(name, *args, ctypes.byref(n))
@@ -79,13 +93,13 @@ def _size(v, what, most=0x7ffffffe):
 # ---- embedding lookup -----------------------------------------------------------------------------------------------------
 def _lookup(table, tokens, scale, out_dtype):
     R, (V, D) = tokens.numel(), table.shape
-    tok, tab = tokens.reshape(-1).contiguous(), _rows(table)
+    tok, (tab, ld) = _flat(tokens), _rows(table)
     out = torch.empty((R, D), dtype=out_dtype, device=table.device)
     if R:
         with _On(table) as st:
-            _lib.call("svae_lookup_fwd", tab.data_ptr(), _TYPES[tab.dtype], _ld(tab), tok.data_ptr(), _IDS[tok.dtype], out.data_ptr(),
+            _lib.call("svae_lookup_fwd", tab.data_ptr(), _TYPES[tab.dtype], ld, tok.data_ptr(), _IDS[tok.dtype], out.data_ptr(),
                       _TYPES[out_dtype], D, R, V, D, scale, st)
-    return out.view(tokens.shape + (D,))
+    return out if tokens.dim() == 1 else out.view(tokens.shape + (D,))
 
 
 class _Embedding(torch.autograd.Function):
@@ -108,7 +122,7 @@ def embedding(table, tokens, scale=1.0, padding_idx=None, out_dtype=None):
     table [V, D] (rows may be strided), tokens int32 / int64 of any shape.  A token outside [0, V) gives a zero row and no
     gradient; ``padding_idx`` is looked up like any other and gets no gradient.  The gradient is dense, in the table's type."""
     _check(table, "table")
-    _check(tokens, "tokens", _IDS, table.device)
+    _check(tokens, "tokens", _IDS, table.get_device())
     out_dtype = table.dtype if out_dtype is None else out_dtype
     if out_dtype not in _TYPES:
         raise TypeError("out_dtype %s is not supported" % (out_dtype,))
@@ -128,7 +142,7 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=No
     Tokens are sorted on the device (stable, so equal tokens are added in their order).  ``out``: the tensor to write (rows may
     be strided); with ``accumulate`` the sums are added to what ``out`` holds, as for a table that another gradient shares."""
     _check(dout, "dout")
-    _check(tokens, "tokens", _IDS, dout.device)
+    _check(tokens, "tokens", _IDS, dout.get_device())
     if dout.dim() < 1 or dout.shape[:-1] != tokens.shape:
         raise ValueError("dout %s does not have one row for each token of %s" % (tuple(dout.shape), tuple(tokens.shape)))
     R, D, V = tokens.numel(), dout.shape[-1], int(num_rows)
@@ -143,35 +157,37 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=No
             raise TypeError("dtype %s is not supported" % (dtype,))
         out = torch.empty((V, D), dtype=dtype, device=dout.device)
     else:
-        _check(out, "out", device=dout.device)
+        _check(out, "out", device=dout.get_device())
         if tuple(out.shape) != (V, D) or (D > 1 and out.stride(1) != 1) or (V > 1 and out.stride(0) < D) or dtype not in (None, out.dtype):
             raise ValueError("out must be [%d, %d] with rows that can be addressed%s" % (V, D, "" if dtype is None else " and type %s" % dtype))
-    tok, dy = tokens.reshape(-1).contiguous(), _rows(dout.reshape(R, D))
     pad = -1 if padding_idx is None else int(padding_idx)
     if padding_idx is not None and not 0 <= pad < V:
         raise ValueError("padding_idx %d is outside the table of %d rows" % (pad, V))
+    tok, (dy, ld) = _flat(tokens), _rows(dout if dout.dim() == 2 else dout.reshape(R, D))
     n_sort, n_sum = _bytes("svae_token_sort_bytes", R, V), _bytes("svae_lookup_bwd_bytes", R, D)
-    work = torch.empty(max(1, (2 * R + 127) // 128 * 128 * 4 + max(n_sort, n_sum)), dtype=torch.uint8, device=dout.device)
-    keys, perm, rest = work.data_ptr(), work.data_ptr() + 4 * R, work.data_ptr() + (2 * R + 127) // 128 * 128 * 4
+    keep = (2 * R + 127) // 128 * 512                     # keys and places, then what either call needs
+    work = torch.empty(keep + max(n_sort, n_sum, 1), dtype=torch.uint8, device=dout.device)
+    keys = work.data_ptr()
+    perm, rest = keys + 4 * R, keys + keep
     with _On(dout) as st:
         _lib.call("svae_token_sort", tok.data_ptr(), _IDS[tok.dtype], R, V, pad, keys, perm, rest, n_sort, st)
-        _lib.call("svae_lookup_bwd", dy.data_ptr(), _TYPES[dy.dtype], _ld(dy), keys, perm, R, V, D, scale, out.data_ptr(), _TYPES[out.dtype],
-                  _ld(out), int(accumulate), rest, n_sum, st)
+        _lib.call("svae_lookup_bwd", dy.data_ptr(), _TYPES[dy.dtype], ld, keys, perm, R, V, D, scale, out.data_ptr(), _TYPES[out.dtype],
+                  out.stride(0) if V > 1 else D, int(accumulate), rest, n_sum, st)
     return out
 
 
 # ---- dropout --------------------------------------------------------------------------------------------------------------
 def _dropout(x, p, seed, step, row_key, out=None):
     C = x.shape[-1]
-    x2 = _rows(x.reshape(-1, C))
+    x2, ld = _rows(x if x.dim() == 2 else x.reshape(-1, C))
     R = x2.shape[0]
-    y = torch.empty((R, C), dtype=x.dtype, device=x.device) if out is None else out.view(R, C)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
     if R:
         dev = isinstance(step, torch.Tensor)
         with _On(x) as st:
-            _lib.call("svae_dropout", x2.data_ptr(), _ld(x2), y.data_ptr(), _ld(y), _TYPES[x.dtype], R, C, p, seed & 0xFFFFFFFFFFFFFFFF,
+            _lib.call("svae_dropout", x2.data_ptr(), ld, y.data_ptr(), C, _TYPES[x.dtype], R, C, p, seed & 0xFFFFFFFFFFFFFFFF,
                       0 if dev else step & 0xFFFFFFFF, step.data_ptr() if dev else None, None if row_key is None else row_key.data_ptr(), st)
-    return y.view(x.shape) if out is None else out
+    return y
 
 
 class _Dropout(torch.autograd.Function):
@@ -207,20 +223,20 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
     if k < 0 or (k == 0) != (p == 0.0) or (k == 65536) != (p == 1.0):
         raise ValueError("p = %r must be 0, 1 or a probability that is at least 2^-17 from both" % (p,))
     if isinstance(step, torch.Tensor):
-        _check(step, "step", {torch.int64: 0}, x.device)
+        _check(step, "step", _INT64, x.get_device())
         if step.numel() != 1:
             raise ValueError("step must have one element")
     if row_key is not None:
-        _check(row_key, "row_key", {torch.int64: 0}, x.device)
+        _check(row_key, "row_key", _INT64, x.get_device())
         if row_key.numel() != rows:
             raise ValueError("row_key has %d elements, x has %d rows" % (row_key.numel(), rows))
-        row_key = row_key.reshape(-1).contiguous()
+        row_key = _flat(row_key)
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:
             raise ValueError("out is for calls outside autograd")
         return _Dropout.apply(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key)
     if out is not None:
-        _check(out, "out", {x.dtype: 0}, x.device)
+        _check(out, "out", {x.dtype: 0}, x.get_device())
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and shaped like x")
     return _dropout(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key, out)
@@ -230,8 +246,8 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
 def _xent_args(hidden, weight, targets, bias):
     """Checks; returns (hidden rows, weight rows, bias, flat targets, R, V, D)."""
     _check(hidden, "hidden")
-    _check(weight, "weight", {hidden.dtype: 0}, hidden.device)
-    _check(targets, "targets", _IDS, hidden.device)
+    _check(weight, "weight", {hidden.dtype: 0}, hidden.get_device())
+    _check(targets, "targets", _IDS, hidden.get_device())
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError("hidden %s and weight %s do not fit: [..., D] and [V, D]" % (tuple(hidden.shape), tuple(weight.shape)))
     if targets.shape != hidden.shape[:-1]:
@@ -242,38 +258,44 @@ def _xent_args(hidden, weight, targets, bias):
     _size(D, "width", 1 << 16)
     _size(R + 1, "rows + 1", (1 << 24) + 1)
     if bias is not None:
-        _check(bias, "bias", {hidden.dtype: 0}, hidden.device)
+        _check(bias, "bias", {hidden.dtype: 0}, hidden.get_device())
         if tuple(bias.shape) != (V,):
             raise ValueError("bias %s must be [%d]" % (tuple(bias.shape), V))
-        bias = bias.contiguous()
-    h, w = _rows(hidden.reshape(R, D)), _rows(weight)
-    return h, w if _ld(w) <= 1 << 20 else w.contiguous(), bias, targets.reshape(-1).contiguous(), R, V, D
-
-
-def _xent_work(w, h, R, V, D, grad):
-    n = _bytes("svae_xent_bytes", w.data_ptr(), _ld(w), _TYPES[h.dtype], R, V, D, int(grad))
-    return torch.empty(n, dtype=torch.uint8, device=h.device)
+        bias = _flat(bias)
+    h, w = _rows(hidden if hidden.dim() == 2 else hidden.reshape(R, D)), _rows(weight)
+    if w[1] > 1 << 20:
+        w = (weight.contiguous(), D)
+    return h, w, bias, _flat(targets), R, V, D
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _xent_fwd(h, w, bias, tok, R, V, D, work, st):
-    nll, lse = torch.empty(2, R, dtype=torch.float32, device=h.device)
-    _lib.call("svae_xent_fwd", h.data_ptr(), _ld(h), w.data_ptr(), _ld(w), _ptr(bias), tok.data_ptr(), _IDS[tok.dtype], _TYPES[h.dtype],
-              R, V, D, nll.data_ptr(), lse.data_ptr(), work.data_ptr(), work.numel(), st)
+def _xent(name, args, grad, middle, out):
+    """One of svae_xent_fwd / _bwd / _fwd_bwd with its workspace; middle: pointers behind D, out: those behind."""
+    (h, ldh), (w, ldw), bias, tok, R, V, D = args
+    n = _bytes("svae_xent_bytes", w.data_ptr() % 16, ldw, _TYPES[h.dtype], R, V, D, int(grad))
+    work = torch.empty(n, dtype=torch.uint8, device=h.device)
+    with _On(h) as st:
+        _lib.call(name, h.data_ptr(), ldh, w.data_ptr(), ldw, _ptr(bias), tok.data_ptr(), _IDS[tok.dtype], _TYPES[h.dtype], R, V, D,
+                  *middle, *out, work.data_ptr(), n, st)
+
+
+def _xent_fwd(args):
+    h, R = args[0][0], args[4]
+    nll, lse = torch.empty(R, dtype=torch.float32, device=h.device), torch.empty(R, dtype=torch.float32, device=h.device)
+    _xent("svae_xent_fwd", args, False, (nll.data_ptr(), lse.data_ptr()), ())
     return nll, lse
 
 
-def _xent_bwd(h, w, bias, tok, R, V, D, lse, row_weight, need, work, st):
+def _xent_grads(args, need):
+    h, R, V, D = args[0][0], *args[4:]
     new = dict(dtype=h.dtype, device=h.device)
     dh = torch.empty((R, D), **new) if need[0] else None
     dw = torch.empty((V, D), **new) if need[1] or need[2] else None
     db = torch.empty(V, **new) if need[2] else None
-    _lib.call("svae_xent_bwd", h.data_ptr(), _ld(h), w.data_ptr(), _ld(w), _ptr(bias), tok.data_ptr(), _IDS[tok.dtype], _TYPES[h.dtype],
-              R, V, D, lse.data_ptr(), row_weight.data_ptr(), _ptr(dh), D, _ptr(dw), D, _ptr(db), work.data_ptr(), work.numel(), st)
-    return dh, dw if need[1] else None, db
+    return (dh, dw, db), (_ptr(dh), D, _ptr(dw), D, _ptr(db))
 
 
 def linear_nll(hidden, weight, targets, bias=None):
@@ -281,44 +303,46 @@ def linear_nll(hidden, weight, targets, bias=None):
 
     hidden [..., D], weight [V, D], bias [V] of one type; targets int32 / int64.  A row whose target is outside [0, V) is left
     out: both are 0.  For scoring, and for programs that run their own backward pass (``linear_nll_grad``)."""
-    h, w, bias, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
-    if R == 0:
-        nll = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
+    args = _xent_args(hidden, weight, targets, bias)
+    if args[4] == 0:
+        nll = torch.empty(targets.shape, dtype=torch.float32, device=hidden.device)
         return nll, nll.clone()
-    with _On(h) as st:
-        nll, lse = _xent_fwd(h, w, bias, tok, R, V, D, _xent_work(w, h, R, V, D, False), st)
-    return nll.view(targets.shape), lse.view(targets.shape)
+    nll, lse = _xent_fwd(args)
+    return (nll, lse) if targets.dim() == 1 else (nll.view(targets.shape), lse.view(targets.shape))
 
 
 def linear_nll_grad(hidden, weight, targets, row_weight, bias=None):
     """(nll, lse, dhidden, dweight, dbias): ``linear_nll`` and the gradients of ``sum(row_weight * nll)`` in the inputs' type
     (dbias None without a bias).  row_weight: fp32, shaped like targets; a row of weight 0 takes no part in the gradient."""
-    h, w, bias, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
-    _check(row_weight, "row_weight", {torch.float32: 0}, h.device)
+    args = _xent_args(hidden, weight, targets, bias)
+    _check(row_weight, "row_weight", _FLOAT, hidden.get_device())
     if row_weight.shape != targets.shape:
         raise ValueError("row_weight %s must be shaped like targets %s" % (tuple(row_weight.shape), tuple(targets.shape)))
+    (h, _), R = args[0], args[4]
+    nll, lse = torch.empty(R, dtype=torch.float32, device=h.device), torch.empty(R, dtype=torch.float32, device=h.device)
     if R == 0:
-        nll = torch.empty(targets.shape, dtype=torch.float32, device=h.device)
-        return nll, nll.clone(), torch.empty_like(hidden), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias)
-    with _On(h) as st:
-        work = _xent_work(w, h, R, V, D, True)
-        nll, lse = _xent_fwd(h, w, bias, tok, R, V, D, work, st)
-        dh, dw, db = _xent_bwd(h, w, bias, tok, R, V, D, lse, row_weight.reshape(-1).contiguous(), (True, True, bias is not None), work, st)
+        return nll.view(targets.shape), lse.view(targets.shape), torch.empty_like(hidden), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias)
+    (dh, dw, db), out = _xent_grads(args, (True, True, bias is not None))
+    wr = _flat(row_weight)
+    _xent("svae_xent_fwd_bwd", args, True, (wr.data_ptr(), nll.data_ptr(), lse.data_ptr()), out)
+    if targets.dim() == 1:
+        return nll, lse, dh, dw, db
     return nll.view(targets.shape), lse.view(targets.shape), dh.view(hidden.shape), dw, db
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, reduction):
-        h, w, b, tok, R, V, D = _xent_args(hidden, weight, targets, bias)
-        ctx.shapes, ctx.reduction = (hidden.shape, R, V, D), reduction
+        args = _xent_args(hidden, weight, targets, bias)
+        (h, ldh), (w, ldw), b, tok, R, V, D = args
+        ctx.shapes, ctx.reduction = (hidden.shape, ldh, ldw, R, V, D), reduction
         out = torch.zeros(2, dtype=torch.float32, device=h.device)
         if R == 0:
             ctx.save_for_backward(h, w, b, tok, out, out)
             return out.new_empty(targets.shape) if reduction == "none" else out[0].clone()
-        with _On(h) as st:
-            nll, lse = _xent_fwd(h, w, b, tok, R, V, D, _xent_work(w, h, R, V, D, False), st)
-            if reduction != "none":
+        nll, lse = _xent_fwd(args)
+        if reduction != "none":
+            with _On(h) as st:
                 _lib.call("svae_xent_reduce", nll.data_ptr(), tok.data_ptr(), _IDS[tok.dtype], R, V, int(reduction == "mean"), out.data_ptr(), st)
         ctx.save_for_backward(h, w, b, tok, lse, out)
         return nll.view(targets.shape) if reduction == "none" else out[0].clone()
@@ -327,14 +351,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         h, w, b, tok, lse, out = ctx.saved_tensors
-        shape, R, V, D = ctx.shapes
+        shape, ldh, ldw, R, V, D = ctx.shapes
         if R == 0:
             return h.new_empty(shape), torch.zeros_like(w), None if b is None else torch.zeros_like(b), None, None
         weight = dloss.reshape(-1).float().contiguous() if ctx.reduction == "none" else (dloss.float() * out[1]).expand(R).contiguous()
-        with _On(h) as st:
-            need = ctx.needs_input_grad[:3]
-            dh, dw, db = _xent_bwd(h, w, b, tok, R, V, D, lse, weight, need, _xent_work(w, h, R, V, D, True), st)
-        return None if dh is None else dh.view(shape), dw, db, None, None
+        args = ((h, ldh), (w, ldw), b, tok, R, V, D)
+        need = ctx.needs_input_grad[:3]
+        (dh, dw, db), outs = _xent_grads(args, need)
+        _xent("svae_xent_bwd", args, True, (lse.data_ptr(), weight.data_ptr()), outs)
+        return None if dh is None else dh.view(shape), dw if need[1] else None, db, None, None
 
 
 def linear_cross_entropy(hidden, weight, targets, bias=None, reduction="mean"):

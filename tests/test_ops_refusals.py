@@ -36,7 +36,8 @@ def test_lookup_entry_points_refuse():
     refused("types", "svae_lookup_fwd", P, 3, 4, P, 0, P, 0, 4, 2, 10, 4, 1.0, None)
     refused("null", "svae_lookup_fwd", None, 0, 4, P, 0, P, 0, 4, 2, 10, 4, 1.0, None)
     refused("sizes", "svae_token_sort", P, 0, 5, 0, -1, P, P, P, 1 << 20, None)
-    refused("workspace", "svae_token_sort", P, 0, 5, 10, -1, P, P, P, 8, None)
+    refused("workspace", "svae_token_sort", P, 0, 5000, 10, -1, P, P, P, 8, None)
+    refused("null", "svae_token_sort", P, 0, 5000, 10, -1, P, P, None, 1 << 20, None)
     refused("null", "svae_token_sort", P, 0, 5, 10, -1, P, None, P, 1 << 20, None)
     refused("workspace", "svae_lookup_bwd", P, 0, 4, P, P, 5, 10, 4, 1.0, P, 0, 4, 0, P, 8, None)
     refused("sizes", "svae_lookup_bwd", P, 0, 4, P, P, 5, 10, 0, 1.0, P, 0, 4, 0, P, 1 << 20, None)
@@ -47,8 +48,10 @@ def test_workspace_sizes():
     n = ctypes.c_longlong()
     _lib.call("svae_token_sort_bytes", 0, 1, ctypes.byref(n))
     assert n.value == 0
-    _lib.call("svae_token_sort_bytes", 5000, 3000000, ctypes.byref(n))          # two workgroups, two digits of 11 bits
-    assert n.value == 2 * 2048 * 4 + 2 * 20224
+    _lib.call("svae_token_sort_bytes", 4096, 3000000, ctypes.byref(n))          # in one workgroup's LDS
+    assert n.value == 0
+    _lib.call("svae_token_sort_bytes", 5000, 3000000, ctypes.byref(n))          # five workgroups, two digits of 11 bits
+    assert n.value == 5 * 2048 * 4 + 2 * 20224
     _lib.call("svae_lookup_bwd_bytes", 65, 10, ctypes.byref(n))
     assert n.value == 256                                                       # two chunks, two slots, 10 floats
 
@@ -65,10 +68,10 @@ def test_dropout_entry_point_refuses():
 
 def test_xent_entry_points_refuse():
     n = ctypes.c_longlong()
-    for bad in ((P, 8, 7, 4, 10, 8, 0), (P, 7, 1, 4, 10, 8, 0), (P, 8, 1, 0, 10, 8, 0), (P, 8, 1, 4, 0, 8, 1), (P, 8, 1, 4, 10, 0, 1),
-                (P, 1 << 21, 1, 4, 10, 8, 0), (P, 1 << 17, 1, 4, 10, (1 << 16) + 1, 0)):
+    for bad in ((0, 8, 7, 4, 10, 8, 0), (0, 7, 1, 4, 10, 8, 0), (0, 8, 1, 0, 10, 8, 0), (0, 8, 1, 4, 0, 8, 1), (0, 8, 1, 4, 10, 0, 1),
+                (0, 1 << 21, 1, 4, 10, 8, 0), (0, 1 << 17, 1, 4, 10, (1 << 16) + 1, 0)):
         refused("svae_xent: (type|sizes)", "svae_xent_bytes", *bad, ctypes.byref(n))
-    refused("null", "svae_xent_bytes", P, 8, 1, 4, 10, 8, 0, None)
+    refused("null", "svae_xent_bytes", 0, 8, 1, 4, 10, 8, 0, None)
     refused("null", "svae_xent_fwd", None, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 1 << 30, None)
     refused("ld", "svae_xent_fwd", P, 7, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 1 << 30, None)
     refused("workspace", "svae_xent_fwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 100, None)
@@ -77,6 +80,8 @@ def test_xent_entry_points_refuse():
     refused("null", "svae_xent_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, None, P, P, 8, P, 8, None, P, 1 << 30, None)
     refused("ld", "svae_xent_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, 7, P, 8, None, P, 1 << 30, None)
     refused("bias gradient", "svae_xent_bwd", P, 8, P, 8, P, P, 0, 1, 4, 10, 8, P, P, P, 8, None, 8, P, P, 1 << 30, None)
+    refused("null", "svae_xent_fwd_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, None, P, P, P, 8, P, 8, None, P, 1 << 30, None)
+    refused("workspace", "svae_xent_fwd_bwd", P, 8, P, 8, None, P, 0, 1, 4, 10, 8, P, P, P, P, 8, P, 8, None, P, 1 << 10, None)
     refused("bad arguments", "svae_xent_reduce", P, P, 0, 0, 10, 1, P, None)
 
 
