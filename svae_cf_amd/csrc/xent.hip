@@ -141,7 +141,11 @@ __device__ __forceinline__ void core(const Operand& A, const Operand& B, int ste
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned oa[L::NA], ob[L::NB];
 #pragma unroll
-    for (int j = 0; j < L::NA; ++j) oa[j] = dma_offset<AKIND, BM>((unsigned)(wave * L::NA + j), lane, A.ld);
+    for (int j = 0; j < L::NA; ++j) {
+        const unsigned inst = (unsigned)(wave * L::NA + j);
+        oa[j] = dma_offset<AKIND, BM>(inst, lane, A.ld);
+        if (AKIND == ACROSS && inst % (BM / 32) * 32u >= 16u * L::WM * MT) oa[j] = NOWHERE;          // columns of no tile
+    }
 #pragma unroll
     for (int j = 0; j < L::NB; ++j) ob[j] = dma_offset<BKIND, BN>((unsigned)(wave * L::NB + j), lane, B.ld);
     const Frag fa = frag_offset<AKIND, BM>(wave / L::WN, lane), fb = frag_offset<BKIND, BN>((wave % L::WN) * 4, lane);
@@ -315,18 +319,20 @@ __device__ __forceinline__ void logit_tile(const LogitArgs& a, int tile, char* c
 
     // where a lane has the logit of a row's target: most tiles have none of a wave's 16 rows' targets
     auto mine = [&](int n) { return a.tgt[r0 + wn + 16 * n + i16] - ((int)v0 + w0 + 4 * q); };
-    auto some = [&](int rel) { return __any(rel >= 0 && rel < EVERY * L::MT && rel % EVERY < 4); };
+    auto has = [&](int rel) { return rel >= 0 && rel < EVERY * L::MT && rel % EVERY < 4; };
+    auto some = [&](int rel) { return __any(has(rel)); };
     if (!GRAD) {
         float top[4], sum[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int rel = mine(n);
             if (some(rel)) {
+                float z = 0.f;
 #pragma unroll
                 for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (rel == EVERY * t + i) a.zt[r0 + wn + 16 * n + i16] = acc[t][n][i];
+                    for (int i = 0; i < 4; ++i) z = rel == EVERY * t + i ? acc[t][n][i] : z;
+                if (has(rel)) a.zt[r0 + wn + 16 * n + i16] = z;
             }
             float m = -INFINITY;
 #pragma unroll
@@ -379,8 +385,7 @@ __device__ __forceinline__ void logit_tile(const LogitArgs& a, int tile, char* c
 #pragma unroll
                 for (int t = 0; t < L::MT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (rel == EVERY * t + i) acc[t][n][i] -= 1.f;
+                    for (int i = 0; i < 4; ++i) acc[t][n][i] -= rel == EVERY * t + i ? 1.f : 0.f;
             }
             if (__any(w == 0.f)) {                       // no part in the gradient, whatever W makes of such a row's zeros
 #pragma unroll
@@ -653,13 +658,14 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
     }
 }
 
-// lse and loss from the tiles' statistics: a workgroup takes 256 / SLICES rows, SLICES threads share the tiles of one
-template <int SLICES>
+// lse and loss from the tiles' statistics.  FEW: a workgroup for a row, its threads share the tiles; else 32 rows a workgroup,
+// eight threads for each.
+template <bool FEW>
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
                                                         const int* __restrict__ tgt, int R, int Rp, int nvt,
                                                         float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ lsec) {
-    constexpr int ROWS = 256 / SLICES;
-    __shared__ float2 red[SLICES][ROWS + 1];
+    constexpr int SLICES = FEW ? 256 : 8, ROWS = 256 / SLICES;
+    __shared__ float2 red[8][33];
     const int i = threadIdx.x % ROWS, s = threadIdx.x / ROWS;
     const long long r = (long long)blockIdx.x * ROWS + i;
     float m = -INFINITY, sum = 0.f;
@@ -671,10 +677,21 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
 #pragma unroll
         for (int k = 0; k < 4; ++k) join_sums(m, sum, p[k].x, p[k].y);
     }
-    red[s][i] = make_float2(m, sum);
+    if (FEW) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(sum, o, 64);
+            join_sums(m, sum, m2, s2);
+        }
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = make_float2(m, sum);
+    } else red[s][i] = make_float2(m, sum);
     __syncthreads();
     if ((int)threadIdx.x >= ROWS) return;
-    for (int k = 1; k < SLICES; ++k) join_sums(m, sum, red[k][i].x, red[k][i].y);
+    if (FEW) {
+        m = red[0][0].x;
+        sum = red[0][0].y;
+    }
+    for (int k = 1; k < (FEW ? 4 : 8); ++k) join_sums(m, sum, red[k][i].x, red[k][i].y);
     const bool here = tgt[r] >= 0;
     const float l = m + logf(sum);
     if (lsec != nullptr) lsec[r] = here ? l : 0.f;
@@ -888,11 +905,10 @@ inline int loss(const Call& c, const Shape& s, float* nll, float* lse, float* ls
         else go(xent_loss_kernel<E, 128, ALONG, P>);
     });
     SV_LAUNCH_CHECK();
-    // few rows and many tiles: more threads a row
-    if ((long long)s.Rp * 8 < s.nvt * 64ll)
-        hipLaunchKernelGGL(xent_rows_kernel<64>, dim3(s.Rp / 4), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
+    if (c.R <= 1024 && s.nvt > 64)
+        hipLaunchKernelGGL(xent_rows_kernel<true>, dim3(lsec ? s.Rp : c.R), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
     else
-        hipLaunchKernelGGL(xent_rows_kernel<8>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
+        hipLaunchKernelGGL(xent_rows_kernel<false>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
     SV_LAUNCH_CHECK();
     return 0;
 }
