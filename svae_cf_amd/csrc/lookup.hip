@@ -271,25 +271,27 @@ __device__ __forceinline__ int segment_end(const int* __restrict__ keys, int i, 
     return lower_bound(keys, i, R, (long long)k + 1, lane);
 }
 
-// acc += sum of dy[place(i)][c .. c + VEC) over i = b, b + step, .. < e, eight rows in flight
+// acc += sum of dy[place(i)][c .. c + VEC) over i = b, b + step, .. < e, sixteen rows in flight (as they lie, 4 registers each)
+template <int U, int VEC, typename T, typename P>
+__device__ __forceinline__ void add_rows(const T* __restrict__ dy, long long ldd, P place, int b, int e, int step, int c, float* acc) {
+    typename SvVec<T, VEC>::type v[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+        if (b + j * step < e) v[j] = *reinterpret_cast<const typename SvVec<T, VEC>::type*>(dy + (long long)place(b + j * step) * ldd + c);
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+        if (b + j * step < e) {
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) acc[q] += (float)v[j][q];
+        }
+}
 template <int VEC, typename T, typename P>
 __device__ __forceinline__ void sum_rows(const T* __restrict__ dy, long long ldd, P place, int b, int e, int step, int c, float* acc) {
-    for (int i = b; i < e; i += 8 * step) {
-        float v[8][VEC];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool in = i + j * step < e;
-            if (in) sv_load<VEC>(dy + (long long)place(i + j * step) * ldd + c, v[j]);
-            else {
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) v[j][q] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) acc[q] += v[j][q];
+    if (e - b <= 4 * step) {                                 // most rows of a table have few
+        add_rows<4, VEC>(dy, ldd, place, b, e, step, c, acc);
+        return;
     }
+    for (int i = b; i < e; i += 16 * step) add_rows<16, VEC>(dy, ldd, place, i, e, step, c, acc);
 }
 
 template <int VEC, typename G>
@@ -313,6 +315,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
     __shared__ float red[4][64 * VEC];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = ((int)blockIdx.y * 64 + lane) * VEC;       // the launch's second dimension goes over slices of the columns
     if ((int)blockIdx.x < nchunk) {
         const int p0 = (int)blockIdx.x * CHUNK, p1 = R - p0 < CHUNK ? R : p0 + CHUNK;
         // the chunk's keys and those of 64 places on either side: enough to tell which runs are long
@@ -328,23 +331,20 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
             const int b = slot == 0 ? p0 : p0 + __builtin_ctzll(ml), z = slot == 0 ? p0 + __popcll(mf) : p1;
             const int length = z - b + (slot == 0 ? run(__ballot(kb == kf)) : 0) + (z == p1 ? run(__ballot(ka == kl)) : 0);
             if (length <= LONG) continue;
-            for (int c0 = 0; c0 < D; c0 += 64 * VEC) {
-                const int c = c0 + lane * VEC;
-                float acc[VEC];
+            float acc[VEC];
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-                if (c < D) sum_rows<VEC>(dy, ldd, [&](int i) { return perm[i]; }, b + wave, z, 4, c, acc);
+            for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+            if (c < D) sum_rows<VEC>(dy, ldd, [&](int i) { return perm[i]; }, b + wave, z, 4, c, acc);
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
-                __syncthreads();
-                if (wave == 0 && c < D) {
+            for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
+            __syncthreads();
+            if (wave == 0 && c < D) {
 #pragma unroll
-                    for (int q = 0; q < VEC; ++q)
-                        acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
-                    sv_store<VEC>(part + ((size_t)blockIdx.x * 2 + slot) * D + c, acc);
-                }
-                __syncthreads();
+                for (int q = 0; q < VEC; ++q)
+                    acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
+                sv_store<VEC>(part + ((size_t)blockIdx.x * 2 + slot) * D + c, acc);
             }
+            __syncthreads();
         }
         return;
     }
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
         if (far) e = segment_end(keys, s > e ? s : e, R, (int)(v0 + g), lane);
         G* dst = grad + (v0 + g) * ldg;
         if (e - s <= LONG && !(accumulate && e == s)) {
-            for (int c = lane * VEC; c < D; c += 64 * VEC) {
+            if (c < D) {
                 float acc[VEC];
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
@@ -396,39 +396,23 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
     const int e = segment_end(keys, p0 + CHUNK, R, k, lane);
     const int last = (e - 1) / CHUNK;
     const int slot0 = s == p0 ? 0 : 1;                       // in chunk p; the following ones have it at their first place
-    for (int c0 = 0; c0 < D; c0 += 64 * VEC) {
-        const int c = c0 + lane * VEC;
-        float acc[VEC];
+    const int c = ((int)blockIdx.y * 64 + lane) * VEC;
+    float acc[VEC];
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-        if (c < D) {
-            for (int j = (int)blockIdx.x + wave; j <= last; j += 32) {       // eight partial sums in flight
-                float v[8][VEC];
+    for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+    if (c < D) {
+        // partial sums are rows of D floats, two for a chunk; only the first chunk's may be in the second one
+        auto at = [&](int j) { return 2 * j + (j == (int)blockIdx.x ? slot0 : 0); };
+        sum_rows<VEC>(part, D, at, (int)blockIdx.x + wave, last + 1, 4, c, acc);
+    }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int jj = j + 4 * u;
-                    if (jj <= last) sv_load<VEC>(part + ((size_t)jj * 2 + (jj == (int)blockIdx.x ? slot0 : 0)) * D + c, v[u]);
-                    else {
+    for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
+    __syncthreads();
+    if (wave == 0 && c < D) {
 #pragma unroll
-                        for (int q = 0; q < VEC; ++q) v[u][q] = 0.f;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) acc[q] += v[u][q];
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
-        __syncthreads();
-        if (wave == 0 && c < D) {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q)
-                acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
-            put_row<VEC>(grad + (long long)k * ldg + c, acc, scale, accumulate);
-        }
-        __syncthreads();
+        for (int q = 0; q < VEC; ++q)
+            acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
+        put_row<VEC>(grad + (long long)k * ldg + c, acc, scale, accumulate);
     }
 }
 
@@ -533,21 +517,24 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
     SV_CHECK_ARG(work_bytes >= need, "svae_lookup_bwd: workspace of %lld bytes, %lld needed", work_bytes, need);
     if (R == 0 && accumulate) return 0;
     const int nchunk = (int)chunks_of(R);
-    // rows of a wave: many where most rows are empty (they are only written), few where most have tokens to wait for
-    const int group = (long long)V >= 8ll * R ? MOST_GROUP : 4;
+    // rows of a wave: as many as leave 8192 waves (131072 rows of 1024, as many tokens: 16 rows 170 us, 4 rows 179 us; 20000
+    // rows of 256, 21800 tokens: 16 rows 16.6 us, 4 rows 12.7 us)
+    const int group = V >= 8192 * MOST_GROUP ? MOST_GROUP : V >= 8192 * 8 ? 8 : 4;
     const long long nrow = ((long long)V + 4 * group - 1) / (4 * group);
     SV_CHECK_ARG(nchunk + nrow < 0x7fffffffll, "svae_lookup_bwd: R %d and V %d need too many workgroups", R, V);
     int vec = sv_vec_for(8, D, R ? dy : grad, R ? ld_dy : ld_grad, sv_elem_size(dy_type), grad, ld_grad, sv_elem_size(grad_type));
     while (vec > 2 && 32 * vec >= D) vec >>= 1;              // rather all 64 lanes with shorter vectors
+    const unsigned slices = (unsigned)((D + 64 * vec - 1) / (64 * vec));
+    SV_CHECK_ARG(slices <= 65535u, "svae_lookup_bwd: D %d is too wide for rows that start at odd places", D);
     sv_by_type(dy_type, [&](auto t) {
         sv_by_type(grad_type, [&](auto o) {
             typedef decltype(t) T;
             typedef decltype(o) G;
             auto go = [&](auto kernel, auto join) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)(nchunk + nrow)), dim3(256), 0, (hipStream_t)stream, (const T*)dy, ld_dy, keys,
+                hipLaunchKernelGGL(kernel, dim3((unsigned)(nchunk + nrow), slices), dim3(256), 0, (hipStream_t)stream, (const T*)dy, ld_dy, keys,
                                    perm, R, V, D, scale, (G*)grad, ld_grad, accumulate, nchunk, group, (float*)work);
                 if (R > LONG)
-                    hipLaunchKernelGGL(join, dim3((unsigned)nchunk), dim3(256), 0, (hipStream_t)stream, keys, R, V, D, scale, (G*)grad,
+                    hipLaunchKernelGGL(join, dim3((unsigned)nchunk, slices), dim3(256), 0, (hipStream_t)stream, keys, R, V, D, scale, (G*)grad,
                                        ld_grad, accumulate, (const float*)work);
             };
             if (vec == 8) go(lookup_bwd_kernel<8, T, G>, lookup_bwd_long_kernel<8, G>);
