@@ -20,9 +20,8 @@
 // Few rows and no gradient: W is read once, as it lies (16-bit types, aligned rows); that is bound by HBM.
 //
 // Types: bf16 and fp16 go to the matrix units as they are; G is rounded to the inputs' type (relative 2^-8 / 2^-11 of each
-// term, as the inputs themselves are), for fp16 after scaling by a power of two that puts the largest row weight near 2^14, so
-// that small probabilities stay above fp16's subnormals.  fp32 is carried as three bf16 parts (24 bits) and every product by
-// its six leading terms.
+// term, as the inputs themselves are) after scaling by the largest row weight.  fp32 is carried as three bf16 parts (24 bits)
+// and every product by its six leading terms.  Few rows (xent_few.h) take other kernels.
 #include "elem.h"
 
 namespace {
@@ -262,7 +261,7 @@ struct LogitArgs {
     float* zt;                // loss: [Rp] the target's logit
     const float* lse;         // gradient: [Rp]
     const float* wrow;        // gradient: [Rp], 0 for rows without a part in it
-    const float* scale;       // gradient, fp16: the scale of G, or NULL
+    const float* scale;       // gradient: the scale of G
     char* g;                  // gradient: blocks of G, [Rp / 16][vocabulary tiles * 8], parts g_part bytes apart
     long long w_part, h_part, g_part;
     unsigned ldw;
@@ -369,7 +368,7 @@ __device__ __forceinline__ void logit_tile(const LogitArgs& a, int tile, char* c
             a.part[(long long)vt * a.Rp + r0 + threadIdx.x] = make_float2(m, s);
         }
     } else {
-        const float up = a.scale != nullptr ? a.scale[0] : 1.f;
+        const float up = a.scale[0];
         const long long nv32 = (long long)a.nvt * (BM / 32);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -440,7 +439,7 @@ struct ProductArgs {
     float* bslab;             // [splits][...] bias gradient, or NULL
     void* out;                // [rows][ld_out] of the caller's type
     void* bout;
-    const float* scale;       // fp16: scale[1] takes the scale of G out again (written only with the final result)
+    const float* scale;       // scale[1] takes the scale of G out again (with the final result)
     long long x_part, g_part, ld_out, slab_stride, bslab_stride;
     int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
 };
@@ -481,7 +480,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int tile, cha
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w0 = 16 * (wave / L::WN), wn = (wave % L::WN) * 64;
     const int i16 = lane & 15, q = lane >> 4;
-    const float down = a.scale != nullptr ? a.scale[1] : 1.f;
+    const float down = a.scale[1];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         const int r = nt * BN + wn + 16 * n + i16;
@@ -550,7 +549,7 @@ struct SumArgs {
 };
 template <typename T>
 __device__ __forceinline__ void sum_slabs(const SumArgs& a, unsigned block) {
-    const float down = a.scale != nullptr ? a.scale[1] : 1.f;
+    const float down = a.scale[1];
     const long long i = (long long)block * 256 + threadIdx.x;
     if (a.Dp == 1) {
         if (i >= a.rows) return;
@@ -658,12 +657,41 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
     }
 }
 
-// lse and loss from the tiles' statistics.  FEW: a workgroup for a row, its threads share the tiles; else 32 rows a workgroup,
-// eight threads for each.
+// What G is multiplied with: its largest weight becomes 2^14 (fp16) or 1, so that heavy rows, and all rows where weights are
+// equal, lose least to G's rounding (with equal weights a target of small probability loses nothing), and small entries stay
+// above the subnormals of fp16, or of bf16 in the third part of fp32.  scale[1] takes it out of the results.
+__device__ __forceinline__ void find_scale(const float* __restrict__ wrow, int Rp, float top, float* __restrict__ scale) {
+    __shared__ float red[4];
+    float m = 0.f;
+#pragma unroll 4
+    for (int r = threadIdx.x; r < Rp / 4; r += 256) {
+        const f32x4 w = reinterpret_cast<const f32x4*>(wrow)[r];
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3]))));
+    }
+    m = sv_wave_max(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    m = m < INFINITY ? fmaxf(m, 0x1p-100f) : top;
+    scale[0] = top / m;
+    scale[1] = m / top;
+}
+__global__ __launch_bounds__(256) void xent_scale_kernel(const float* __restrict__ wrow, int Rp, float top, float* __restrict__ scale) {
+    find_scale(wrow, Rp, top, scale);
+}
+
+// lse and loss from the tiles' statistics; one workgroup more for the scale, where it is wanted.  FEW: a workgroup for a row, its
+// threads share the tiles; else 32 rows a workgroup, eight threads for each.
 template <bool FEW>
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
                                                         const int* __restrict__ tgt, int R, int Rp, int nvt,
-                                                        float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ lsec) {
+                                                        float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ lsec,
+                                                        const float* __restrict__ wrow, float top, float* __restrict__ scale) {
+    if (scale != nullptr && blockIdx.x == gridDim.x - 1) {
+        find_scale(wrow, Rp, top, scale);
+        return;
+    }
     constexpr int SLICES = FEW ? 256 : 8, ROWS = 256 / SLICES;
     __shared__ float2 red[8][33];
     const int i = threadIdx.x % ROWS, s = threadIdx.x / ROWS;
@@ -729,34 +757,20 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
     }
 }
 
-// fp16: the power of two that brings the largest row weight to 2^13 .. 2^14, and its reciprocal
-__global__ __launch_bounds__(1024) void xent_scale_kernel(const float* __restrict__ wrow, int Rp, float* __restrict__ scale) {
-    __shared__ float red[16];
-    float m = 0.f;
-    for (int r = threadIdx.x; r < Rp; r += 1024) m = fmaxf(m, fabsf(wrow[r]));
-    m = sv_wave_max(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) m = fmaxf(m, red[k]);
-        int e = 0;
-        if (m > 0.f && m < INFINITY) frexpf(m, &e);          // m = f 2^e, f in [1/2, 1)
-        e = e > 100 ? 100 : e < -100 ? -100 : e;
-        scale[0] = ldexpf(1.f, 14 - e);
-        scale[1] = ldexpf(1.f, e - 14);
-    }
-}
+#include "xent_few.h"
 
 // ------------------------------------------------------------------------------------------------
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
+constexpr int FEW_ROWS_F32 = 64, FEW_ROWS_16 = 32;          // up to here: the kernels for few rows
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
 constexpr long long PIECE_LEAST = 128ll << 20, PIECE_MOST = 512ll << 20;     // what G of a piece may take; there are two
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
     int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, h_splits, w_splits, ndt, dblocks;
-    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab, b_slab, total;
+    int few, R4, wd, chunks;  // few: the kernels for few rows, with this many tiles of 16
+    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab, b_slab, z, total;
 };
 
 // parts of a product's contraction: no workgroup should work longer than a slot's share of the launch
@@ -771,6 +785,36 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     SV_CHECK_ARG(type >= 0 && type <= 2, "svae_xent: type %d", type);
     SV_CHECK_ARG(R > 0 && R <= 1 << 24 && V > 0 && V <= 1 << 28 && D > 0 && D <= 1 << 16 && ld_w >= D && ld_w <= 1 << 20,
                  "svae_xent: sizes R %lld, V %lld, D %lld, ld %lld", R, V, D, ld_w);
+    long long at = 0;
+    auto take = [&](long long bytes) {
+        const long long p = at;
+        at += (bytes + 1023) / 1024 * 1024;
+        return p;
+    };
+    if (R <= (type == SV_F32 ? FEW_ROWS_F32 : FEW_ROWS_16)) {
+        s->few = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+        s->Rp = 16 * s->few;
+        s->R4 = (int)(R + 3) / 4 * 4;
+        s->nvt = (int)((V + 255) / 256);
+        s->Dp = (int)((D + 63) / 64 * 64);
+        s->wd = D <= 64 ? 1 : D <= 128 ? 2 : 4;
+        s->ndt = (s->Dp / 64 + s->wd - 1) / s->wd;
+        const int steps = (int)((V + few_step(s->wd) - 1) / few_step(s->wd)), most = (s->few == 1 ? 768 : 512) / s->ndt;      // as many as run at a time: three or two on a CU
+        s->chunks = most < 1 ? 1 : most < steps ? most : steps;
+        s->h = take((long long)s->Rp * s->Dp * sv_elem_size(type));
+        s->tgt = take(4ll * s->Rp);
+        s->lse = take(4ll * s->Rp);
+        s->zt = take(4ll * s->Rp);
+        s->part = take(8ll * s->nvt * s->Rp);
+        if (grad != LOSS) {
+            s->hg = take((long long)s->Rp * s->Dp * sv_elem_size(type));
+            s->wrow = take(4ll * s->Rp);
+            s->z = take(4ll * V * s->R4);
+            s->h_slab = take(4ll * s->chunks * (4 / s->wd) * R * s->Dp);
+        }
+        s->total = at;
+        return 0;
+    }
     s->parts = type == SV_F32 ? 3 : 1;
     s->direct = grad == LOSS && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
     s->BN = R <= 64 ? 64 : 128;
@@ -784,12 +828,6 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->dblocks = (s->Dp / 32 + s->ndt - 1) / s->ndt;
     s->dblocks = s->BN == 64 ? 8 : s->dblocks <= 2 ? 2 : s->dblocks <= 4 ? 4 : s->dblocks;
     SV_CHECK_ARG((long long)s->nvt * s->nrt < 0x7ffffff0ll, "svae_xent: R %lld and V %lld need too many workgroups", R, V);
-    long long at = 0;
-    auto take = [&](long long bytes) {
-        const long long p = at;
-        at += (bytes + 1023) / 1024 * 1024;
-        return p;
-    };
     s->h_part = (long long)s->Rp * s->Dp * 2;
     s->h = take(s->h_part * s->parts);
     s->hg = grad == LOSS ? 0 : take(s->h_part * s->parts);
@@ -805,9 +843,9 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->part = s->g[0] = at;                                // the loss's statistics are done with when G is made
     const long long end = at + 8ll * s->nvt * s->Rp;
     if (grad != LOSS) {
-        // A piece's G is written and read twice: small pieces stay near the chip (21800 x 20000 x 200, bf16: G from HBM takes
-        // longer than its products).  Every piece adds to all of dH, so that a piece is at least 16 times dH's sums.
-        long long bytes = 64ll * s->Rp * s->Dp;
+        // A piece's G is written and read twice, and every piece adds to all of dH's sums (4 Rp Dp bytes, read and written): at
+        // least four times those, and 128 MiB for large launches (8192 x 131072 x 1024: 7.2 ms with pieces of 128 MiB, 7.4 with 512)
+        long long bytes = 16ll * s->Rp * s->Dp;
         bytes = bytes < PIECE_LEAST ? PIECE_LEAST : bytes > PIECE_MOST ? PIECE_MOST : bytes;
         long long tiles = bytes / (2ll * s->parts * s->Rp * BM);
         tiles = tiles < 1 ? 1 : tiles > s->nvt ? s->nvt : tiles;
@@ -884,7 +922,10 @@ inline LogitArgs logit_args(const Call& c, const Shape& s) {
     return a;
 }
 
-inline int loss(const Call& c, const Shape& s, float* nll, float* lse, float* lsec) {
+inline float top_of(int type) { return type == SV_F16 ? 16384.f : 1.f; }
+
+// grad: gradients follow, which read lse and the scale from the workspace
+inline int loss(const Call& c, const Shape& s, float* nll, float* lse, bool grad) {
     LogitArgs a = logit_args(c, s);
     a.part = (float2*)(c.work + s.part);
     a.zt = (float*)(c.work + s.zt);
@@ -905,10 +946,11 @@ inline int loss(const Call& c, const Shape& s, float* nll, float* lse, float* ls
         else go(xent_loss_kernel<E, 128, ALONG, P>);
     });
     SV_LAUNCH_CHECK();
-    if (c.R <= 1024 && s.nvt > 64)
-        hipLaunchKernelGGL(xent_rows_kernel<true>, dim3(lsec ? s.Rp : c.R), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
-    else
-        hipLaunchKernelGGL(xent_rows_kernel<false>, dim3(s.Rp / 32), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse, lsec);
+    const bool few_rows = c.R <= 1024 && s.nvt > 64;
+    float* const scale = grad ? (float*)(c.work + s.scale) : nullptr;
+    const unsigned blocks = (unsigned)(!few_rows ? s.Rp / 32 : grad ? s.Rp : c.R) + (scale ? 1 : 0);
+    hipLaunchKernelGGL(few_rows ? xent_rows_kernel<true> : xent_rows_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R,
+                       s.Rp, s.nvt, nll, lse, grad ? (float*)(c.work + s.lse) : nullptr, (const float*)(c.work + s.wrow), top_of(c.type), scale);
     SV_LAUNCH_CHECK();
     return 0;
 }
@@ -929,14 +971,58 @@ inline void piece(const Call& c, const Shape& s, const PieceArgs& a, unsigned bl
     });
 }
 
+// the kernels for few rows: loss (nll and lse given), gradients (row_weight and dh or dw given; lse: fwd's, where no loss is wanted)
+inline int few(const Call& c, const Shape& s, float* nll, float* lse, const float* given, const float* row_weight, void* dh, long long ld_dh,
+               void* dw, long long ld_dw, void* db) {
+    FewPrepArgs p;
+    p.h = c.hidden; p.tok = c.targets; p.row_weight = row_weight; p.lse = given;
+    p.hc = c.work + s.h; p.hg = row_weight ? c.work + s.hg : nullptr;
+    p.wrow = (float*)(c.work + s.wrow); p.lsec = (float*)(c.work + s.lse); p.tgt = (int*)(c.work + s.tgt);
+    p.ldh = c.ld_h; p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.D = c.D; p.Dp = s.Dp;
+    FewArgs a{};
+    a.w = c.weight; a.h = p.hc; a.hg = p.hg; a.bias = c.bias; a.tgt = p.tgt; a.lse = p.lsec; a.wrow = p.wrow;
+    a.part = nll ? (float2*)(c.work + s.part) : nullptr; a.zt = (float*)(c.work + s.zt);
+    a.z = row_weight ? (float*)(c.work + s.z) : nullptr; a.slab = dh ? (float*)(c.work + s.h_slab) : nullptr;
+    a.dw = dw; a.db = db; a.ldw = c.ld_w; a.ld_dw = ld_dw;
+    a.V = c.V; a.D = c.D; a.Dp = s.Dp; a.R = c.R; a.R4 = s.R4; a.Rp = s.Rp; a.ndt = s.ndt; a.chunks = s.chunks;
+    int rc = 0;
+    sv_by_type(c.type, [&](auto type) {
+        typedef decltype(type) T;
+        auto go = [&](auto kernel, long long blocks, auto... args) {
+            if (rc == 0) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, c.stream, args...);
+                rc = [&]() -> int {
+                    SV_LAUNCH_CHECK();
+                    return 0;
+                }();
+            }
+        };
+        go(few_prep_kernel<T>, ((long long)s.Rp * s.Dp + 255) / 256, p);
+        if (s.few == 1) go(few_logit_kernel<T, 1>, s.nvt, a);
+        else if (s.few == 2) go(few_logit_kernel<T, 2>, s.nvt, a);
+        else go(few_logit_kernel<T, 4>, s.nvt, a);
+        if (nll)
+            go(xent_rows_kernel<true>, row_weight ? s.Rp : c.R, (const float2*)a.part, (const float*)a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse,
+               row_weight ? p.lsec : (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);
+        if (!dh && !dw) return;
+        const long long blocks = (long long)s.chunks * s.ndt;
+        auto grad = [&](auto wide) {
+            constexpr int WD = decltype(wide)::value;
+            if (s.few == 1) go(few_grad_kernel<T, 1, WD>, blocks, a);
+            else if (s.few == 2) go(few_grad_kernel<T, 2, WD>, blocks, a);
+            else go(few_grad_kernel<T, 4, WD>, blocks, a);
+        };
+        if (s.wd == 1) grad(std::integral_constant<int, 1>{});
+        else if (s.wd == 2) grad(std::integral_constant<int, 2>{});
+        else grad(std::integral_constant<int, 4>{});
+        if (dh) go(few_sum_kernel<T>, (long long)c.R * (s.Dp / 4) / 8, (const float*)a.slab, s.chunks * (4 / s.wd), c.R, c.D, s.Dp, (T*)dh, ld_dh);
+    });
+    return rc;
+}
+
 // h: the rows of H that tiles of z are made from (the loss's or the gradient's copy; rows of weight 0 come to nothing either way)
 inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long long ld_dh, void* dw, long long ld_dw, void* db) {
-    const float* scale = nullptr;
-    if (c.type == SV_F16) {
-        scale = (const float*)(c.work + s.scale);
-        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, c.stream, (const float*)(c.work + s.wrow), s.Rp, (float*)(c.work + s.scale));
-        SV_LAUNCH_CHECK();
-    }
+    const float* const scale = (const float*)(c.work + s.scale);
     const int es = sv_elem_size(c.type);
     LogitArgs z = logit_args(c, s);
     z.h = c.work + h;
@@ -1044,9 +1130,10 @@ extern "C" int svae_xent_fwd(const void* hidden, long long ld_h, const void* wei
     int rc = check_call("svae_xent_fwd", c, work, work_bytes, LOSS, &s);
     if (rc != 0) return rc;
     SV_CHECK_ARG(nll && lse, "svae_xent_fwd: null pointer");
+    if (s.few) return few(c, s, nll, lse, nullptr, nullptr, nullptr, 0, nullptr, 0, nullptr);
     rc = prepare(c, s, true, nullptr, nullptr);
     if (rc != 0) return rc;
-    return loss(c, s, nll, lse, nullptr);
+    return loss(c, s, nll, lse, false);
 }
 
 extern "C" int svae_xent_reduce(const float* nll, const void* targets, int tok64, int R, int V, int mean, float* out, void* stream) {
@@ -1067,8 +1154,11 @@ extern "C" int svae_xent_bwd(const void* hidden, long long ld_h, const void* wei
     if (rc != 0) return rc;
     SV_CHECK_ARG(lse, "svae_xent_bwd: null pointer");
     if (!dh && !dw) return 0;
+    if (s.few) return few(c, s, nullptr, nullptr, lse, row_weight, dh, ld_dh, dw, ld_dw, db);
     rc = prepare(c, s, false, row_weight, lse);
     if (rc != 0) return rc;
+    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(256), 0, c.stream, (const float*)(c.work + s.wrow), s.Rp, top_of(type), (float*)(c.work + s.scale));
+    SV_LAUNCH_CHECK();
     return gradients(c, s, s.hg, dh, ld_dh, dw, ld_dw, db);
 }
 
@@ -1082,8 +1172,9 @@ extern "C" int svae_xent_fwd_bwd(const void* hidden, long long ld_h, const void*
     if (rc == 0) rc = check_gradients("svae_xent_fwd_bwd", D, row_weight, dh, ld_dh, dw, ld_dw, db);
     if (rc != 0) return rc;
     SV_CHECK_ARG(nll && lse, "svae_xent_fwd_bwd: null pointer");
+    if (s.few) return few(c, s, nll, lse, nullptr, row_weight, dh, ld_dh, dw, ld_dw, db);
     rc = prepare(c, s, true, row_weight, nullptr);
-    if (rc == 0) rc = loss(c, s, nll, lse, (float*)(c.work + s.lse));
+    if (rc == 0) rc = loss(c, s, nll, lse, true);
     if (rc != 0 || (!dh && !dw)) return rc;
     return gradients(c, s, s.h, dh, ld_dh, dw, ld_dw, db);
 }

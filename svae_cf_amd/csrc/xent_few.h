@@ -1,0 +1,420 @@
+// Softmax cross entropy for few rows: bound by reading W and writing its gradient, so that W is taken as it lies, once for the
+// loss and once for the gradients, without copies.  Part of xent.hip, whose formulas stand there.
+//
+//   loss       a wave holds z^T of 64 vocabulary entries and all rows; W goes from memory straight into the matrix units' registers.
+//              For a gradient z is kept (fp32, 4 R bytes a vocabulary entry; W has 2 D or 4 D).
+//   gradients  a workgroup makes G of 32 or 64 entries after the other from z, in LDS; its waves have 64 columns each, read W once
+//              for dH, whose sums stay in registers, and write dW.  Workgroups share the vocabulary and leave slabs of dH that are
+//              added in order.
+//
+// fp32 products are fp32 (v_mfma_f32_16x16x4), G and the gradients' products are for all types: nothing is rounded in between.
+// At NT tiles of 16 rows the products take 28 NT us for the loss (fp32; little for 16 bits) and 55 NT us for the gradients where
+// W has 131072 x 1024 numbers; reading W once takes 53 us (16 bits) or 106 us (fp32), writing its gradient as long.
+//
+// Measured there, loss | loss and gradients (us), against the kernels for many rows:
+//   fp32   1 row 135 | 358    (566 | 1285)     32 rows 144 | 411    (555 | 1320)     64 rows 235 | 754    (554 | 1333)
+//   bf16   1 row  50 | 206    ( 53 |  400)     32 rows  50 | 290    ( 52 |  397)     64 rows  53 | 433    ( 53 |  401)
+// so that they take up to 64 rows of fp32 and up to 32 of 16 bits.  (Loss and gradients have to take the same ones: z has to have
+// the same bits in both, or errors of z and of lse do not cancel in the gradient of a confident row.)
+#pragma once
+
+struct FewArgs {
+    const void *w, *h, *hg;   // W as it is; copies of H, zeros where a row does not take part: in the loss, in the gradient ([Rp][Dp])
+    const void* bias;         // or NULL
+    const int* tgt;           // [Rp], -1: left out
+    const float *lse, *wrow;  // [Rp], gradient
+    float2* part;             // loss: [vocabulary tiles][Rp], or NULL (z only)
+    float *zt, *z;            // z: [V][R4] or NULL
+    float* slab;              // [chunks * waves along V][R][Dp], or NULL: no dH
+    void *dw, *db;            // or NULL
+    long long ldw, ld_dw;     // elements
+    int V, D, Dp, R, R4, Rp, ndt, chunks;
+};
+
+// N numbers of any type from any address a number may have (the hardware's vector loads and stores need no more)
+template <typename T, int N>
+struct SomeOf {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T, int N>
+using Some = typename SomeOf<T, N>::type;
+
+// copies of H, targets, weights and lse of the rows
+struct FewPrepArgs {
+    const void *h, *tok;
+    const float *row_weight, *lse;        // NULL: loss only
+    void *hc, *hg;                        // NULL: not wanted
+    float *wrow, *lsec;
+    int* tgt;
+    long long ldh;
+    int tok64, R, Rp, V, D, Dp;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void few_prep_kernel(FewPrepArgs a) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / a.Dp;
+    const int c = (int)(i - r * a.Dp);
+    if (r >= a.Rp) return;
+    int tg = -1;
+    float w = 0.f;
+    if (r < a.R) {
+        const long long t = a.tok64 ? reinterpret_cast<const long long*>(a.tok)[r] : (long long)reinterpret_cast<const int*>(a.tok)[r];
+        if (t >= 0 && t < a.V) tg = (int)t;
+        if (tg >= 0 && a.row_weight != nullptr) w = a.row_weight[r];
+    }
+    if (c == 0) {
+        a.tgt[r] = tg;
+        if (a.row_weight != nullptr) a.wrow[r] = w;
+        if (a.lse != nullptr) a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
+    }
+    const T x = tg >= 0 && c < a.D ? reinterpret_cast<const T*>(a.h)[r * a.ldh + c] : (T)0.f;
+    // the loss's copy in the order in which the matrix units take it: 1 KiB for 16 rows and four times 16 bytes of them (rows a
+    // power of two apart fall on few channels of the cache: 64 rows of 256 fp32 took 457 us instead of 381 against a million)
+    constexpr int N = 16 / (int)sizeof(T);
+    const long long at = ((((long long)(c / (4 * N) / 2) * (a.Rp / 16) + r / 16) * 2 + c / (4 * N) % 2) * 64 + c / N % 4 * 16 + r % 16) * N + c % N;
+    if (a.hc != nullptr) reinterpret_cast<T*>(a.hc)[at] = x;
+    if (a.hg != nullptr) reinterpret_cast<T*>(a.hg)[i] = w != 0.f ? x : (T)0.f;
+}
+
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <typename T, int NT>
+__global__ __launch_bounds__(256, 2) void few_logit_kernel(FewArgs a) {
+    constexpr int N = 16 / (int)sizeof(T), STEP = 8 * N, MT = 4;       // 128 bytes of a row at a time, in two loads
+    typedef Some<T, N> Chunk;
+    __shared__ float2 red[4][16 * NT];
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long v0 = (long long)blockIdx.x * 256 + wave * 64;
+    const T* w[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const long long v = v0 + 16 * t + i16;                         // (entries behind V: another's row, put out below)
+        w[t] = reinterpret_cast<const T*>(a.w) + (v < a.V ? v : a.V - 1) * a.ldw + q * N;
+    }
+    const T* h = reinterpret_cast<const T*>(a.h) + lane * N;
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    Chunk x[MT][2], y[NT][2];
+    auto load_h = [&](int k, Chunk (&to)[NT][2]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) to[n][c] = *reinterpret_cast<const Chunk*>(h + ((k / STEP * NT + n) * 2 + c) * (64 * N));
+    };
+    auto load_w = [&](int k, Chunk (&to)[MT][2]) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) to[t][c] = *reinterpret_cast<const Chunk*>(w[t] + k + c * 4 * N);
+    };
+    auto multiply = [&]() {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            if constexpr (N == 8) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[t][n] = mfma<T>(__builtin_bit_cast(s16x8, x[t][c]), __builtin_bit_cast(s16x8, y[n][c]), acc[t][n]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)                            // (products of one sum do not follow on each other)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[t][n] = mfma_f32(x[t][c][e], y[n][c][e], acc[t][n]);
+            }
+        }
+    };
+    const int full = a.D / STEP;
+    if (full > 0) {
+        load_w(0, x);
+        load_h(0, y);
+    }
+    for (int s = 1; s < full; ++s) {                                   // the next step's loads are under way during the products
+        Chunk x2[MT][2], y2[NT][2];
+        load_w(s * STEP, x2);
+        load_h(s * STEP, y2);
+        __builtin_amdgcn_sched_barrier(0);                             // (the compiler would put them behind)
+        multiply();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[t][c] = x2[t][c];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) y[n][c] = y2[n][c];
+        }
+    }
+    if (full > 0) multiply();
+    if (full * STEP < a.D) {                                           // the rest of a row; H's copy has zeros there, up to Dp
+        load_h(full * STEP, y);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int k = full * STEP + c * 4 * N, left = a.D - k - q * N;
+                if (left >= N) x[t][c] = *reinterpret_cast<const Chunk*>(w[t] + k);
+                else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[t][c][e] = e < left ? w[t][k + e] : (T)0.f;
+                }
+            }
+        multiply();
+    }
+
+    // C: lane has row i16 of tile n, entries 4 q + i of tile t
+    const int rest = (int)(a.V - v0 < 64 ? a.V - v0 : 64);
+    if (a.bias != nullptr) {
+        const T* bias = reinterpret_cast<const T*>(a.bias) + v0;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = 16 * t + 4 * q + i;
+                const float b = rest == 64 || e < rest ? (float)bias[e] : 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[t][n][i] += b;
+            }
+    }
+    if (rest < 64) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[t][n][i] = 16 * t + 4 * q + i < rest ? acc[t][n][i] : -INFINITY;
+    }
+    if (a.z != nullptr) {
+        float* z = a.z + (v0 + 4 * q) * a.R4 + i16;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (16 * n + i16 < a.R4) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * t + 4 * q + i < rest) z[(16 * t + i) * a.R4 + 16 * n] = acc[t][n][i];
+            }
+    }
+    if (a.part == nullptr) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int rel = a.tgt[16 * n + i16] - ((int)v0 + 4 * q);       // (v0 is below 2^28)
+        if (__any(rel >= 0 && rel < 64)) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (rel == 16 * t + i) a.zt[16 * n + i16] = acc[t][n][i];
+        }
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, acc[t][n][i]);
+        // fmaxf leaves NaN out; the sum brings it back (exp(NaN - top))
+        const float base = m == -INFINITY ? 0.f : m * -LOG2E;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(fmaf(acc[t][n][i], LOG2E, base));
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+            join_sums(m, s, m2, s2);
+        }
+        if (q == 0) red[wave][16 * n + i16] = make_float2(m, s);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < 16 * NT) {
+        float m = red[0][threadIdx.x].x, s = red[0][threadIdx.x].y;
+#pragma unroll
+        for (int k = 1; k < 4; ++k) join_sums(m, s, red[k][threadIdx.x].x, red[k][threadIdx.x].y);
+        a.part[(long long)blockIdx.x * a.Rp + threadIdx.x] = make_float2(m, s);
+    }
+}
+
+// WD waves along the columns of W, 64 each; the others share the entries of a step
+constexpr int few_step(int wd) { return wd == 4 ? 32 : 64; }
+
+template <typename T, int NT, int WD>
+__global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs a) {
+    constexpr int WV = 4 / WD, STEP = few_step(WD), MINE = STEP / WV, ROWS = 16 * NT, PITCH = ROWS + 1;
+    constexpr int QUADS = (STEP * ROWS / 4 + 255) / 256;               // of G, that a thread makes in a step, at most
+    typedef Some<T, 4> Quad;
+    __shared__ float gs[2][STEP][PITCH];
+    __shared__ float wrow[ROWS], lse[ROWS];
+    __shared__ int tgt[ROWS];
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int dt = blockIdx.x % a.ndt, chunk = blockIdx.x / a.ndt;
+    const int d0 = (dt * WD + wave % WD) * 64, first = wave / WD * MINE;        // the wave's columns; its first entry in a step
+    const int steps = (a.V + STEP - 1) / STEP;
+    const int s0 = (int)((long long)steps * chunk / a.chunks), s1 = (int)((long long)steps * (chunk + 1) / a.chunks);
+    for (int i = threadIdx.x; i < ROWS; i += 256) {
+        wrow[i] = a.wrow[i];
+        lse[i] = a.lse[i];
+        tgt[i] = a.tgt[i];
+    }
+    for (int i = threadIdx.x; i < 2 * STEP * PITCH; i += 256) (&gs[0][0][0])[i] = 0.f;
+    __syncthreads();
+
+    const bool on = d0 < a.D;                                          // (else the wave only makes G)
+    // column of dW's tile j: a lane's entries 4 q ... 4 q + 3 of two tiles are eight columns in a row
+    auto column = [&](int j, int m) { return d0 + 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3); };
+    float ah[4 * NT][4];                                               // H for dW: rows 4 k + q, column i16 of tile j
+#pragma unroll
+    for (int k = 0; k < 4 * NT; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ah[k][j] = on ? (float)reinterpret_cast<const T*>(a.hg)[(4 * k + q) * a.Dp + column(j, i16)] : 0.f;
+    f32x4 sum[4][NT];                                                  // dH: columns 4 (4 q + i) + j, row i16 of tile n
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sum[j][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int per = a.R4 / 4, left = on ? a.D - d0 - 4 * i16 : 0;      // quads of an entry; columns of W that the lane has
+    f32x4 z[QUADS];
+    Quad x[MINE / 4], x2[MINE / 4];
+    auto load_z = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            const long long at = (long long)s * STEP * per + i;
+            z[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (i < STEP * per && at < (long long)a.V * per) z[k] = reinterpret_cast<const f32x4*>(a.z)[at];
+        }
+    };
+    auto make_g = [&](int s, float (*to)[PITCH]) {
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            if (i >= STEP * per) break;
+            const int e = i / per, r = (i - e * per) * 4;
+            const long long v = (long long)s * STEP + e;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float wr = wrow[r + j];
+                const float p = __builtin_amdgcn_exp2f((z[k][j] - lse[r + j]) * LOG2E) - (tgt[r + j] == v ? 1.f : 0.f);
+                to[e][r + j] = wr == 0.f || v >= a.V ? 0.f : p * wr;   // (a row without a part comes to nothing, whatever its z is)
+            }
+        }
+    };
+    auto load_w = [&](int s, Quad (&to)[MINE / 4]) {
+#pragma unroll
+        for (int g = 0; g < MINE / 4; ++g) {
+            const long long v = (long long)s * STEP + first + 4 * g + q;        // (entries behind V: another's row times zero)
+            const T* p = reinterpret_cast<const T*>(a.w) + (v < a.V ? v : a.V - 1) * a.ldw + d0 + 4 * i16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[g][e] = (T)0.f;
+            if (left >= 4) to[g] = *reinterpret_cast<const Quad*>(p);
+            else if (left > 0) {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (e < left) to[g][e] = p[e];
+            }
+        }
+    };
+    if (s0 < s1) {
+        load_z(s0);
+        if (a.slab != nullptr) load_w(s0, x);
+        make_g(s0, gs[s0 & 1]);
+    }
+    __syncthreads();
+    for (int s = s0; s < s1; ++s) {
+        const float (*g)[PITCH] = gs[s & 1];
+        const bool more = s + 1 < s1;
+        if (more) {
+            load_z(s + 1);
+            if (a.slab != nullptr) load_w(s + 1, x2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (a.slab != nullptr && on) {
+#pragma unroll
+            for (int k = 0; k < MINE / 4; ++k) {
+                float b[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) b[n] = g[first + 4 * k + q][16 * n + i16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) sum[j][n] = mfma_f32((float)x[k][j], b[n], sum[j][n]);
+            }
+        }
+        if (a.dw != nullptr && on) {
+#pragma unroll
+            for (int t = 0; t < MINE / 16; ++t) {
+                f32x4 c[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4 * NT; ++k) {
+                    const float b = g[first + 16 * t + i16][4 * k + q];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = mfma_f32(ah[k][j], b, c[j]);
+                }
+                const long long v = (long long)s * STEP + first + 16 * t + i16;
+                if (v < a.V) {
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        const int d = column(j, 4 * q);
+                        T* o = reinterpret_cast<T*>(a.dw) + v * a.ld_dw + d;
+                        Some<T, 8> out;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) out[e] = (T)c[j + e / 4][e % 4];
+                        if (d + 7 < a.D) *reinterpret_cast<Some<T, 8>*>(o) = out;
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 7; ++e)
+                                if (d + e < a.D) o[e] = out[e];
+                        }
+                    }
+                }
+            }
+        }
+        if (a.db != nullptr && dt == 0 && (int)threadIdx.x < STEP) {
+            const long long v = (long long)s * STEP + threadIdx.x;
+            float b = 0.f;
+            for (int r = 0; r < a.R; ++r) b += g[threadIdx.x][r];
+            if (v < a.V) reinterpret_cast<T*>(a.db)[v] = (T)b;
+        }
+        if (more) {
+            make_g(s + 1, gs[(s + 1) & 1]);                            // (read by every wave before the last barrier)
+#pragma unroll
+            for (int k = 0; k < MINE / 4; ++k) x[k] = x2[k];
+        }
+        __syncthreads();
+    }
+    if (a.slab == nullptr || !on) return;
+    float* slab = a.slab + (long long)(chunk * WV + wave / WD) * a.R * a.Dp;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (16 * n + i16 < a.R)
+                *reinterpret_cast<f32x4*>(slab + (long long)(16 * n + i16) * a.Dp + d0 + 16 * q + 4 * i) =
+                    (f32x4){sum[0][n][i], sum[1][n][i], sum[2][n][i], sum[3][n][i]};
+}
+
+// dH: sum of the slabs in a fixed order; a workgroup has 8 quads of columns, 32 threads share the slabs of each
+template <typename T>
+__global__ __launch_bounds__(256) void few_sum_kernel(const float* __restrict__ slab, int slabs, int R, int D, int Dp, T* __restrict__ out, long long ld) {
+    __shared__ f32x4 red[32][8];
+    const int i = threadIdx.x & 7, s = threadIdx.x >> 3;
+    const long long at = (long long)blockIdx.x * 8 + i, all = (long long)R * (Dp / 4);        // (Dp / 4 is a multiple of 16)
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = s; k < slabs; k += 32) x += *reinterpret_cast<const f32x4*>(slab + ((long long)k * all + at) * 4);
+    red[s][i] = x;
+    __syncthreads();
+    if (s != 0) return;
+    for (int k = 1; k < 32; ++k) x += red[k][i];
+    const long long r = at / (Dp / 4);
+    const int d = (int)(at - r * (Dp / 4)) * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (d + j < D) out[r * ld + d + j] = (T)x[j];
+}
