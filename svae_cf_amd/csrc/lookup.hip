@@ -316,8 +316,9 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = ((int)blockIdx.y * 64 + lane) * VEC;       // the launch's second dimension goes over slices of the columns
-    if ((int)blockIdx.x < nchunk) {
-        const int p0 = (int)blockIdx.x * CHUNK, p1 = R - p0 < CHUNK ? R : p0 + CHUNK;
+    const int block = (int)(blockIdx.z * gridDim.x + blockIdx.x);
+    if (block < nchunk) {
+        const int p0 = block * CHUNK, p1 = R - p0 < CHUNK ? R : p0 + CHUNK;
         // the chunk's keys and those of 64 places on either side: enough to tell which runs are long
         const int kin = p0 + lane < p1 ? keys[p0 + lane] : -1;
         const int kf = __builtin_amdgcn_readfirstlane(kin), kl = __builtin_amdgcn_readlane(kin, p1 - p0 - 1);
@@ -342,13 +343,13 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
 #pragma unroll
                 for (int q = 0; q < VEC; ++q)
                     acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
-                sv_store<VEC>(part + ((size_t)blockIdx.x * 2 + slot) * D + c, acc);
+                sv_store<VEC>(part + ((size_t)block * 2 + slot) * D + c, acc);
             }
             __syncthreads();
         }
         return;
     }
-    const long long v0 = ((long long)((int)blockIdx.x - nchunk) * 4 + wave) * group;
+    const long long v0 = ((long long)(block - nchunk) * 4 + wave) * group;
     if (v0 >= V) return;
     const int s0 = lower_bound(keys, 0, R, v0, lane);
     // the keys from there on tell the other bounds, unless there are more than 64 of them
@@ -383,7 +384,8 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
     __shared__ float red[4][64 * VEC];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int p0 = (int)blockIdx.x * CHUNK;
+    const int block = (int)(blockIdx.z * gridDim.x + blockIdx.x);
+    const int p0 = block * CHUNK;
     if (R - p0 <= CHUNK) return;                             // no segment of more than LONG starts in the last places
     const int kin = keys[p0 + lane];
     const int k = __builtin_amdgcn_readlane(kin, 63);
@@ -402,8 +404,8 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
     for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
     if (c < D) {
         // partial sums are rows of D floats, two for a chunk; only the first chunk's may be in the second one
-        auto at = [&](int j) { return 2 * j + (j == (int)blockIdx.x ? slot0 : 0); };
-        sum_rows<VEC>(part, D, at, (int)blockIdx.x + wave, last + 1, 4, c, acc);
+        auto at = [&](int j) { return 2 * j + (j == block ? slot0 : 0); };
+        sum_rows<VEC>(part, D, at, block + wave, last + 1, 4, c, acc);
     }
 #pragma unroll
     for (int q = 0; q < VEC; ++q) red[wave][q * 64 + lane] = acc[q];
@@ -430,14 +432,16 @@ extern "C" int svae_lookup_fwd(const void* table, int table_type, long long ld_t
     const int vec = sv_vec_for(8, D, table, ld_table, sv_elem_size(table_type), out, ld_out, sv_elem_size(out_type));
     int lg = 0;
     while (lg < 8 && (vec << lg) < D) ++lg;
-    const unsigned nwg = (unsigned)(((long long)R + (256 >> lg) - 1) / (256 >> lg));
-    sv_by_type(table_type, [&](auto t) {
+    const long long most = 1ll << (31 - lg);                        // rows of a launch: its threads are counted in 32 bits
+    for (long long r0 = 0; r0 < R; r0 += most) sv_by_type(table_type, [&](auto t) {
         sv_by_type(out_type, [&](auto o) {
             typedef decltype(t) T;
             typedef decltype(o) O;
+            const int rows = R - r0 < most ? (int)(R - r0) : most;
+            const unsigned nwg = (unsigned)(((long long)rows + (256 >> lg) - 1) / (256 >> lg));
             auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(nwg), dim3(256), 0, (hipStream_t)stream, (const T*)table, ld_table, tokens, tok64,
-                                   (O*)out, ld_out, R, V, D, lg, scale);
+                hipLaunchKernelGGL(kernel, dim3(nwg), dim3(256), 0, (hipStream_t)stream, (const T*)table, ld_table,
+                                   (const char*)tokens + r0 * (tok64 ? 8 : 4), tok64, (O*)out + r0 * ld_out, ld_out, rows, V, D, lg, scale);
             };
             if (vec == 8) go(lookup_fwd_kernel<8, T, O>);
             else if (vec == 4) go(lookup_fwd_kernel<4, T, O>);
@@ -483,7 +487,9 @@ extern "C" int svae_token_sort(const void* tokens, int tok64, int R, int V, int 
     int* k2 = (int*)w;
     int* p2 = (int*)(w + align256(4ll * R));
     const size_t lds = ((size_t)18 << s.bits) * 4 + 64;
-    const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    // (always the most that a call may need, so that calls from several threads do not take it from each other)
+    const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                (18 << SORT_MAX_BITS) * 4 + 64);
     if (attr != hipSuccess) return svae_fail((int)attr, "svae_token_sort: %s", hipGetErrorString(attr));
     for (int p = 0; p < s.passes; ++p) {
         const bool to_out = ((s.passes - 1 - p) & 1) == 0;
@@ -521,20 +527,24 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
     // rows of 256, 21800 tokens: 16 rows 16.6 us, 4 rows 12.7 us)
     const int group = V >= 8192 * MOST_GROUP ? MOST_GROUP : V >= 8192 * 8 ? 8 : 4;
     const long long nrow = ((long long)V + 4 * group - 1) / (4 * group);
-    SV_CHECK_ARG(nchunk + nrow < 0x7fffffffll, "svae_lookup_bwd: R %d and V %d need too many workgroups", R, V);
     int vec = sv_vec_for(8, D, R ? dy : grad, R ? ld_dy : ld_grad, sv_elem_size(dy_type), grad, ld_grad, sv_elem_size(grad_type));
     while (vec > 2 && 32 * vec >= D) vec >>= 1;              // rather all 64 lanes with shorter vectors
     const unsigned slices = (unsigned)((D + 64 * vec - 1) / (64 * vec));
     SV_CHECK_ARG(slices <= 65535u, "svae_lookup_bwd: D %d is too wide for rows that start at odd places", D);
+    // (threads of a dimension are counted in 32 bits: more workgroups than 2^23 go on in the third one)
+    auto grid = [&](long long blocks) {
+        const long long most = 1ll << 23;
+        return dim3((unsigned)(blocks < most ? blocks : most), slices, (unsigned)((blocks + most - 1) / most));
+    };
     sv_by_type(dy_type, [&](auto t) {
         sv_by_type(grad_type, [&](auto o) {
             typedef decltype(t) T;
             typedef decltype(o) G;
             auto go = [&](auto kernel, auto join) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)(nchunk + nrow), slices), dim3(256), 0, (hipStream_t)stream, (const T*)dy, ld_dy, keys,
+                hipLaunchKernelGGL(kernel, grid(nchunk + nrow), dim3(256), 0, (hipStream_t)stream, (const T*)dy, ld_dy, keys,
                                    perm, R, V, D, scale, (G*)grad, ld_grad, accumulate, nchunk, group, (float*)work);
                 if (R > LONG)
-                    hipLaunchKernelGGL(join, dim3((unsigned)nchunk, slices), dim3(256), 0, (hipStream_t)stream, keys, R, V, D, scale, (G*)grad,
+                    hipLaunchKernelGGL(join, grid(nchunk), dim3(256), 0, (hipStream_t)stream, keys, R, V, D, scale, (G*)grad,
                                        ld_grad, accumulate, (const float*)work);
             };
             if (vec == 8) go(lookup_bwd_kernel<8, T, G>, lookup_bwd_long_kernel<8, G>);

@@ -241,6 +241,13 @@ __device__ __forceinline__ int tile_of(unsigned block, int total) {
     return (int)(block >> 3) < per && t < total ? t : -1;
 }
 inline unsigned blocks_for(long long tiles) { return (unsigned)((tiles + 7) / 8 * 8); }
+// launches of more than 2^24 workgroups of 256 threads need a second dimension (threads are counted in 32 bits); workgroups behind
+// the last one asked for have to find nothing to do
+constexpr long long MOST_BLOCKS = 1ll << 23;
+inline dim3 grid_of(long long blocks) {
+    return blocks <= MOST_BLOCKS ? dim3((unsigned)blocks) : dim3((unsigned)MOST_BLOCKS, (unsigned)((blocks + MOST_BLOCKS - 1) / MOST_BLOCKS));
+}
+__device__ __forceinline__ long long block_of() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
 
 // (maximum, sum of exponentials above it) of two sets of logits
 __device__ __forceinline__ void join_sums(float& m, float& s, float m2, float s2) {
@@ -545,12 +552,13 @@ struct SumArgs {
     const float* scale;
     long long slab_stride, ld_out;
     int splits, rows, D, Dp;              // (the bias gradient: one column, Dp = 1)
-    unsigned blocks;
+    long long blocks;
 };
 template <typename T>
-__device__ __forceinline__ void sum_slabs(const SumArgs& a, unsigned block) {
+__device__ __forceinline__ void sum_slabs(const SumArgs& a, long long block) {
+    if (block >= a.blocks) return;
     const float down = a.scale[1];
-    const long long i = (long long)block * 256 + threadIdx.x;
+    const long long i = block * 256 + threadIdx.x;
     if (a.Dp == 1) {
         if (i >= a.rows) return;
         float s = 0.f;
@@ -572,9 +580,10 @@ __device__ __forceinline__ void sum_slabs(const SumArgs& a, unsigned block) {
 }
 template <typename T>
 __global__ __launch_bounds__(256) void xent_slab_sum_kernel(SumArgs h, SumArgs w, SumArgs b) {
-    if (blockIdx.x < h.blocks) sum_slabs<T>(h, blockIdx.x);
-    else if (blockIdx.x < h.blocks + w.blocks) sum_slabs<T>(w, blockIdx.x - h.blocks);
-    else sum_slabs<T>(b, blockIdx.x - h.blocks - w.blocks);
+    const long long block = block_of();
+    if (block < h.blocks) sum_slabs<T>(h, block);
+    else if (block < h.blocks + w.blocks) sum_slabs<T>(w, block - h.blocks);
+    else sum_slabs<T>(b, block - h.blocks - w.blocks);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -588,8 +597,8 @@ struct PrepArgs {
     char *hc, *hg, *wc;                   // hg (or NULL): without the rows of weight 0; wc NULL: W is not copied, and hc has rows
     float *biasf, *wrow, *lsec;           // lsec: a copy of lse, where it is given
     int* tgt;
-    long long ldh, ldw, h_part, w_part;
-    int tok64, R, Rp, V, Vp, D, Dp, nh, nb, wide_h, wide_w;
+    long long ldh, ldw, h_part, w_part, nh, nb;       // nh, nb: workgroups of H and of the bias; the others copy W
+    int tok64, R, Rp, V, Vp, D, Dp, wide_h, wide_w;
 };
 
 // eight columns of one row: from T to E, in PARTS parts
@@ -625,8 +634,8 @@ __device__ __forceinline__ long long block_at(long long r, int c, int Dp) {
 template <typename T, typename E, int PARTS>
 __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
     const int per = a.Dp / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if ((int)blockIdx.x < a.nh) {
+    const long long block = block_of(), i = block * 256 + threadIdx.x;
+    if (block < a.nh) {
         const long long r = i / per;
         const int c = (int)(i - r * per) * 8;
         if (r >= a.Rp) return;
@@ -646,11 +655,11 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
         const long long to = a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2;
         if (a.hc != nullptr) copy8<T, E, PARTS>(src, a.D - c, tg >= 0, a.wide_h, a.hc + to, a.h_part);
         if (a.hg != nullptr) copy8<T, E, PARTS>(src, a.D - c, w != 0.f, a.wide_h, a.hg + to, a.h_part);
-    } else if ((int)blockIdx.x < a.nh + a.nb) {
-        const long long v = i - (long long)a.nh * 256;
+    } else if (block < a.nh + a.nb) {
+        const long long v = i - a.nh * 256;
         if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
     } else {
-        const long long j = i - (long long)(a.nh + a.nb) * 256, r = j / per;
+        const long long j = i - (a.nh + a.nb) * 256, r = j / per;
         const int c = (int)(j - r * per) * 8;
         if (r >= a.Vp) return;
         copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + (r < a.V ? r : 0) * a.ldw + c, a.D - c, r < a.V, a.wide_w, a.wc + block_at(r, c, a.Dp), a.w_part);
@@ -827,7 +836,6 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->ndt = (s->Dp + BM - 1) / BM;
     s->dblocks = (s->Dp / 32 + s->ndt - 1) / s->ndt;
     s->dblocks = s->BN == 64 ? 8 : s->dblocks <= 2 ? 2 : s->dblocks <= 4 ? 4 : s->dblocks;
-    SV_CHECK_ARG((long long)s->nvt * s->nrt < 0x7ffffff0ll, "svae_xent: R %lld and V %lld need too many workgroups", R, V);
     s->h_part = (long long)s->Rp * s->Dp * 2;
     s->h = take(s->h_part * s->parts);
     s->hg = grad == LOSS ? 0 : take(s->h_part * s->parts);
@@ -899,13 +907,12 @@ inline int prepare(const Call& c, const Shape& s, bool loss, const float* row_we
     p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.Vp = s.Vp; p.D = c.D; p.Dp = s.Dp;
     const long long nh = ((long long)s.Rp * (s.Dp / 8) + 255) / 256, nb = (s.Vp + 255) / 256,
                     nw = s.direct ? 0 : ((long long)s.Vp * (s.Dp / 8) + 255) / 256;
-    SV_CHECK_ARG(nh + nb + nw < 0x7ffffff0ll, "svae_xent: too large");
-    p.nh = (int)nh; p.nb = (int)nb;
+    p.nh = nh; p.nb = nb;
     const int es = sv_elem_size(c.type);
     p.wide_h = sv_vec_for(8, c.D, c.hidden, c.ld_h, es, c.hidden, c.ld_h, es) == 8;
     p.wide_w = sv_vec_for(8, c.D, c.weight, c.ld_w, es, c.weight, c.ld_w, es) == 8;
     by_type(c.type, [&](auto t, auto e, auto parts) {
-        hipLaunchKernelGGL((xent_prep_kernel<decltype(t), decltype(e), decltype(parts)::value>), dim3((unsigned)(nh + nb + nw)), dim3(256), 0, c.stream, p);
+        hipLaunchKernelGGL((xent_prep_kernel<decltype(t), decltype(e), decltype(parts)::value>), grid_of(nh + nb + nw), dim3(256), 0, c.stream, p);
     });
     SV_LAUNCH_CHECK();
     return 0;
@@ -927,12 +934,14 @@ inline float top_of(int type) { return type == SV_F16 ? 16384.f : 1.f; }
 // grad: gradients follow, which read lse and the scale from the workspace
 inline int loss(const Call& c, const Shape& s, float* nll, float* lse, bool grad) {
     LogitArgs a = logit_args(c, s);
-    a.part = (float2*)(c.work + s.part);
     a.zt = (float*)(c.work + s.zt);
-    a.v_begin = 0; a.nvt = s.nvt;
-    by_type(c.type, [&](auto, auto e, auto parts) {
+    const int slice = (int)(MOST_BLOCKS / s.nrt);          // vocabulary tiles of a launch, at most
+    for (int v = 0; v < s.nvt; v += slice) by_type(c.type, [&](auto, auto e, auto parts) {
         typedef decltype(e) E;
         constexpr int P = decltype(parts)::value;
+        a.v_begin = v * BM;
+        a.nvt = s.nvt - v < slice ? s.nvt - v : slice;
+        a.part = (float2*)(c.work + s.part) + (long long)v * s.Rp;
         const dim3 grid(blocks_for((long long)a.nvt * a.nrt));
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, a); };
         if constexpr (P == 1) {
@@ -949,8 +958,8 @@ inline int loss(const Call& c, const Shape& s, float* nll, float* lse, bool grad
     const bool few_rows = c.R <= 1024 && s.nvt > 64;
     float* const scale = grad ? (float*)(c.work + s.scale) : nullptr;
     const unsigned blocks = (unsigned)(!few_rows ? s.Rp / 32 : grad ? s.Rp : c.R) + (scale ? 1 : 0);
-    hipLaunchKernelGGL(few_rows ? xent_rows_kernel<true> : xent_rows_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, a.part, a.zt, a.tgt, c.R,
-                       s.Rp, s.nvt, nll, lse, grad ? (float*)(c.work + s.lse) : nullptr, (const float*)(c.work + s.wrow), top_of(c.type), scale);
+    hipLaunchKernelGGL(few_rows ? xent_rows_kernel<true> : xent_rows_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, (const float2*)(c.work + s.part), a.zt,
+                       a.tgt, c.R, s.Rp, s.nvt, nll, lse, grad ? (float*)(c.work + s.lse) : nullptr, (const float*)(c.work + s.wrow), top_of(c.type), scale);
     SV_LAUNCH_CHECK();
     return 0;
 }
@@ -1068,6 +1077,7 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
                 a.nw = blocks_for((long long)a.w.ndt * a.w.nnt * a.w.splits);
             }
         }
+        SV_CHECK_ARG((long long)nz + a.nh + a.nw < 1ll << 24, "svae_xent: R %d, V %d, D %d need too many workgroups", c.R, c.V, c.D);
         piece(c, s, a, nz + a.nh + a.nw);
         SV_LAUNCH_CHECK();
     }
@@ -1075,20 +1085,20 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
     if (dh) {
         h1.slab = (const float*)(c.work + s.h_slab); h1.slab_stride = (long long)s.Rp * s.Dp; h1.out = dh; h1.ld_out = ld_dh;
         h1.scale = scale; h1.splits = s.h_splits; h1.rows = c.R; h1.D = c.D; h1.Dp = s.Dp;
-        h1.blocks = (unsigned)(((long long)c.R * (s.Dp / 4) + 255) / 256);
+        h1.blocks = ((long long)c.R * (s.Dp / 4) + 255) / 256;
     }
     if (dw && wslab) {
         w1.slab = wslab; w1.slab_stride = (long long)s.Vp * s.Dp; w1.out = dw; w1.ld_out = ld_dw;
         w1.scale = scale; w1.splits = s.w_splits; w1.rows = c.V; w1.D = c.D; w1.Dp = s.Dp;
-        w1.blocks = (unsigned)(((long long)c.V * (s.Dp / 4) + 255) / 256);
+        w1.blocks = ((long long)c.V * (s.Dp / 4) + 255) / 256;
     }
     if (db && bslab) {
         b1.slab = bslab; b1.slab_stride = s.Vp; b1.out = db; b1.scale = scale; b1.splits = s.w_splits; b1.rows = c.V; b1.D = b1.Dp = 1;
-        b1.blocks = (unsigned)((c.V + 255) / 256);
+        b1.blocks = (c.V + 255) / 256;
     }
     if (h1.blocks + w1.blocks + b1.blocks > 0) {
         by_type(c.type, [&](auto t, auto, auto) {
-            hipLaunchKernelGGL(xent_slab_sum_kernel<decltype(t)>, dim3(h1.blocks + w1.blocks + b1.blocks), dim3(256), 0, c.stream, h1, w1, b1);
+            hipLaunchKernelGGL(xent_slab_sum_kernel<decltype(t)>, grid_of(h1.blocks + w1.blocks + b1.blocks), dim3(256), 0, c.stream, h1, w1, b1);
         });
         SV_LAUNCH_CHECK();
     }

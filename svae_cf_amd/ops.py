@@ -74,6 +74,14 @@ def _rows(t):
     return t, ld
 
 
+def _apart(a, b):
+    """Whether two tensors share no address."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return not a.numel() or not b.numel() or a1 <= b0 or b1 <= a0
+
+
 def _flat(t):
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
@@ -100,6 +108,14 @@ def _lookup(table, tokens, scale, out_dtype):
             _lib.call("svae_lookup_fwd", tab.data_ptr(), _TYPES[tab.dtype], ld, tok.data_ptr(), _IDS[tok.dtype], out.data_ptr(),
                       _TYPES[out_dtype], D, R, V, D, scale, st)
     return out if tokens.dim() == 1 else out.view(tokens.shape + (D,))
+
+
+def _pad(padding_idx, V):
+    if padding_idx is None:
+        return -1
+    if not 0 <= int(padding_idx) < V:
+        raise ValueError("padding_idx %d is outside the table of %d rows" % (padding_idx, V))
+    return int(padding_idx)
 
 
 class _Embedding(torch.autograd.Function):
@@ -131,6 +147,7 @@ def embedding(table, tokens, scale=1.0, padding_idx=None, out_dtype=None):
     _size(table.shape[0], "vocabulary")
     _size(table.shape[1], "width", 1 << 24)
     _size(tokens.numel() + 1, "tokens + 1", (1 << 30) + 1)
+    _pad(padding_idx, table.shape[0])
     if torch.is_grad_enabled() and table.requires_grad:
         return _Embedding.apply(table, tokens, float(scale), padding_idx, out_dtype)
     return _lookup(table, tokens, float(scale), out_dtype)
@@ -160,9 +177,9 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=No
         _check(out, "out", device=dout.get_device())
         if tuple(out.shape) != (V, D) or (D > 1 and out.stride(1) != 1) or (V > 1 and out.stride(0) < D) or dtype not in (None, out.dtype):
             raise ValueError("out must be [%d, %d] with rows that can be addressed%s" % (V, D, "" if dtype is None else " and type %s" % dtype))
-    pad = -1 if padding_idx is None else int(padding_idx)
-    if padding_idx is not None and not 0 <= pad < V:
-        raise ValueError("padding_idx %d is outside the table of %d rows" % (pad, V))
+        if not _apart(out, dout):
+            raise ValueError("out must lie apart from dout")
+    pad = _pad(padding_idx, V)
     tok, (dy, ld) = _flat(tokens), _rows(dout if dout.dim() == 2 else dout.reshape(R, D))
     n_sort, n_sum = _bytes("svae_token_sort_bytes", R, V), _bytes("svae_lookup_bwd_bytes", R, D)
     keep = (2 * R + 127) // 128 * 512                     # keys and places, then what either call needs
@@ -195,13 +212,14 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, p, seed, step, row_key):
         # (a step on the device is copied: the program may advance it before the backward pass makes the mask again)
         step = step.clone() if isinstance(step, torch.Tensor) else step
-        ctx.args = (p, seed, step, row_key)
+        ctx.save_for_backward(row_key)
+        ctx.args = (p, seed, step)
         return _dropout(x, p, seed, step, row_key)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _dropout(dy, *ctx.args), None, None, None, None
+        return _dropout(dy, *ctx.args, *ctx.saved_tensors), None, None, None, None
 
 
 def dropout(x, p, seed, step=0, row_key=None, out=None):
@@ -211,7 +229,7 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
     kept); 0 and 1 are allowed, other values must not round to them.  seed: 64 bits.  step: int, or an int64 tensor of one
     element on the GPU that the kernel reads, so that a captured graph draws a new mask at every replay.  row_key: int64, one
     for each row (default: the row's index); with keys that travel with the rows a mask does not depend on how rows are dealt
-    to GPUs.  The gradient is the same call on dy.  ``out`` (contiguous, may be x) is for calls outside autograd."""
+    to GPUs.  The gradient is the same call on dy.  ``out`` (contiguous; x itself or apart from it) is for calls outside autograd."""
     _check(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have columns, got %s" % (tuple(x.shape),))
@@ -239,6 +257,8 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
         _check(out, "out", {x.dtype: 0}, x.get_device())
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and shaped like x")
+        if not _apart(x, out) and not (x.is_contiguous() and x.data_ptr() == out.data_ptr()):
+            raise ValueError("out must be x itself or lie apart from it")
     return _dropout(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key, out)
 
 

@@ -294,3 +294,39 @@ def test_operators_on_another_stream():
     both = ops.embedding_grad(dy, tok, V)
     torch.cuda.synchronize()
     assert all(torch.equal(w, want) for w in got + [both])
+
+
+def test_calls_that_are_refused():
+    from svae_cf_amd import ops
+    table, tok = torch.randn(10, 8, device="cuda", requires_grad=True), torch.tensor([1, 2], device="cuda")
+    with pytest.raises(ValueError, match="padding_idx"):           # (not only in the backward pass)
+        ops.embedding(table, tok, padding_idx=10)
+    x = torch.randn(40, 16, device="cuda")
+    for out in (x.view(-1)[8:8 + 320].view(20, 16), x[10:30]):
+        with pytest.raises(ValueError, match="apart"):
+            ops.dropout(x[:20], 0.5, 1, out=out)
+    with pytest.raises(ValueError, match="apart"):                 # rows of the input behind others of the output
+        ops.dropout(x[::2], 0.5, 1, out=x[:20])
+    with pytest.raises(ValueError, match="apart"):
+        ops.embedding_grad(x[:2], tok, 10, out=x[:10])
+    key = torch.arange(5, device="cuda")
+    y = ops.dropout(torch.randn(5, 8, device="cuda", requires_grad=True), 0.5, 1, row_key=key)
+    key += 1                                                       # the mask of the backward pass would be another
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+def test_more_threads_than_32_bits_count():
+    """16 777 221 rows of 257 numbers, 256 threads each; 2^29 tokens, whose chunks of 64 are more than 2^23 workgroups."""
+    from svae_cf_amd import ops
+    table = torch.randn(50, 257, device="cuda").to(BF16)
+    tok = (torch.arange((1 << 24) + 5, device="cuda") % 50).int()
+    y = ops.embedding(table, tok)
+    for at in (0, (1 << 23) - 3, (1 << 23), (1 << 24) - 2, (1 << 24)):
+        assert torch.equal(y[at:at + 5], table[tok[at:at + 5].long()])
+    del y
+    R, V = (1 << 29) + 77, 1000
+    tok = (torch.arange(R, device="cuda") % V).int()
+    grad = ops.embedding_grad(torch.ones(R, 1, dtype=BF16, device="cuda"), tok, V, dtype=F32)
+    want = R // V + (torch.arange(V, device="cuda") < R % V)       # sums of ones, below 2^24: exact
+    assert torch.equal(grad.view(-1).long(), want)

@@ -346,6 +346,20 @@ def test_weight_past_32_bit_offsets(R):
     assert abs(float(dh[0, 0]) - (4 * p[1] + 8 * (p[0] - 1))) <= 3 * 2.0 ** -8 * 8 and float(dh[0, 1]) == 0
 
 
+def test_loss_of_more_tiles_than_a_launch_takes():
+    """2^24 rows and 130 tiles of the vocabulary: three launches.  Logits that are the bias alone: every sum is known."""
+    from svae_cf_amd import ops
+    R, V = 1 << 24, 33100
+    b = torch.zeros(V, dtype=BF16, device="cuda")
+    b[[5, 16384, V - 1]] = torch.tensor([2.0, 4.0, 6.0], device="cuda").to(BF16)
+    t = torch.arange(R, device="cuda", dtype=torch.int32) % V
+    nll, lse = ops.linear_nll(torch.randn(R, 8, device="cuda").to(BF16), torch.zeros(V, 8, dtype=BF16, device="cuda"), t, bias=b)
+    want = np.log(V - 3 + np.exp(2.0) + np.exp(4.0) + np.exp(6.0))
+    tol = (V / 16384 + 200) * U + 2.0 ** -22 + 2 * U * want        # as Ref's, with exact logits
+    assert float((lse.double() - want).abs().max()) <= tol
+    assert float((nll.double() - (want - b.double()[t.long()])).abs().max()) <= tol + U * want
+
+
 def test_captured_gradients_two_graphs():
     """Two graphs of different sizes replayed in turn on new inputs, with eager calls between: every replay equals the eager result."""
     from svae_cf_amd import ops
