@@ -772,6 +772,9 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS_F32 = 64, FEW_ROWS_16 = 32;          // up to here: the kernels for few rows
+// vocabulary tiles up to which a loss of one tile of rows takes H as it lies: without the launch for the copy, which however is
+// read faster (bf16, one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
+constexpr int FEW_OWN_TILES = 2048;
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
 constexpr long long PIECE_LEAST = 128ll << 20, PIECE_MOST = 512ll << 20;     // what G of a piece may take; there are two
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
@@ -992,7 +995,7 @@ inline int few(const Call& c, const Shape& s, float* nll, float* lse, const floa
     a.w = c.weight; a.h = p.hc; a.hg = p.hg; a.bias = c.bias; a.tgt = p.tgt; a.lse = p.lsec; a.wrow = p.wrow;
     a.part = nll ? (float2*)(c.work + s.part) : nullptr; a.zt = (float*)(c.work + s.zt);
     a.z = row_weight ? (float*)(c.work + s.z) : nullptr; a.slab = dh ? (float*)(c.work + s.h_slab) : nullptr;
-    a.dw = dw; a.db = db; a.ldw = c.ld_w; a.ld_dw = ld_dw;
+    a.dw = dw; a.db = db; a.ldw = c.ld_w; a.ld_dw = ld_dw; a.ldh = c.ld_h; a.tok = c.targets; a.tok64 = c.tok64;
     a.V = c.V; a.D = c.D; a.Dp = s.Dp; a.R = c.R; a.R4 = s.R4; a.Rp = s.Rp; a.ndt = s.ndt; a.chunks = s.chunks;
     int rc = 0;
     sv_by_type(c.type, [&](auto type) {
@@ -1006,10 +1009,15 @@ inline int few(const Call& c, const Shape& s, float* nll, float* lse, const floa
                 }();
             }
         };
-        go(few_prep_kernel<T>, ((long long)s.Rp * s.Dp + 255) / 256, p);
-        if (s.few == 1) go(few_logit_kernel<T, 1>, s.nvt, a);
-        else if (s.few == 2) go(few_logit_kernel<T, 2>, s.nvt, a);
-        else go(few_logit_kernel<T, 4>, s.nvt, a);
+        if (s.few == 1 && !row_weight && s.nvt <= FEW_OWN_TILES) {
+            a.h = c.hidden;
+            go(few_logit_kernel<T, 1, true>, s.nvt, a);
+        } else {
+            go(few_prep_kernel<T>, ((long long)s.Rp * s.Dp + 255) / 256, p);
+            if (s.few == 1) go(few_logit_kernel<T, 1, false>, s.nvt, a);
+            else if (s.few == 2) go(few_logit_kernel<T, 2, false>, s.nvt, a);
+            else go(few_logit_kernel<T, 4, false>, s.nvt, a);
+        }
         if (nll)
             go(xent_rows_kernel<true>, row_weight ? s.Rp : c.R, (const float2*)a.part, (const float*)a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse,
                row_weight ? p.lsec : (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);

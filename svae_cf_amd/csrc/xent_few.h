@@ -21,14 +21,15 @@
 struct FewArgs {
     const void *w, *h, *hg;   // W as it is; copies of H, zeros where a row does not take part: in the loss, in the gradient ([Rp][Dp])
     const void* bias;         // or NULL
-    const int* tgt;           // [Rp], -1: left out
+    int* tgt;                 // [Rp], -1: left out
+    const void* tok;          // the caller's targets, with tok64 and ldh: where H is taken without a copy
     const float *lse, *wrow;  // [Rp], gradient
     float2* part;             // loss: [vocabulary tiles][Rp], or NULL (z only)
     float *zt, *z;            // z: [V][R4] or NULL
     float* slab;              // [chunks * waves along V][R][Dp], or NULL: no dH
     void *dw, *db;            // or NULL
-    long long ldw, ld_dw;     // elements
-    int V, D, Dp, R, R4, Rp, ndt, chunks;
+    long long ldw, ld_dw, ldh;      // elements
+    int tok64, V, D, Dp, R, R4, Rp, ndt, chunks;
 };
 
 // N numbers of any type from any address a number may have (the hardware's vector loads and stores need no more)
@@ -49,6 +50,11 @@ struct FewPrepArgs {
     long long ldh;
     int tok64, R, Rp, V, D, Dp;
 };
+__device__ __forceinline__ int target_at(const void* tok, int tok64, long long r, int V) {
+    const long long t = tok64 ? reinterpret_cast<const long long*>(tok)[r] : (long long)reinterpret_cast<const int*>(tok)[r];
+    return t >= 0 && t < V ? (int)t : -1;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void few_prep_kernel(FewPrepArgs a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / a.Dp;
@@ -57,8 +63,7 @@ __global__ __launch_bounds__(256) void few_prep_kernel(FewPrepArgs a) {
     int tg = -1;
     float w = 0.f;
     if (r < a.R) {
-        const long long t = a.tok64 ? reinterpret_cast<const long long*>(a.tok)[r] : (long long)reinterpret_cast<const int*>(a.tok)[r];
-        if (t >= 0 && t < a.V) tg = (int)t;
+        tg = target_at(a.tok, a.tok64, r, a.V);
         if (tg >= 0 && a.row_weight != nullptr) w = a.row_weight[r];
     }
     if (c == 0) {
@@ -77,8 +82,10 @@ __global__ __launch_bounds__(256) void few_prep_kernel(FewPrepArgs a) {
 
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(256, 2) void few_logit_kernel(FewArgs a) {
+// OWN: H and the targets as the caller has them, without a launch for copies (a left out row, whatever it holds, is a column of
+// its own in every product, and its statistics are not taken)
+template <typename T, int NT, bool OWN>
+__global__ __launch_bounds__(256, NT == 1 ? 4 : 2) void few_logit_kernel(FewArgs a) {
     constexpr int N = 16 / (int)sizeof(T), STEP = 8 * N, MT = 4;       // 128 bytes of a row at a time, in two loads
     typedef Some<T, N> Chunk;
     __shared__ float2 red[4][16 * NT];
@@ -91,18 +98,40 @@ __global__ __launch_bounds__(256, 2) void few_logit_kernel(FewArgs a) {
         const long long v = v0 + 16 * t + i16;                         // (entries behind V: another's row, put out below)
         w[t] = reinterpret_cast<const T*>(a.w) + (v < a.V ? v : a.V - 1) * a.ldw + q * N;
     }
-    const T* h = reinterpret_cast<const T*>(a.h) + lane * N;
+    int target[NT];
+    const T* h[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = 16 * n + i16;
+        target[n] = !OWN ? a.tgt[r] : r < a.R ? target_at(a.tok, a.tok64, r, a.V) : -1;
+        h[n] = reinterpret_cast<const T*>(a.h) + (OWN ? (r < a.R ? r : 0) * a.ldh + q * N : (long long)(n * 2 * 64 + lane) * N);
+        if (OWN && blockIdx.x == 0 && threadIdx.x < 16) a.tgt[r] = target[n];
+    }
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     Chunk x[MT][2], y[NT][2];
+    auto part = [&](const T* row, int k) {                             // a lane's 16 bytes from k on, zeros behind the row's end
+        const int left = a.D - k - q * N;
+        Chunk x;
+        if (left >= N) x = *reinterpret_cast<const Chunk*>(row + k);
+        else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = e < left ? row[k + e] : (T)0.f;
+        }
+        return x;
+    };
     auto load_h = [&](int k, Chunk (&to)[NT][2]) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) to[n][c] = *reinterpret_cast<const Chunk*>(h + ((k / STEP * NT + n) * 2 + c) * (64 * N));
+            for (int c = 0; c < 2; ++c) {
+                if (!OWN) to[n][c] = *reinterpret_cast<const Chunk*>(h[n] + (k / STEP * NT * 2 + c) * (64 * N));
+                else if (k + STEP <= a.D) to[n][c] = *reinterpret_cast<const Chunk*>(h[n] + k + c * 4 * N);
+                else to[n][c] = part(h[n], k + c * 4 * N);
+            }
     };
     auto load_w = [&](int k, Chunk (&to)[MT][2]) {
 #pragma unroll
@@ -149,19 +178,12 @@ __global__ __launch_bounds__(256, 2) void few_logit_kernel(FewArgs a) {
         }
     }
     if (full > 0) multiply();
-    if (full * STEP < a.D) {                                           // the rest of a row; H's copy has zeros there, up to Dp
+    if (full * STEP < a.D) {                                           // the rest of a row; copies of H have zeros there, up to Dp
         load_h(full * STEP, y);
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int k = full * STEP + c * 4 * N, left = a.D - k - q * N;
-                if (left >= N) x[t][c] = *reinterpret_cast<const Chunk*>(w[t] + k);
-                else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) x[t][c][e] = e < left ? w[t][k + e] : (T)0.f;
-                }
-            }
+            for (int c = 0; c < 2; ++c) x[t][c] = part(w[t], full * STEP + c * 4 * N);
         multiply();
     }
 
@@ -202,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void few_logit_kernel(FewArgs a) {
     if (a.part == nullptr) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int rel = a.tgt[16 * n + i16] - ((int)v0 + 4 * q);       // (v0 is below 2^28)
+        const int rel = target[n] - ((int)v0 + 4 * q);       // (v0 is below 2^28)
         if (__any(rel >= 0 && rel < 64)) {
 #pragma unroll
             for (int t = 0; t < MT; ++t)

@@ -102,7 +102,7 @@ def _size(v, what, most=0x7ffffffe):
 def _lookup(table, tokens, scale, out_dtype):
     R, (V, D) = tokens.numel(), table.shape
     tok, (tab, ld) = _flat(tokens), _rows(table)
-    out = torch.empty((R, D), dtype=out_dtype, device=table.device)
+    out = table.new_empty((R, D), dtype=out_dtype)
     if R:
         with _On(table) as st:
             _lib.call("svae_lookup_fwd", tab.data_ptr(), _TYPES[tab.dtype], ld, tok.data_ptr(), _IDS[tok.dtype], out.data_ptr(),
@@ -198,7 +198,7 @@ def _dropout(x, p, seed, step, row_key, out=None):
     C = x.shape[-1]
     x2, ld = _rows(x if x.dim() == 2 else x.reshape(-1, C))
     R = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
     if R:
         dev = isinstance(step, torch.Tensor)
         with _On(x) as st:
