@@ -829,7 +829,9 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     }
     s->parts = type == SV_F32 ? 3 : 1;
     s->direct = grad == LOSS && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
-    s->BN = R <= 64 ? 64 : 128;
+    // 128 rows a tile, but 64 where that leaves less than a workgroup for each CU (loss and gradients in us, 64 | 128 rows: fp32
+    // 184 x 6038 x 1024, 48 tiles of 128 rows, 159 | 240; bf16 300 x 20000 x 512, 237 tiles, 67 | 71; 200 x 50000 x 512, 392, 119 | 112)
+    s->BN = R <= 64 || (R + 127) / 128 * ((V + 255) / 256) < SLOTS / 2 ? 64 : 128;
     s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
     s->Vp = (int)((V + BM - 1) / BM * BM);
     s->Dp = (int)((D + BK - 1) / BK * BK);
