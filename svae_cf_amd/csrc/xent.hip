@@ -771,7 +771,7 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------------
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS_F32 = 64, FEW_ROWS_16 = 32;          // up to here: the kernels for few rows
+constexpr int FEW_ROWS_F32 = 64, FEW_ROWS_16 = 64;          // up to here: the kernels for few rows
 // vocabulary tiles up to which a loss of one tile of rows takes H as it lies: without the launch for the copy, which however is
 // read faster (bf16, one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
 constexpr int FEW_OWN_TILES = 2048;
@@ -811,7 +811,8 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         s->Dp = (int)((D + 63) / 64 * 64);
         s->wd = D <= 64 ? 1 : D <= 128 ? 2 : 4;
         s->ndt = (s->Dp / 64 + s->wd - 1) / s->wd;
-        const int steps = (int)((V + few_step(s->wd) - 1) / few_step(s->wd)), most = (s->few == 1 ? 768 : 512) / s->ndt;      // as many as run at a time: three or two on a CU
+        const int step = type == SV_F32 || s->few == 1 ? few_step(s->wd) : few_step16(s->wd);
+        const int steps = (int)((V + step - 1) / step), most = (s->few == 1 ? 768 : 512) / s->ndt;      // as many as run at a time: three or two on a CU
         s->chunks = most < 1 ? 1 : most < steps ? most : steps;
         s->h = take((long long)s->Rp * s->Dp * sv_elem_size(type));
         s->tgt = take(4ll * s->Rp);
@@ -884,6 +885,9 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     return 0;
 }
 
+// what the largest row weight becomes in G
+inline float top_of(int type) { return type == SV_F16 ? 16384.f : 1.f; }
+
 struct Call {
     const void *hidden, *weight, *bias, *targets;
     long long ld_h, ld_w;
@@ -933,8 +937,6 @@ inline LogitArgs logit_args(const Call& c, const Shape& s) {
     a.V = c.V; a.D = c.D; a.Dp = s.Dp; a.Rp = s.Rp; a.nrt = s.nrt;
     return a;
 }
-
-inline float top_of(int type) { return type == SV_F16 ? 16384.f : 1.f; }
 
 // grad: gradients follow, which read lse and the scale from the workspace
 inline int loss(const Call& c, const Shape& s, float* nll, float* lse, bool grad) {
@@ -1028,8 +1030,13 @@ inline int few(const Call& c, const Shape& s, float* nll, float* lse, const floa
         auto grad = [&](auto wide) {
             constexpr int WD = decltype(wide)::value;
             if (s.few == 1) go(few_grad_kernel<T, 1, WD>, blocks, a);
-            else if (s.few == 2) go(few_grad_kernel<T, 2, WD>, blocks, a);
-            else go(few_grad_kernel<T, 4, WD>, blocks, a);
+            else if constexpr (sizeof(T) == 2) {
+                if (s.few == 2) go(few_grad16_kernel<T, 2, WD>, blocks, a, top_of(c.type));
+                else go(few_grad16_kernel<T, 4, WD>, blocks, a, top_of(c.type));
+            } else {
+                if (s.few == 2) go(few_grad_kernel<T, 2, WD>, blocks, a);
+                else go(few_grad_kernel<T, 4, WD>, blocks, a);
+            }
         };
         if (s.wd == 1) grad(std::integral_constant<int, 1>{});
         else if (s.wd == 2) grad(std::integral_constant<int, 2>{});

@@ -261,6 +261,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : 2) void few_logit_kernel(FewArgs
 
 // WD waves along the columns of W, 64 each; the others share the entries of a step
 constexpr int few_step(int wd) { return wd == 4 ? 32 : 64; }
+constexpr int few_step16(int wd) { return 128 / wd; }
 
 template <typename T, int NT, int WD>
 __global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs a) {
@@ -419,6 +420,181 @@ __global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs a) {
             if (16 * n + i16 < a.R)
                 *reinterpret_cast<f32x4*>(slab + (long long)(16 * n + i16) * a.Dp + d0 + 16 * q + 4 * i) =
                     (f32x4){sum[0][n][i], sum[1][n][i], sum[2][n][i], sum[3][n][i]};
+}
+
+// The same for 16-bit types and more than one tile of rows: G in the inputs' type like the kernels for many rows, whose scale it
+// has, so that products are v_mfma_f32_16x16x32.  A contraction may take its terms in any order that both operands have:
+//   dH  over entries: a lane has four columns of the entries q + 4 g from memory (as they lie); eight of them, g = 0 .. 7, are
+//       its part of A, and G lies in that order in LDS (to_h).
+//   dW  over rows: eight rows 8 q ... of G lie side by side in LDS (to_w), those of H stay in registers.
+template <typename T, int NT, int WD>
+__global__ __launch_bounds__(256, 2) void few_grad16_kernel(FewArgs a, float top) {
+    constexpr int WV = 4 / WD, MINE = 32, STEP = MINE * WV, ROWS = 16 * NT, PITCH = ROWS + 8;
+    constexpr int QUADS = STEP * ROWS / 4 / 256;
+    typedef Some<T, 4> Quad;
+    __shared__ __attribute__((aligned(16))) T to_h[2][WV][ROWS][MINE], to_w[2][STEP][PITCH];
+    __shared__ float wrow[ROWS], lse[ROWS];
+    __shared__ int tgt[ROWS];
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int dt = blockIdx.x % a.ndt, chunk = blockIdx.x / a.ndt;
+    const int d0 = (dt * WD + wave % WD) * 64, part = wave / WD;       // the wave's columns; its entries in a step
+    const int steps = (a.V + STEP - 1) / STEP;
+    const int s0 = (int)((long long)steps * chunk / a.chunks), s1 = (int)((long long)steps * (chunk + 1) / a.chunks);
+    float most = lane < ROWS ? fabsf(a.wrow[lane]) : 0.f;              // (ROWS is at most 64; fmaxf leaves NaN out)
+    most = sv_wave_max(fmaxf(most, 0.f));
+    most = most < INFINITY ? fmaxf(most, 0x1p-100f) : top;
+    const float up = top / most, down = most / top;
+    for (int i = threadIdx.x; i < ROWS; i += 256) {
+        wrow[i] = a.wrow[i] * up;
+        lse[i] = a.lse[i];
+        tgt[i] = a.tgt[i];
+    }
+    for (int i = threadIdx.x; i < 2 * STEP * ROWS; i += 256) (&to_h[0][0][0][0])[i] = (T)0.f;
+    for (int i = threadIdx.x; i < 2 * STEP * PITCH; i += 256) (&to_w[0][0][0])[i] = (T)0.f;
+    __syncthreads();
+
+    const bool on = d0 < a.D;                                          // (else the wave only makes G)
+    auto column = [&](int j, int m) { return d0 + 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3); };
+    Some<T, 8> ah[NT / 2][4];                                          // H for dW: rows 32 k + 8 q ..., column i16 of tile j
+#pragma unroll
+    for (int k = 0; k < NT / 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ah[k][j][e] = on ? reinterpret_cast<const T*>(a.hg)[(32 * k + 8 * q + e) * a.Dp + column(j, i16)] : (T)0.f;
+    f32x4 sum[4][NT];                                                  // dH: columns 4 (4 q + i) + j, row i16 of tile n
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sum[j][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int per = a.R4 / 4, left = on ? a.D - d0 - 4 * i16 : 0;      // quads of an entry; columns of W that the lane has
+    f32x4 z[QUADS];
+    Quad x[8], x2[8];
+    auto load_z = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            const long long at = (long long)s * STEP * per + i;
+            z[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (i < STEP * per && at < (long long)a.V * per) z[k] = reinterpret_cast<const f32x4*>(a.z)[at];
+        }
+    };
+    auto make_g = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            if (i < STEP * per) {
+                const int e = i / per, r = (i - e * per) * 4;
+                const long long v = (long long)s * STEP + e;
+                Some<T, 4> g;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float wr = wrow[r + j];
+                    const float p = __builtin_amdgcn_exp2f((z[k][j] - lse[r + j]) * LOG2E) - (tgt[r + j] == v ? 1.f : 0.f);
+                    g[j] = (T)(wr == 0.f || v >= a.V ? 0.f : p * wr);  // (a row without a part comes to nothing, whatever its z is)
+                    to_h[s & 1][e / MINE][r + j][(e & 3) * 8 + (e % MINE >> 2)] = g[j];
+                }
+                *reinterpret_cast<Some<T, 4>*>(&to_w[s & 1][e][r]) = g;
+            }
+        }
+    };
+    auto load_w = [&](int s, Quad (&to)[8]) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            const long long v = (long long)s * STEP + part * MINE + 4 * g + q;  // (entries behind V: another's row times zero)
+            const T* p = reinterpret_cast<const T*>(a.w) + (v < a.V ? v : a.V - 1) * a.ldw + d0 + 4 * i16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[g][e] = (T)0.f;
+            if (left >= 4) to[g] = *reinterpret_cast<const Quad*>(p);
+            else if (left > 0) {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (e < left) to[g][e] = p[e];
+            }
+        }
+    };
+    if (s0 < s1) {
+        load_z(s0);
+        if (a.slab != nullptr) load_w(s0, x);
+        make_g(s0);
+    }
+    __syncthreads();
+    for (int s = s0; s < s1; ++s) {
+        const int b = s & 1;
+        const bool more = s + 1 < s1;
+        if (more) {
+            load_z(s + 1);
+            if (a.slab != nullptr) load_w(s + 1, x2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (a.slab != nullptr && on) {
+            s16x8 g[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) g[n] = *reinterpret_cast<const s16x8*>(&to_h[b][part][16 * n + i16][8 * q]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                Some<T, 8> w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = x[e][j];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sum[j][n] = mfma<T>(__builtin_bit_cast(s16x8, w), g[n], sum[j][n]);
+            }
+        }
+        if (a.dw != nullptr && on) {
+#pragma unroll
+            for (int t = 0; t < MINE / 16; ++t) {
+                f32x4 c[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NT / 2; ++k) {
+                    const s16x8 g = *reinterpret_cast<const s16x8*>(&to_w[b][part * MINE + 16 * t + i16][32 * k + 8 * q]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = mfma<T>(__builtin_bit_cast(s16x8, ah[k][j]), g, c[j]);
+                }
+                const long long v = (long long)s * STEP + part * MINE + 16 * t + i16;
+                if (v < a.V) {
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        const int d = column(j, 4 * q);
+                        T* o = reinterpret_cast<T*>(a.dw) + v * a.ld_dw + d;
+                        Some<T, 8> out;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) out[e] = (T)(c[j + e / 4][e % 4] * down);
+                        if (d + 7 < a.D) *reinterpret_cast<Some<T, 8>*>(o) = out;
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 7; ++e)
+                                if (d + e < a.D) o[e] = out[e];
+                        }
+                    }
+                }
+            }
+        }
+        if (a.db != nullptr && dt == 0 && (int)threadIdx.x < STEP) {
+            const long long v = (long long)s * STEP + threadIdx.x;
+            float sum_g = 0.f;
+            for (int r = 0; r < a.R; ++r) sum_g += (float)to_w[b][threadIdx.x][r];
+            if (v < a.V) reinterpret_cast<T*>(a.db)[v] = (T)(sum_g * down);
+        }
+        if (more) {
+            make_g(s + 1);                                             // (read by every wave before the last barrier)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = x2[k];
+        }
+        __syncthreads();
+    }
+    if (a.slab == nullptr || !on) return;
+    float* slab = a.slab + (long long)(chunk * WV + part) * a.R * a.Dp;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (16 * n + i16 < a.R)
+                *reinterpret_cast<f32x4*>(slab + (long long)(16 * n + i16) * a.Dp + d0 + 16 * q + 4 * i) =
+                    (f32x4){sum[0][n][i], sum[1][n][i], sum[2][n][i], sum[3][n][i]} * down;
 }
 
 // dH: sum of the slabs in a fixed order; a workgroup has 8 quads of columns, 32 threads share the slabs of each
