@@ -771,7 +771,7 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------------
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS_F32 = 64, FEW_ROWS_16 = 64;          // up to here: the kernels for few rows
+constexpr int FEW_ROWS = 64;                               // up to here: the kernels for few rows (both sides measured there)
 // vocabulary tiles up to which a loss of one tile of rows takes H as it lies: without the launch for the copy, which however is
 // read faster (bf16, one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
 constexpr int FEW_OWN_TILES = 2048;
@@ -803,7 +803,7 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         at += (bytes + 1023) / 1024 * 1024;
         return p;
     };
-    if (R <= (type == SV_F32 ? FEW_ROWS_F32 : FEW_ROWS_16)) {
+    if (R <= FEW_ROWS) {
         s->few = R <= 16 ? 1 : R <= 32 ? 2 : 4;
         s->Rp = 16 * s->few;
         s->R4 = (int)(R + 3) / 4 * 4;
@@ -832,7 +832,7 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->direct = grad == LOSS && type != SV_F32 && R <= DIRECT_ROWS && D % 8 == 0 && ld_w % 8 == 0 && (unsigned long long)weight % 16 == 0;
     // 128 rows a tile, but 64 where that leaves less than a workgroup for each CU (loss and gradients in us, 64 | 128 rows: fp32
     // 184 x 6038 x 1024, 48 tiles of 128 rows, 159 | 240; bf16 300 x 20000 x 512, 237 tiles, 67 | 71; 200 x 50000 x 512, 392, 119 | 112)
-    s->BN = R <= 64 || (R + 127) / 128 * ((V + 255) / 256) < SLOTS / 2 ? 64 : 128;
+    s->BN = (R + 127) / 128 * ((V + 255) / 256) < SLOTS / 2 ? 64 : 128;
     s->Rp = (int)((R + s->BN - 1) / s->BN * s->BN);
     s->Vp = (int)((V + BM - 1) / BM * BM);
     s->Dp = (int)((D + BK - 1) / BK * BK);

@@ -7,15 +7,17 @@
 //              for dH, whose sums stay in registers, and write dW.  Workgroups share the vocabulary and leave slabs of dH that are
 //              added in order.
 //
-// fp32 products are fp32 (v_mfma_f32_16x16x4), G and the gradients' products are for all types: nothing is rounded in between.
-// At NT tiles of 16 rows the products take 28 NT us for the loss (fp32; little for 16 bits) and 55 NT us for the gradients where
-// W has 131072 x 1024 numbers; reading W once takes 53 us (16 bits) or 106 us (fp32), writing its gradient as long.
+// fp32 products are fp32 (v_mfma_f32_16x16x4); for one tile of 16 rows G and the gradients' products are fp32 for all types.  More
+// rows of 16 bits: 16-bit products, G rounded as by the kernels for many rows.
+// At NT tiles of 16 rows fp32 products take 28 NT us for the loss and 55 NT us for the gradients where W has 131072 x 1024 numbers;
+// reading W once takes 53 us (16 bits) or 106 us (fp32), writing its gradient as long.
 //
 // Measured there, loss | loss and gradients (us), against the kernels for many rows:
-//   fp32   1 row 135 | 358    (566 | 1285)     32 rows 144 | 411    (555 | 1320)     64 rows 235 | 754    (554 | 1333)
-//   bf16   1 row  50 | 206    ( 53 |  400)     32 rows  50 | 290    ( 52 |  397)     64 rows  53 | 433    ( 53 |  401)
-// so that they take up to 64 rows of fp32 and up to 32 of 16 bits.  (Loss and gradients have to take the same ones: z has to have
-// the same bits in both, or errors of z and of lse do not cancel in the gradient of a confident row.)
+//   fp32   1 row 133 | 358    (566 | 1285)     32 rows 144 | 411    (555 | 1320)     64 rows 235 | 754    (554 | 1333)
+//   bf16   1 row  48 | 206    ( 53 |  400)     32 rows  50 | 208    ( 52 |  397)     64 rows  55 | 239    ( 53 |  401)
+// The loss of 64 rows of 16 bits is the one that loses (a million x 256: 138 | 490 against 113 | 1065): loss and gradients have to
+// take the same kernels, as z has to have the same bits in both, or errors of z and of lse do not cancel in the gradient of a
+// confident row.
 #pragma once
 
 struct FewArgs {
