@@ -6,6 +6,10 @@
 // Both are bound by HBM: the lookup reads a table row and writes an output row per token, the gradient reads every dy row
 // once and writes every table row once (rows without a token as zeros).  The gradient uses no atomics on sums: a stable radix
 // sort brings the rows of one token together in their order, so results are the same in every run.
+//
+// Measured: lookup of 131072 x 1024 bf16 92 us (268 MB written, as much read, popular rows from the caches); its gradient 131 us
+// (4.1 TB/s of rows in random order and gradient), with 11603 tokens against 1000000 x 256 fp32 186 us (1.02 GB, nearly all
+// zeros, 5.5 TB/s); the sort 20 us for 21800 tokens (latency of four launches), 33 us for 131072.
 #include "elem.h"
 
 namespace {

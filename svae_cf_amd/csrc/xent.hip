@@ -7,6 +7,9 @@
 // the target's logit.  Gradient: for one piece of the vocabulary after the other, the tiles of z are made again and G of the
 // piece is written to the workspace, then two products take it up.  Everything is bound by the matrix units (6 R V D flops for
 // loss and gradient and 2 R V D for making z again), except that few rows leave the loss bound by reading W.
+// Loss and gradients, bf16: 8192 x 131072 x 1024 7.0 ms (8.8e12 operations, 1.26e15 a second; a library's products of these
+// shapes alone 1.10 .. 1.24e15), 21800 x 20000 x 200 1.0 ms; fp32 2049 x 17770 x 150 0.34 ms.  Loss alone, fp16: 256 x 1000000 x 256
+// 0.2 ms.
 //
 // All products run on one core: 256 x BN outputs a workgroup, steps of 32 along the contraction, three stages of LDS filled by
 // LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from writes to the other and
