@@ -775,8 +775,8 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS = 64;                               // up to here: the kernels for few rows (both sides measured there)
-// vocabulary tiles up to which a loss of one tile of rows takes H as it lies: without the launch for the copy, which however is
-// read faster (bf16, one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
+// vocabulary tiles up to which logits of one tile of rows take H as it lies: without the launch for the copy, which however is
+// read faster (bf16, loss of one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
 constexpr int FEW_OWN_TILES = 2048;
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
 constexpr long long PIECE_LEAST = 128ll << 20, PIECE_MOST = 512ll << 20;     // what G of a piece may take; there are two
@@ -819,12 +819,9 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         s->chunks = most < 1 ? 1 : most < steps ? most : steps;
         s->h = take((long long)s->Rp * s->Dp * sv_elem_size(type));
         s->tgt = take(4ll * s->Rp);
-        s->lse = take(4ll * s->Rp);
         s->zt = take(4ll * s->Rp);
         s->part = take(8ll * s->nvt * s->Rp);
         if (grad != LOSS) {
-            s->hg = take((long long)s->Rp * s->Dp * sv_elem_size(type));
-            s->wrow = take(4ll * s->Rp);
             s->z = take(4ll * V * s->R4);
             s->h_slab = take(4ll * s->chunks * (4 / s->wd) * R * s->Dp);
         }
@@ -990,19 +987,16 @@ inline void piece(const Call& c, const Shape& s, const PieceArgs& a, unsigned bl
     });
 }
 
-// the kernels for few rows: loss (nll and lse given), gradients (row_weight and dh or dw given; lse: fwd's, where no loss is wanted)
+// the kernels for few rows: loss (nll and lse are written), gradients (row_weight; dh or dw is written; given: fwd's lse, where no
+// loss is wanted)
 inline int few(const Call& c, const Shape& s, float* nll, float* lse, const float* given, const float* row_weight, void* dh, long long ld_dh,
                void* dw, long long ld_dw, void* db) {
-    FewPrepArgs p;
-    p.h = c.hidden; p.tok = c.targets; p.row_weight = row_weight; p.lse = given;
-    p.hc = c.work + s.h; p.hg = row_weight ? c.work + s.hg : nullptr;
-    p.wrow = (float*)(c.work + s.wrow); p.lsec = (float*)(c.work + s.lse); p.tgt = (int*)(c.work + s.tgt);
-    p.ldh = c.ld_h; p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.D = c.D; p.Dp = s.Dp;
     FewArgs a{};
-    a.w = c.weight; a.h = p.hc; a.hg = p.hg; a.bias = c.bias; a.tgt = p.tgt; a.lse = p.lsec; a.wrow = p.wrow;
+    a.w = c.weight; a.hidden = a.h = c.hidden; a.bias = c.bias; a.tok = c.targets; a.tgt = (int*)(c.work + s.tgt);
+    a.lse = given ? given : lse; a.row_weight = row_weight;
     a.part = nll ? (float2*)(c.work + s.part) : nullptr; a.zt = (float*)(c.work + s.zt);
     a.z = row_weight ? (float*)(c.work + s.z) : nullptr; a.slab = dh ? (float*)(c.work + s.h_slab) : nullptr;
-    a.dw = dw; a.db = db; a.ldw = c.ld_w; a.ld_dw = ld_dw; a.ldh = c.ld_h; a.tok = c.targets; a.tok64 = c.tok64;
+    a.dw = dw; a.db = db; a.ldw = c.ld_w; a.ld_dw = ld_dw; a.ldh = c.ld_h; a.tok64 = c.tok64;
     a.V = c.V; a.D = c.D; a.Dp = s.Dp; a.R = c.R; a.R4 = s.R4; a.Rp = s.Rp; a.ndt = s.ndt; a.chunks = s.chunks;
     int rc = 0;
     sv_by_type(c.type, [&](auto type) {
@@ -1016,18 +1010,20 @@ inline int few(const Call& c, const Shape& s, float* nll, float* lse, const floa
                 }();
             }
         };
-        if (s.few == 1 && !row_weight && s.nvt <= FEW_OWN_TILES) {
-            a.h = c.hidden;
-            go(few_logit_kernel<T, 1, true>, s.nvt, a);
-        } else {
+        if (s.few == 1 && s.nvt <= FEW_OWN_TILES) go(few_logit_kernel<T, 1, true>, s.nvt, a);
+        else {
+            FewPrepArgs p;
+            p.h = c.hidden; p.tok = c.targets; p.hc = c.work + s.h; p.tgt = a.tgt;
+            p.ldh = c.ld_h; p.tok64 = c.tok64; p.R = c.R; p.Rp = s.Rp; p.V = c.V; p.D = c.D; p.Dp = s.Dp;
             go(few_prep_kernel<T>, ((long long)s.Rp * s.Dp + 255) / 256, p);
+            a.h = p.hc;
             if (s.few == 1) go(few_logit_kernel<T, 1, false>, s.nvt, a);
             else if (s.few == 2) go(few_logit_kernel<T, 2, false>, s.nvt, a);
             else go(few_logit_kernel<T, 4, false>, s.nvt, a);
         }
         if (nll)
-            go(xent_rows_kernel<true>, row_weight ? s.Rp : c.R, (const float2*)a.part, (const float*)a.zt, a.tgt, c.R, s.Rp, s.nvt, nll, lse,
-               row_weight ? p.lsec : (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);
+            go(xent_rows_kernel<true>, c.R, (const float2*)a.part, (const float*)a.zt, (const int*)a.tgt, c.R, s.Rp, s.nvt, nll, lse,
+               (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);
         if (!dh && !dw) return;
         const long long blocks = (long long)s.chunks * s.ndt;
         auto grad = [&](auto wide) {

@@ -21,11 +21,12 @@
 #pragma once
 
 struct FewArgs {
-    const void *w, *h, *hg;   // W as it is; copies of H, zeros where a row does not take part: in the loss, in the gradient ([Rp][Dp])
+    const void *w, *h;        // W as it is; H as it is or its copy (few_logit_kernel)
+    const void* hidden;       // H as it is, with ldh
     const void* bias;         // or NULL
     int* tgt;                 // [Rp], -1: left out
-    const void* tok;          // the caller's targets, with tok64 and ldh: where H is taken without a copy
-    const float *lse, *wrow;  // [Rp], gradient
+    const void* tok;          // the caller's targets, with tok64
+    const float *lse, *row_weight;        // gradient: the caller's, [R]
     float2* part;             // loss: [vocabulary tiles][Rp], or NULL (z only)
     float *zt, *z;            // z: [V][R4] or NULL
     float* slab;              // [chunks * waves along V][R][Dp], or NULL: no dH
@@ -42,12 +43,10 @@ struct SomeOf {
 template <typename T, int N>
 using Some = typename SomeOf<T, N>::type;
 
-// copies of H, targets, weights and lse of the rows
+// the loss's copy of H and the rows' targets
 struct FewPrepArgs {
     const void *h, *tok;
-    const float *row_weight, *lse;        // NULL: loss only
-    void *hc, *hg;                        // NULL: not wanted
-    float *wrow, *lsec;
+    void* hc;
     int* tgt;
     long long ldh;
     int tok64, R, Rp, V, D, Dp;
@@ -62,24 +61,31 @@ __global__ __launch_bounds__(256) void few_prep_kernel(FewPrepArgs a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / a.Dp;
     const int c = (int)(i - r * a.Dp);
     if (r >= a.Rp) return;
-    int tg = -1;
-    float w = 0.f;
-    if (r < a.R) {
-        tg = target_at(a.tok, a.tok64, r, a.V);
-        if (tg >= 0 && a.row_weight != nullptr) w = a.row_weight[r];
-    }
-    if (c == 0) {
-        a.tgt[r] = tg;
-        if (a.row_weight != nullptr) a.wrow[r] = w;
-        if (a.lse != nullptr) a.lsec[r] = r < a.R ? a.lse[r] : 0.f;
-    }
-    const T x = tg >= 0 && c < a.D ? reinterpret_cast<const T*>(a.h)[r * a.ldh + c] : (T)0.f;
-    // the loss's copy in the order in which the matrix units take it: 1 KiB for 16 rows and four times 16 bytes of them (rows a
-    // power of two apart fall on few channels of the cache: 64 rows of 256 fp32 took 457 us instead of 381 against a million)
+    const int tg = r < a.R ? target_at(a.tok, a.tok64, r, a.V) : -1;
+    if (c == 0) a.tgt[r] = tg;
+    // in the order in which the matrix units take it, zeros for a left out row: 1 KiB for 16 rows and four times 16 bytes of them (rows
+    // a power of two apart fall on few channels of the cache: 64 rows of 256 fp32 took 457 us instead of 381 against a million)
     constexpr int N = 16 / (int)sizeof(T);
     const long long at = ((((long long)(c / (4 * N) / 2) * (a.Rp / 16) + r / 16) * 2 + c / (4 * N) % 2) * 64 + c / N % 4 * 16 + r % 16) * N + c % N;
-    if (a.hc != nullptr) reinterpret_cast<T*>(a.hc)[at] = x;
-    if (a.hg != nullptr) reinterpret_cast<T*>(a.hg)[i] = w != 0.f ? x : (T)0.f;
+    reinterpret_cast<T*>(a.hc)[at] = tg >= 0 && c < a.D ? reinterpret_cast<const T*>(a.h)[r * a.ldh + c] : (T)0.f;
+}
+
+// weight (0: no part in the gradient), lse and target of the rows, in LDS; ends behind a barrier
+template <int ROWS>
+__device__ __forceinline__ void few_rows(const FewArgs& a, float* wrow, float* lse, int* tgt) {
+    if ((int)threadIdx.x < ROWS) {
+        const int r = threadIdx.x;
+        const int t = r < a.R ? target_at(a.tok, a.tok64, r, a.V) : -1;
+        wrow[r] = t >= 0 ? a.row_weight[r] : 0.f;
+        lse[r] = t >= 0 ? a.lse[r] : 0.f;
+        tgt[r] = t;
+    }
+    __syncthreads();
+}
+// H for dW: zeros behind a row's end and for rows without a part
+template <typename T>
+__device__ __forceinline__ T few_hidden(const FewArgs& a, const float* wrow, int r, int d) {
+    return d < a.D && wrow[r] != 0.f ? reinterpret_cast<const T*>(a.hidden)[r * a.ldh + d] : (T)0.f;
 }
 
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -279,13 +285,8 @@ __global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs a) {
     const int d0 = (dt * WD + wave % WD) * 64, first = wave / WD * MINE;        // the wave's columns; its first entry in a step
     const int steps = (a.V + STEP - 1) / STEP;
     const int s0 = (int)((long long)steps * chunk / a.chunks), s1 = (int)((long long)steps * (chunk + 1) / a.chunks);
-    for (int i = threadIdx.x; i < ROWS; i += 256) {
-        wrow[i] = a.wrow[i];
-        lse[i] = a.lse[i];
-        tgt[i] = a.tgt[i];
-    }
     for (int i = threadIdx.x; i < 2 * STEP * PITCH; i += 256) (&gs[0][0][0])[i] = 0.f;
-    __syncthreads();
+    few_rows<ROWS>(a, wrow, lse, tgt);
 
     const bool on = d0 < a.D;                                          // (else the wave only makes G)
     // column of dW's tile j: a lane's entries 4 q ... 4 q + 3 of two tiles are eight columns in a row
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs a) {
 #pragma unroll
     for (int k = 0; k < 4 * NT; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ah[k][j] = on ? (float)reinterpret_cast<const T*>(a.hg)[(4 * k + q) * a.Dp + column(j, i16)] : 0.f;
+        for (int j = 0; j < 4; ++j) ah[k][j] = (float)few_hidden<T>(a, wrow, 4 * k + q, column(j, i16));
     f32x4 sum[4][NT];                                                  // dH: columns 4 (4 q + i) + j, row i16 of tile n
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -443,18 +444,12 @@ __global__ __launch_bounds__(256, 2) void few_grad16_kernel(FewArgs a, float top
     const int d0 = (dt * WD + wave % WD) * 64, part = wave / WD;       // the wave's columns; its entries in a step
     const int steps = (a.V + STEP - 1) / STEP;
     const int s0 = (int)((long long)steps * chunk / a.chunks), s1 = (int)((long long)steps * (chunk + 1) / a.chunks);
-    float most = lane < ROWS ? fabsf(a.wrow[lane]) : 0.f;              // (ROWS is at most 64; fmaxf leaves NaN out)
-    most = sv_wave_max(fmaxf(most, 0.f));
-    most = most < INFINITY ? fmaxf(most, 0x1p-100f) : top;
-    const float up = top / most, down = most / top;
-    for (int i = threadIdx.x; i < ROWS; i += 256) {
-        wrow[i] = a.wrow[i] * up;
-        lse[i] = a.lse[i];
-        tgt[i] = a.tgt[i];
-    }
     for (int i = threadIdx.x; i < 2 * STEP * ROWS; i += 256) (&to_h[0][0][0][0])[i] = (T)0.f;
     for (int i = threadIdx.x; i < 2 * STEP * PITCH; i += 256) (&to_w[0][0][0])[i] = (T)0.f;
-    __syncthreads();
+    few_rows<ROWS>(a, wrow, lse, tgt);
+    float most = sv_wave_max(fmaxf(lane < ROWS ? fabsf(wrow[lane]) : 0.f, 0.f));        // (ROWS is at most 64; fmaxf leaves NaN out)
+    most = most < INFINITY ? fmaxf(most, 0x1p-100f) : top;
+    const float up = top / most, down = most / top;
 
     const bool on = d0 < a.D;                                          // (else the wave only makes G)
     auto column = [&](int j, int m) { return d0 + 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3); };
@@ -464,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void few_grad16_kernel(FewArgs a, float top
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ah[k][j][e] = on ? reinterpret_cast<const T*>(a.hg)[(32 * k + 8 * q + e) * a.Dp + column(j, i16)] : (T)0.f;
+            for (int e = 0; e < 8; ++e) ah[k][j][e] = few_hidden<T>(a, wrow, 32 * k + 8 * q + e, column(j, i16));
     f32x4 sum[4][NT];                                                  // dH: columns 4 (4 q + i) + j, row i16 of tile n
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -495,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void few_grad16_kernel(FewArgs a, float top
                 for (int j = 0; j < 4; ++j) {
                     const float wr = wrow[r + j];
                     const float p = __builtin_amdgcn_exp2f((z[k][j] - lse[r + j]) * LOG2E) - (tgt[r + j] == v ? 1.f : 0.f);
-                    g[j] = (T)(wr == 0.f || v >= a.V ? 0.f : p * wr);  // (a row without a part comes to nothing, whatever its z is)
+                    g[j] = (T)(wr == 0.f || v >= a.V ? 0.f : p * (wr * up));     // (a row without a part comes to nothing, whatever its z is)
                     to_h[s & 1][e / MINE][r + j][(e & 3) * 8 + (e % MINE >> 2)] = g[j];
                 }
                 *reinterpret_cast<Some<T, 4>*>(&to_w[s & 1][e][r]) = g;
