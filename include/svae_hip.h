@@ -430,7 +430,7 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
  * z = hidden weight^T + bias, [R][V], never kept.  hidden [R][D], weight [V][D] (rows ld elements apart), bias [V] or NULL, all
  * of one type (0 fp32, 1 bf16, 2 fp16); targets [R] int32, or int64 with tok64 != 0.  A row whose target is outside [0, V) is
  * left out: nll = lse = 0, no gradient, whatever the row holds.  Products of bf16 / fp16 run on the matrix units as they are,
- * fp32 ones as six products of bf16 parts (24 bits) or, up to 64 rows, in fp32; sums, statistics and losses are fp32.  In the
+ * fp32 ones as six products of bf16 parts (24 bits) or, for few rows, in fp32; sums, statistics and losses are fp32.  In the
  * gradient w (softmax - onehot) is rounded to a 16-bit type after a scale by the largest row weight (16 rows or fewer: not at all).
  *   svae_xent_fwd     lse[r] = log sum_v exp z[r][v], nll[r] = lse[r] - z[r][target] (fp32)
  *   svae_xent_reduce  out[0] = the sum of nll or (mean != 0) its mean over the rows with a target (0 over none), out[1] = the
@@ -440,10 +440,10 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
  *                     takes no part, whatever it holds.
  *   svae_xent_fwd_bwd both in one call, for programs that know the rows' weights beforehand (copies of the inputs are made once)
  * Workspace, aligned to 256 bytes: svae_xent_bytes(address of weight modulo 16, ld_w, type, R, V, D, grad, &bytes), grad != 0 for
- * the gradients.  Up to 64 rows read weight as it lies; their gradients have 4 bytes for each of the R x V logits in the workspace.
- * The loss of up to 512 rows of a 16-bit type takes weight as it lies too if its address and rows are multiples of 16 bytes.  Else the workspace
- * holds a copy of weight (16-bit types: of its size, fp32: one and a half times that), and gradients have two pieces of up to
- * 512 MiB, or of 256 columns if those are larger, in it. */
+ * the gradients.  Up to 32 rows (64 of fp32, or against a weight of 2^23 numbers) read weight as it lies; their gradients have 4
+ * bytes for each of the R x V logits in the workspace.  The loss of up to 512 rows of a 16-bit type takes weight as it lies too if
+ * its address and rows are multiples of 16 bytes.  Else the workspace holds a copy of weight (16-bit types: of its size, fp32: one
+ * and a half times that), and gradients have two pieces of up to 512 MiB, or of 256 columns if those are larger, in it. */
 int svae_xent_bytes(int weight_align, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes);
 int svae_xent_fwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                   const void* targets, int tok64, int type, int R, int V, int D, float* nll, float* lse, void* work,

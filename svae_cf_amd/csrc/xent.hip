@@ -774,7 +774,11 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------------
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
-constexpr int FEW_ROWS = 64;                               // up to here: the kernels for few rows (both sides measured there)
+// Up to here: the kernels for few rows.  More than 32 rows of 16 bits only for a W of 2^23 numbers or more, whose copy costs more than
+// those kernels' slower start (64 rows, loss and gradients in us, few | many: 5000 x 64 41 | 35, 32768 x 256 55 | 51, 32768 x 1024
+// 93 | 99, 65536 x 256 64 | 90; fp32 39 | 41, 83 | 114, 221 | 344, 113 | 285).
+constexpr int FEW_ROWS = 64, FEW_ROWS_16 = 32;
+constexpr long long FEW_WEIGHT_16 = 1ll << 23;
 // vocabulary tiles up to which logits of one tile of rows take H as it lies: without the launch for the copy, which however is
 // read faster (bf16, loss of one row: 5000 x 64 17 us | 20 with a copy, 411353 x 96 (1607 tiles) 27 | 28, 1000000 x 256 (3907) 114 | 105)
 constexpr int FEW_OWN_TILES = 2048;
@@ -806,7 +810,7 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         at += (bytes + 1023) / 1024 * 1024;
         return p;
     };
-    if (R <= FEW_ROWS) {
+    if (R <= FEW_ROWS_16 || (R <= FEW_ROWS && (type == SV_F32 || V * D >= FEW_WEIGHT_16))) {
         s->few = R <= 16 ? 1 : R <= 32 ? 2 : 4;
         s->Rp = 16 * s->few;
         s->R4 = (int)(R + 3) / 4 * 4;

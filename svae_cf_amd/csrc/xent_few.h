@@ -14,10 +14,10 @@
 //
 // Measured there, loss | loss and gradients (us), against the kernels for many rows:
 //   fp32   1 row 133 | 358    (566 | 1285)     32 rows 144 | 411    (555 | 1320)     64 rows 235 | 754    (554 | 1333)
-//   bf16   1 row  48 | 206    ( 53 |  400)     32 rows  50 | 208    ( 52 |  397)     64 rows  55 | 239    ( 53 |  401)
-// The loss of 64 rows of 16 bits is the one that loses (a million x 256: 138 | 490 against 113 | 1065): loss and gradients have to
-// take the same kernels, as z has to have the same bits in both, or errors of z and of lse do not cancel in the gradient of a
-// confident row.
+//   bf16   1 row  48 | 203    ( 53 |  400)     32 rows  50 | 208    ( 52 |  397)     64 rows  55 | 239    ( 53 |  401)
+// xent.hip has the limits.  The loss of 64 rows of 16 bits is the one that loses (a million x 256: 138 | 490 against 113 | 1065): loss
+// and gradients have to take the same kernels, as z has to have the same bits in both, or errors of z and of lse do not cancel in
+// the gradient of a confident row.
 #pragma once
 
 struct FewArgs {

@@ -115,7 +115,7 @@ def test_loss_and_gradients(R, V, D, dtype):
     check(*make(R, V, D, dtype, bias=(R + V) % 2 == 1))
 
 
-FEW = [(5, 70000, 3), (9, 90001, 8), (16, 1000, 300), (17, 40000, 65), (31, 31, 128), (32, 4097, 129), (33, 2000, 96), (50, 20000, 260), (64, 33, 4), (64, 70001, 64)]
+FEW = [(5, 70000, 3), (9, 90001, 8), (16, 1000, 300), (17, 40000, 65), (31, 31, 128), (32, 4097, 129), (33, 2000, 96), (50, 20000, 260), (64, 33, 4), (64, 70001, 64), (41, 33000, 260), (64, 140001, 61)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
