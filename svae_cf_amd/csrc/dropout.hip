@@ -14,8 +14,9 @@
 
 namespace {
 
-// a thread makes one group of 8 columns; division by the groups of a row through a precomputed reciprocal
-template <int VEC, typename T>
+// a thread makes one group of 8 columns, the last one of an odd width in vectors of TAIL (which divides the width); division by the
+// groups of a row through a precomputed reciprocal
+template <int TAIL, typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, long long ldx, T* y, long long ldy, long long row0,
                                                       unsigned n, int C, unsigned ng, unsigned long long magic, unsigned below,
                                                       float up, unsigned long long seed, unsigned step,
@@ -31,19 +32,25 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, long long ldx,
     const T* src = x + row * ldx + (long long)g * 8;
     T* dst = y + row * ldy + (long long)g * 8;
     const int left = C - (int)g * 8;
-    float v[8];
+    float v[8] = {};
+    if (TAIL == 8 || left >= 8) sv_load<8>(src, v);
+    else {
 #pragma unroll
-    for (int j = 0; j < 8; j += VEC)
-        if (VEC == 8 || j < left) sv_load<VEC>(src + j, v + j);
+        for (int j = 0; j < 8; j += TAIL)
+            if (j < left) sv_load<TAIL>(src + j, v + j);
+    }
     philox4x32_10(c, (uint32_t)seed, (uint32_t)(seed >> 32));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const unsigned u = (j & 1) ? c[j >> 1] >> 16 : c[j >> 1] & 0xFFFFu;
         v[j] = u >= below ? v[j] * up : 0.f;
     }
+    if (TAIL == 8 || left >= 8) sv_store<8>(dst, v);
+    else {
 #pragma unroll
-    for (int j = 0; j < 8; j += VEC)
-        if (VEC == 8 || j < left) sv_store<VEC>(dst + j, v + j);
+        for (int j = 0; j < 8; j += TAIL)
+            if (j < left) sv_store<TAIL>(dst + j, v + j);
+    }
 }
 
 }  // namespace
@@ -59,7 +66,7 @@ extern "C" int svae_dropout(const void* x, long long ldx, void* y, long long ldy
     if (R == 0) return 0;
     SV_CHECK_ARG(x && y, "svae_dropout: null pointer");
     const float up = below == 65536u ? 0.f : (float)(65536.0 / (65536.0 - below));
-    const int vec = sv_vec_for(8, C, x, ldx, sv_elem_size(type), y, ldy, sv_elem_size(type));
+    const int tail = sv_vec_for(8, C, true);
     const unsigned ng = (unsigned)((C + 7) / 8);
     // i / ng = high word of i * ceil(2^64 / ng), exact for i and ng below 2^32 (ng = 1, whose reciprocal does not fit, apart)
     const unsigned long long magic = ng == 1 ? 0 : ~0ull / ng + 1;
@@ -73,9 +80,9 @@ extern "C" int svae_dropout(const void* x, long long ldx, void* y, long long ldy
                 hipLaunchKernelGGL(kernel, dim3((n + 255u) / 256u), dim3(256), 0, (hipStream_t)stream, (const T*)x, ldx, (T*)y, ldy, r0, n, C,
                                    ng, magic, below, up, seed, step, step_dev, row_key);
             };
-            if (vec == 8) go(dropout_kernel<8, T>);
-            else if (vec == 4) go(dropout_kernel<4, T>);
-            else if (vec == 2) go(dropout_kernel<2, T>);
+            if (tail == 8) go(dropout_kernel<8, T>);
+            else if (tail == 4) go(dropout_kernel<4, T>);
+            else if (tail == 2) go(dropout_kernel<2, T>);
             else go(dropout_kernel<1, T>);
         });
         SV_LAUNCH_CHECK();

@@ -31,7 +31,8 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const T* __restrict__ t
     const bool here = t >= 0 && t < V;
     const T* src = table + (here ? t : 0) * ldt;
     O* dst = out + row * ldo;
-    for (int c = lane * VEC; c < D; c += VEC << lg) {
+    for (int c0 = lane * VEC; c0 < D; c0 += VEC << lg) {
+        const int c = c0 < D - VEC ? c0 : D - VEC;               // (the last vector of an odd width: some columns twice)
         float v[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = 0.f;
@@ -319,7 +320,8 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
     __shared__ float red[4][64 * VEC];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = ((int)blockIdx.y * 64 + lane) * VEC;       // the launch's second dimension goes over slices of the columns
+    // the launch's second dimension goes over slices of the columns; the last vector of an odd width takes some columns twice
+    const int c0 = ((int)blockIdx.y * 64 + lane) * VEC, c = c0 < D && c0 > D - VEC ? D - VEC : c0;
     const int block = (int)(blockIdx.z * gridDim.x + blockIdx.x);
     if (block < nchunk) {
         const int p0 = block * CHUNK, p1 = R - p0 < CHUNK ? R : p0 + CHUNK;
@@ -402,7 +404,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
     const int e = segment_end(keys, p0 + CHUNK, R, k, lane);
     const int last = (e - 1) / CHUNK;
     const int slot0 = s == p0 ? 0 : 1;                       // in chunk p; the following ones have it at their first place
-    const int c = ((int)blockIdx.y * 64 + lane) * VEC;
+    const int c0 = ((int)blockIdx.y * 64 + lane) * VEC, c = c0 < D && c0 > D - VEC ? D - VEC : c0;
     float acc[VEC];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
@@ -433,7 +435,7 @@ extern "C" int svae_lookup_fwd(const void* table, int table_type, long long ld_t
     SV_CHECK_ARG(table_type >= 0 && table_type <= 2 && out_type >= 0 && out_type <= 2, "svae_lookup_fwd: types %d, %d", table_type, out_type);
     if (R == 0) return 0;
     SV_CHECK_ARG(table && tokens && out, "svae_lookup_fwd: null pointer");
-    const int vec = sv_vec_for(8, D, table, ld_table, sv_elem_size(table_type), out, ld_out, sv_elem_size(out_type));
+    const int vec = sv_vec_for(8, D, false);
     int lg = 0;
     while (lg < 8 && (vec << lg) < D) ++lg;
     const long long most = 1ll << (31 - lg);                        // rows of a launch: its threads are counted in 32 bits
@@ -531,7 +533,7 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
     // rows of 256, 21800 tokens: 16 rows 16.6 us, 4 rows 12.7 us)
     const int group = V >= 8192 * MOST_GROUP ? MOST_GROUP : V >= 8192 * 8 ? 8 : 4;
     const long long nrow = ((long long)V + 4 * group - 1) / (4 * group);
-    int vec = sv_vec_for(8, D, R ? dy : grad, R ? ld_dy : ld_grad, sv_elem_size(dy_type), grad, ld_grad, sv_elem_size(grad_type));
+    int vec = sv_vec_for(8, D, accumulate);                  // (columns twice would be added twice)
     while (vec > 2 && 32 * vec >= D) vec >>= 1;              // rather all 64 lanes with shorter vectors
     const unsigned slices = (unsigned)((D + 64 * vec - 1) / (64 * vec));
     SV_CHECK_ARG(slices <= 65535u, "svae_lookup_bwd: D %d is too wide for rows that start at odd places", D);

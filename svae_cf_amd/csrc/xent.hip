@@ -451,7 +451,7 @@ struct ProductArgs {
     void* bout;
     const float* scale;       // scale[1] takes the scale of G out again (with the final result)
     long long x_part, g_part, ld_out, slab_stride, bslab_stride;
-    int D, Dp, rows, ndt, nnt, splits, steps, nv32, add, out_vec;
+    int D, Dp, rows, ndt, nnt, splits, steps, nv32, add;
 };
 
 template <typename E, typename T, int BN, int MT, int PARTS, bool OVER_V>
@@ -508,10 +508,10 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int tile, cha
                 float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = acc[t][n][i] * down;
-                if (a.out_vec && d < a.D) sv_store<4>(o, v);
+                if (d + 3 < a.D) sv_store<4>(o, v);
                 else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 3; ++i)
                         if (d + i < a.D) o[i] = (T)v[i];
                 }
             }
@@ -601,18 +601,17 @@ struct PrepArgs {
     float *biasf, *wrow, *lsec;           // lsec: a copy of lse, where it is given
     int* tgt;
     long long ldh, ldw, h_part, w_part, nh, nb;       // nh, nb: workgroups of H and of the bias; the others copy W
-    int tok64, R, Rp, V, Vp, D, Dp, wide_h, wide_w;
+    int tok64, R, Rp, V, Vp, D, Dp;
 };
 
 // eight columns of one row: from T to E, in PARTS parts
 template <typename T, typename E, int PARTS>
-__device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool live, bool wide, char* dst, long long part) {
+__device__ __forceinline__ void copy8(const T* __restrict__ src, int left, bool live, char* dst, long long part) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (live && wide) {                                  // rows of whole aligned vectors: left is at least 8, or nothing
-        if (left > 0) sv_load<8>(src, v);
-    } else if (live) {
+    if (live && left >= 8) sv_load<8>(src, v);
+    else if (live) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < left) v[j] = (float)src[j];
@@ -656,8 +655,8 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
         }
         const T* src = reinterpret_cast<const T*>(a.h) + (tg >= 0 ? r : 0) * a.ldh + c;
         const long long to = a.wc != nullptr ? block_at(r, c, a.Dp) : (r * a.Dp + c) * 2;
-        if (a.hc != nullptr) copy8<T, E, PARTS>(src, a.D - c, tg >= 0, a.wide_h, a.hc + to, a.h_part);
-        if (a.hg != nullptr) copy8<T, E, PARTS>(src, a.D - c, w != 0.f, a.wide_h, a.hg + to, a.h_part);
+        if (a.hc != nullptr) copy8<T, E, PARTS>(src, a.D - c, tg >= 0, a.hc + to, a.h_part);
+        if (a.hg != nullptr) copy8<T, E, PARTS>(src, a.D - c, w != 0.f, a.hg + to, a.h_part);
     } else if (block < a.nh + a.nb) {
         const long long v = i - a.nh * 256;
         if (v < a.Vp) a.biasf[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? (float)reinterpret_cast<const T*>(a.bias)[v] : 0.f;
@@ -665,7 +664,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(PrepArgs a) {
         const long long j = i - (a.nh + a.nb) * 256, r = j / per;
         const int c = (int)(j - r * per) * 8;
         if (r >= a.Vp) return;
-        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + (r < a.V ? r : 0) * a.ldw + c, a.D - c, r < a.V, a.wide_w, a.wc + block_at(r, c, a.Dp), a.w_part);
+        copy8<T, E, PARTS>(reinterpret_cast<const T*>(a.w) + (r < a.V ? r : 0) * a.ldw + c, a.D - c, r < a.V, a.wc + block_at(r, c, a.Dp), a.w_part);
     }
 }
 
@@ -921,9 +920,6 @@ inline int prepare(const Call& c, const Shape& s, bool loss, const float* row_we
     const long long nh = ((long long)s.Rp * (s.Dp / 8) + 255) / 256, nb = (s.Vp + 255) / 256,
                     nw = s.direct ? 0 : ((long long)s.Vp * (s.Dp / 8) + 255) / 256;
     p.nh = nh; p.nb = nb;
-    const int es = sv_elem_size(c.type);
-    p.wide_h = sv_vec_for(8, c.D, c.hidden, c.ld_h, es, c.hidden, c.ld_h, es) == 8;
-    p.wide_w = sv_vec_for(8, c.D, c.weight, c.ld_w, es, c.weight, c.ld_w, es) == 8;
     by_type(c.type, [&](auto t, auto e, auto parts) {
         hipLaunchKernelGGL((xent_prep_kernel<decltype(t), decltype(e), decltype(parts)::value>), grid_of(nh + nb + nw), dim3(256), 0, c.stream, p);
     });
@@ -1092,8 +1088,6 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
                 a.w.bout = db ? (char*)db + v0 * es : nullptr;
                 a.w.slab = wslab ? wslab + v0 * s.Dp : nullptr; a.w.slab_stride = (long long)s.Vp * s.Dp;
                 a.w.bslab = bslab ? bslab + v0 : nullptr; a.w.bslab_stride = s.Vp;
-                const int wide = es * 4 < 16 ? es * 4 : 16;
-                a.w.out_vec = c.D % 4 == 0 && ld_dw * es % wide == 0 && (unsigned long long)a.w.out % wide == 0;
                 a.nw = blocks_for((long long)a.w.ndt * a.w.nnt * a.w.splits);
             }
         }
