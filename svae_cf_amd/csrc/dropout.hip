@@ -8,7 +8,7 @@
 // 16 bits an element: one generator call (20 products of 32 x 32 bits) serves 8 elements.  With 32 bits an element the
 // generator, not HBM, would bound the bf16 form.  The 2^31 keeps the counters apart from those of the reparameterisation noise
 // (svae_philox_normal: column group below 16), so the same seed and step can serve both.  The gradient of dropout is the same
-// map of dy.  65536 x 2048 bf16: 89 us, 6.1 TB/s; 21800 x 150: 6.8 us; 256 x 256: 2.6 us, less than its launch.
+// map of dy.  65536 x 2048 bf16: 89 us, 6.1 TB/s; 21800 x 150: 5.3 us; 256 x 256: 2.6 us, less than its launch.
 #include "elem.h"
 #include "philox.h"
 

@@ -577,9 +577,13 @@ __device__ __forceinline__ void sum_slabs(const SumArgs& a, long long block) {
 #pragma unroll 4
     for (int k = 0; k < a.splits; ++k) s += *reinterpret_cast<const f32x4*>(a.slab + k * a.slab_stride + r * a.Dp + d);
     T* o = reinterpret_cast<T*>(a.out) + r * a.ld_out + d;
+    const float v[4] = {s[0] * down, s[1] * down, s[2] * down, s[3] * down};
+    if (d + 3 < a.D) sv_store<4>(o, v);
+    else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (d + j < a.D) o[j] = (T)(s[j] * down);
+        for (int j = 0; j < 3; ++j)
+            if (d + j < a.D) o[j] = (T)v[j];
+    }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void xent_slab_sum_kernel(SumArgs h, SumArgs w, SumArgs b) {
