@@ -330,3 +330,30 @@ def test_more_threads_than_32_bits_count():
     grad = ops.embedding_grad(torch.ones(R, 1, dtype=BF16, device="cuda"), tok, V, dtype=F32)
     want = R // V + (torch.arange(V, device="cuda") < R % V)       # sums of ones, below 2^24: exact
     assert torch.equal(grad.view(-1).long(), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [1, 3, 7, 9, 13, 141, 515])
+def test_odd_widths_between_other_columns(D, dtype):
+    """Rows at any address: the bits of aligned copies, NaN beside the inputs is not read, what lies beside the output stays."""
+    from svae_cf_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(D)
+    R, V = 3000, 45
+    tok = torch.randint(0, V, (R,), generator=g, device="cuda")
+    tok[:700] = 11                                                 # a segment of many chunks
+    wide = torch.full((R, D + 5), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 3:3 + D] = torch.randn(R, D, generator=g, device="cuda").to(dtype)
+    dy, flat = wide[:, 3:3 + D], wide[:, 3:3 + D].contiguous()
+    want = ops.embedding_grad(flat, tok, V)
+    buf = torch.full((V, D + 4), 7.0, dtype=dtype, device="cuda")
+    ops.embedding_grad(dy, tok, V, out=buf[:, 1:1 + D])
+    assert torch.equal(buf[:, 1:1 + D], want) and bool((buf[:, :1] == 7).all()) and bool((buf[:, 1 + D:] == 7).all())
+    one = torch.full((V, D + 4), 1.0, dtype=dtype, device="cuda")
+    ops.embedding_grad(dy, tok, V, out=one[:, 1:1 + D], accumulate=True)
+    two = torch.full((V, D), 1.0, dtype=dtype, device="cuda")
+    ops.embedding_grad(flat, tok, V, out=two, accumulate=True)
+    assert torch.equal(one[:, 1:1 + D], two) and bool((one[:, :1] == 1).all()) and bool((one[:, 1 + D:] == 1).all())
+    assert torch.equal(ops.embedding(dy[:V], tok), flat[tok])
+    y = ops.dropout(dy, 0.3, 9, step=4)
+    assert torch.equal(y, ops.dropout(flat, 0.3, 9, step=4)) and not bool(torch.isnan(y).any())
+    assert torch.equal(ops.dropout(flat, 0.3, 9, step=4, out=flat), y)
