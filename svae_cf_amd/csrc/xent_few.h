@@ -245,12 +245,12 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : 2) void few_logit_kernel(FewArgs
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) m = fmaxf(m, acc[t][n][i]);
-        // fmaxf leaves NaN out; the sum brings it back (exp(NaN - top))
-        const float base = m == -INFINITY ? 0.f : m * -LOG2E;
+        // fmaxf leaves NaN out; the sum brings it back (exp(NaN - top)).  The difference first: exact where logits are far from 0
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(fmaf(acc[t][n][i], LOG2E, base));
+            for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((acc[t][n][i] - base) * LOG2E);
 #pragma unroll
         for (int o = 16; o < 64; o <<= 1) {
             const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
