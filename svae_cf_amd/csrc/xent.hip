@@ -466,7 +466,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void xent_loss_kernel(LogitArgs a) {
 struct ProductArgs {
     const char* x;            // blocks of W (from the piece's first row on) or of H
     const char* g;            // blocks of G
-    float* slab;              // [splits][...][Dp] at the first row of this launch, added to when add != 0; NULL: out is written
+    float* slab;              // [splits][...][Dp], added to when add != 0; NULL: out is written
     float* bslab;             // [splits][...] bias gradient, or NULL
     void* out;                // [rows][ld_out] of the caller's type
     void* bout;
@@ -544,32 +544,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int tile, cha
     }
 }
 
-// One launch of the gradient: G of one piece of the vocabulary, and the products of the piece before (its G is in the other of
-// two buffers).  The long workgroups come first, the short tiles of G fill what they leave.
-struct PieceArgs {
-    LogitArgs z;
-    ProductArgs h, w;
-    unsigned nh, nw;          // workgroups of dH and of dW, multiples of 8; the rest make G
-};
-
-template <typename E, typename T, int BN, int MT, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, 2) void xent_piece_kernel(PieceArgs a) {
-    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[128 * BK * 2], b1[128 * BK * 2], b2[128 * BK * 2];
-    char* const sa[STAGES] = {a0, a1, a2};
-    char* const sb[STAGES] = {b0, b1, b2};
-    if (blockIdx.x < a.nw) {
-        const int tile = tile_of(blockIdx.x, a.w.ndt * a.w.nnt * a.w.splits);
-        if (tile >= 0) product_tile<E, T, 128, MT, PARTS, false>(a.w, tile, sa, sb);
-    } else if (blockIdx.x < a.nw + a.nh) {
-        const int tile = tile_of(blockIdx.x - a.nw, a.h.ndt * a.h.nnt * a.h.splits);
-        if (tile >= 0) product_tile<E, T, BN, BN == 64 ? MT / 2 : MT, PARTS, true>(a.h, tile, sa, sb);
-    } else {
-        const int tile = tile_of(blockIdx.x - a.nw - a.nh, a.z.nvt * a.z.nrt);
-        if (tile >= 0) logit_tile<E, BN, ALONG, PARTS, true>(a.z, tile, sa, sb, (float2(*)[BN])nullptr);
-    }
-}
-
-// out[r][d] = sum of the slabs, in order; the slabs of dH, of dW and of the bias gradient in one launch
+// out[r][d] = sum of the slabs, in order
 struct SumArgs {
     const float* slab;
     void* out;
@@ -606,6 +581,41 @@ __device__ __forceinline__ void sum_slabs(const SumArgs& a, long long block) {
             if (d + j < a.D) o[j] = (T)v[j];
     }
 }
+
+// One launch of the gradient: G of one piece of the vocabulary, the products of the piece before (its G is in the other of two
+// buffers), and the sums of the slabs that dW and db have of the piece before that (in the other of two again, so that slabs take the
+// memory of two pieces, whatever the vocabulary).  The long workgroups come first, the short tiles of G fill what they leave; the sums
+// in between (21800 x 20000 x 200 bf16 1073 us, behind them 1097).
+struct PieceArgs {
+    LogitArgs z;
+    ProductArgs h, w;
+    SumArgs sw, sb;
+    unsigned nh, nw;          // workgroups of dH and of dW, multiples of 8; then those of the sums; the rest make G
+};
+
+template <typename E, typename T, int BN, int MT, int PARTS>
+__global__ __launch_bounds__(64 * WAVES, 2) void xent_piece_kernel(PieceArgs a) {
+    __shared__ __attribute__((aligned(1024))) char a0[BM * BK * 2], a1[BM * BK * 2], a2[BM * BK * 2], b0[128 * BK * 2], b1[128 * BK * 2], b2[128 * BK * 2];
+    char* const sa[STAGES] = {a0, a1, a2};
+    char* const sb[STAGES] = {b0, b1, b2};
+    const unsigned ns = (unsigned)(a.sw.blocks + a.sb.blocks);
+    if (blockIdx.x < a.nw) {
+        const int tile = tile_of(blockIdx.x, a.w.ndt * a.w.nnt * a.w.splits);
+        if (tile >= 0) product_tile<E, T, 128, MT, PARTS, false>(a.w, tile, sa, sb);
+    } else if (blockIdx.x < a.nw + a.nh) {
+        const int tile = tile_of(blockIdx.x - a.nw, a.h.ndt * a.h.nnt * a.h.splits);
+        if (tile >= 0) product_tile<E, T, BN, BN == 64 ? MT / 2 : MT, PARTS, true>(a.h, tile, sa, sb);
+    } else if (blockIdx.x < a.nw + a.nh + ns) {
+        const long long block = blockIdx.x - a.nw - a.nh;
+        if (block < a.sw.blocks) sum_slabs<T>(a.sw, block);
+        else sum_slabs<T>(a.sb, block - a.sw.blocks);
+    } else {
+        const int tile = tile_of(blockIdx.x - a.nw - a.nh - ns, a.z.nvt * a.z.nrt);
+        if (tile >= 0) logit_tile<E, BN, ALONG, PARTS, true>(a.z, tile, sa, sb, (float2(*)[BN])nullptr);
+    }
+}
+
+// the slabs of dH, and those of dW and of the bias gradient that the last piece has, in one launch
 template <typename T>
 __global__ __launch_bounds__(256) void xent_slab_sum_kernel(SumArgs h, SumArgs w, SumArgs b) {
     const long long block = block_of();
@@ -813,7 +823,7 @@ constexpr int SLOTS = 512;                                 // workgroups at a ti
 struct Shape {
     int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, h_splits, w_splits, ndt, dblocks;
     int few, R4, wd, chunks;  // few: the kernels for few rows, with this many tiles of 16
-    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab, b_slab, z, total;
+    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab[2], b_slab[2], z, total;
 };
 
 // parts of a product's contraction: no workgroup should work longer than a slot's share of the launch
@@ -906,8 +916,12 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
         if (s->h_splits > s->piece_tiles * (BM / BK) / 4) s->h_splits = s->piece_tiles * (BM / BK) / 4;
         if (s->w_splits > s->Rp / BK / 2) s->w_splits = s->Rp / BK / 2;
         s->h_slab = take(4ll * s->Rp * s->Dp * s->h_splits);
-        s->w_slab = take(s->w_splits > 1 ? 4ll * s->Vp * s->Dp * s->w_splits : 0);
-        s->b_slab = take(s->w_splits > 1 ? 4ll * s->Vp * s->w_splits : 0);
+        // (more than one slab only of fewer than 512 tiles: 128 MiB at most, of dH's as of a piece of dW's)
+        for (int k = 0; k < 2; ++k) {
+            const long long rows = s->w_splits > 1 && k < s->pieces ? (long long)s->piece_tiles * BM * s->w_splits : 0;
+            s->w_slab[k] = take(4 * rows * s->Dp);
+            s->b_slab[k] = take(4 * rows);
+        }
     }
     s->total = at > end ? at : end;
     return 0;
@@ -1079,9 +1093,21 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
     z.lse = (const float*)(c.work + s.lse); z.wrow = (const float*)(c.work + s.wrow); z.scale = scale;
     ProductArgs d{};
     d.scale = scale; d.g_part = s.g_part; d.D = c.D; d.Dp = s.Dp; d.ndt = s.ndt;
-    float* const wslab = s.w_splits > 1 ? (float*)(c.work + s.w_slab) : nullptr;
-    float* const bslab = s.w_splits > 1 && db ? (float*)(c.work + s.b_slab) : nullptr;
-    for (int p = 0; p <= s.pieces; ++p) {                  // launch p: G of piece p, products of piece p - 1
+    const bool slabs = s.w_splits > 1;
+    const long long piece_rows = (long long)s.piece_tiles * BM;
+    // the sums of the slabs of dW and db that piece p has
+    auto sums = [&](int p, SumArgs& w, SumArgs& b) {
+        if (!dw || !slabs) return;
+        const long long v0 = p * piece_rows;
+        w.slab = (float*)(c.work + s.w_slab[p & 1]); w.slab_stride = piece_rows * s.Dp; w.out = (char*)dw + v0 * ld_dw * es; w.ld_out = ld_dw;
+        w.scale = scale; w.splits = s.w_splits; w.rows = (int)(c.V - v0 < piece_rows ? c.V - v0 : piece_rows); w.D = c.D; w.Dp = s.Dp;
+        w.blocks = ((long long)w.rows * (s.Dp / 4) + 255) / 256;
+        if (!db) return;
+        b = w;
+        b.slab = (float*)(c.work + s.b_slab[p & 1]); b.slab_stride = piece_rows; b.out = (char*)db + v0 * es; b.D = b.Dp = 1;
+        b.blocks = (w.rows + 255) / 256;
+    };
+    for (int p = 0; p <= s.pieces; ++p) {                  // launch p: G of piece p, products of piece p - 1, sums of piece p - 2
         PieceArgs a{};
         unsigned nz = 0;
         if (p < s.pieces) {
@@ -1111,13 +1137,15 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
                 a.w.nnt = nt * (BM / 128); a.w.splits = s.w_splits; a.w.steps = s.Rp / BK; a.w.add = 0;
                 a.w.out = (char*)dw + v0 * ld_dw * es; a.w.ld_out = ld_dw;
                 a.w.bout = db ? (char*)db + v0 * es : nullptr;
-                a.w.slab = wslab ? wslab + v0 * s.Dp : nullptr; a.w.slab_stride = (long long)s.Vp * s.Dp;
-                a.w.bslab = bslab ? bslab + v0 : nullptr; a.w.bslab_stride = s.Vp;
+                a.w.slab = slabs ? (float*)(c.work + s.w_slab[(p - 1) & 1]) : nullptr; a.w.slab_stride = piece_rows * s.Dp;
+                a.w.bslab = slabs && db ? (float*)(c.work + s.b_slab[(p - 1) & 1]) : nullptr; a.w.bslab_stride = piece_rows;
                 a.nw = blocks_for((long long)a.w.ndt * a.w.nnt * a.w.splits);
             }
         }
-        SV_CHECK_ARG((long long)nz + a.nh + a.nw < 1ll << 24, "svae_xent: R %d, V %d, D %d need too many workgroups", c.R, c.V, c.D);
-        piece(c, s, a, nz + a.nh + a.nw);
+        if (p > 1) sums(p - 2, a.sw, a.sb);
+        const long long blocks = (long long)nz + a.nh + a.nw + a.sw.blocks + a.sb.blocks;
+        SV_CHECK_ARG(blocks < 1ll << 24, "svae_xent: R %d, V %d, D %d need too many workgroups", c.R, c.V, c.D);
+        piece(c, s, a, (unsigned)blocks);
         SV_LAUNCH_CHECK();
     }
     SumArgs h1{}, w1{}, b1{};
@@ -1126,15 +1154,7 @@ inline int gradients(const Call& c, const Shape& s, long long h, void* dh, long 
         h1.scale = scale; h1.splits = s.h_splits; h1.rows = c.R; h1.D = c.D; h1.Dp = s.Dp;
         h1.blocks = ((long long)c.R * (s.Dp / 4) + 255) / 256;
     }
-    if (dw && wslab) {
-        w1.slab = wslab; w1.slab_stride = (long long)s.Vp * s.Dp; w1.out = dw; w1.ld_out = ld_dw;
-        w1.scale = scale; w1.splits = s.w_splits; w1.rows = c.V; w1.D = c.D; w1.Dp = s.Dp;
-        w1.blocks = ((long long)c.V * (s.Dp / 4) + 255) / 256;
-    }
-    if (db && bslab) {
-        b1.slab = bslab; b1.slab_stride = s.Vp; b1.out = db; b1.scale = scale; b1.splits = s.w_splits; b1.rows = c.V; b1.D = b1.Dp = 1;
-        b1.blocks = (c.V + 255) / 256;
-    }
+    sums(s.pieces - 1, w1, b1);
     if (h1.blocks + w1.blocks + b1.blocks > 0) {
         by_type(c.type, [&](auto t, auto, auto) {
             hipLaunchKernelGGL(xent_slab_sum_kernel<decltype(t)>, grid_of(h1.blocks + w1.blocks + b1.blocks), dim3(256), 0, c.stream, h1, w1, b1);
