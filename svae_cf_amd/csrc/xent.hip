@@ -728,10 +728,11 @@ __global__ __launch_bounds__(256) void xent_scale_kernel(const float* __restrict
 }
 
 // lse and loss from the tiles' statistics; one workgroup more for the scale, where it is wanted.  FEW: a workgroup for a row, its
-// threads share the tiles; else 32 rows a workgroup, eight threads for each.
+// threads share the tiles; else 32 rows a workgroup, eight threads for each.  run: the statistics of the launches before, where the
+// vocabulary is taken in several (begun: there are any), to which this launch adds; the last one (lse) has the results.
 template <bool FEW>
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
-                                                        const int* __restrict__ tgt, int R, int Rp, int nvt,
+                                                        const int* __restrict__ tgt, int R, int Rp, int nvt, float2* __restrict__ run, int begun,
                                                         float* __restrict__ nll, float* __restrict__ lse, float* __restrict__ lsec,
                                                         const float* __restrict__ wrow, float top, float* __restrict__ scale) {
     if (scale != nullptr && blockIdx.x == gridDim.x - 1) {
@@ -743,6 +744,10 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
     const int i = threadIdx.x % ROWS, s = threadIdx.x / ROWS;
     const long long r = (long long)blockIdx.x * ROWS + i;
     float m = -INFINITY, sum = 0.f;
+    if (begun && s == 0) {
+        m = run[r].x;
+        sum = run[r].y;
+    }
     for (int v = s; v < nvt; v += 4 * SLICES) {          // four tiles at a time: their loads do not wait for each other
         float2 p[4];
 #pragma unroll
@@ -766,6 +771,10 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
         sum = red[0][0].y;
     }
     for (int k = 1; k < (FEW ? 4 : 8); ++k) join_sums(m, sum, red[k][i].x, red[k][i].y);
+    if (lse == nullptr) {
+        run[r] = make_float2(m, sum);
+        return;
+    }
     const bool here = tgt[r] >= 0;
     const float l = m + logf(sum);
     if (lsec != nullptr) lsec[r] = here ? l : 0.f;
@@ -818,12 +827,14 @@ constexpr long long FEW_WEIGHT_16 = 1ll << 23;
 constexpr int FEW_OWN_TILES = 2048;
 constexpr int DIRECT_ROWS = 512;                           // up to here a loss takes W as it lies
 constexpr long long PIECE_LEAST = 128ll << 20, PIECE_MOST = 512ll << 20;     // what G of a piece may take; there are two
+constexpr long long STATISTICS_MOST = 512ll << 20;         // what the loss's tiles may leave before their rows are joined
 constexpr int SLOTS = 512;                                 // workgroups at a time: two on each of 256 CUs
 
 struct Shape {
     int parts, Rp, Vp, Dp, BN, nrt, nvt, direct, pieces, piece_tiles, h_splits, w_splits, ndt, dblocks;
     int few, R4, wd, chunks;  // few: the kernels for few rows, with this many tiles of 16
-    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, g[2], g_part, h_slab, w_slab[2], b_slab[2], z, total;
+    int slice;                // vocabulary tiles of a launch of the loss, at most
+    long long h, hg, h_part, w, w_part, ldw, bias, tgt, wrow, lse, zt, part, scale, run, g[2], g_part, h_slab, w_slab[2], b_slab[2], z, total;
 };
 
 // parts of a product's contraction: no workgroup should work longer than a slot's share of the launch
@@ -892,8 +903,12 @@ inline int shape_of(const void* weight, long long ld_w, int type, long long R, l
     s->lse = take(4ll * s->Rp);
     s->zt = take(4ll * s->Rp);
     s->scale = take(8);
+    long long slice = STATISTICS_MOST / (8ll * s->Rp);
+    slice = slice < MOST_BLOCKS / s->nrt ? slice : MOST_BLOCKS / s->nrt;
+    s->slice = (int)(slice < s->nvt ? slice : s->nvt);     // (at least four: Rp is at most 2^24)
+    s->run = take(s->slice < s->nvt ? 8ll * s->Rp : 0);
     s->part = s->g[0] = at;                                // the loss's statistics are done with when G is made
-    const long long end = at + 8ll * s->nvt * s->Rp;
+    const long long end = at + 8ll * s->slice * s->Rp;
     if (grad != LOSS) {
         // A piece's G is written and read twice, and every piece adds to all of dH's sums (4 Rp Dp bytes, read and written): at
         // least four times those, and 128 MiB for large launches (8192 x 131072 x 1024: 7.2 ms with pieces of 128 MiB, 7.4 with 512)
@@ -981,32 +996,36 @@ inline LogitArgs logit_args(const Call& c, const Shape& s) {
 inline int loss(const Call& c, const Shape& s, float* nll, float* lse, bool grad) {
     LogitArgs a = logit_args(c, s);
     a.zt = (float*)(c.work + s.zt);
-    const int slice = (int)(MOST_BLOCKS / s.nrt);          // vocabulary tiles of a launch, at most
-    for (int v = 0; v < s.nvt; v += slice) by_type(c.type, [&](auto, auto e, auto parts) {
-        typedef decltype(e) E;
-        constexpr int P = decltype(parts)::value;
-        a.v_begin = v * BM;
-        a.nvt = s.nvt - v < slice ? s.nvt - v : slice;
-        a.part = (float2*)(c.work + s.part) + (long long)v * s.Rp;
-        const dim3 grid(blocks_for((long long)a.nvt * a.nrt));
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, a); };
-        if constexpr (P == 1) {
-            if (s.direct) {
-                if (s.BN == 64) go(xent_loss_kernel<E, 64, PLAIN, P>);
-                else go(xent_loss_kernel<E, 128, PLAIN, P>);
-                return;
-            }
-        }
-        if (s.BN == 64) go(xent_loss_kernel<E, 64, ALONG, P>);
-        else go(xent_loss_kernel<E, 128, ALONG, P>);
-    });
-    SV_LAUNCH_CHECK();
+    a.part = (float2*)(c.work + s.part);
     const bool few_rows = c.R <= 1024 && s.nvt > 64;
-    float* const scale = grad ? (float*)(c.work + s.scale) : nullptr;
-    const unsigned blocks = (unsigned)(!few_rows ? s.Rp / 32 : grad ? s.Rp : c.R) + (scale ? 1 : 0);
-    hipLaunchKernelGGL(few_rows ? xent_rows_kernel<true> : xent_rows_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, (const float2*)(c.work + s.part), a.zt,
-                       a.tgt, c.R, s.Rp, s.nvt, nll, lse, grad ? (float*)(c.work + s.lse) : nullptr, (const float*)(c.work + s.wrow), top_of(c.type), scale);
-    SV_LAUNCH_CHECK();
+    for (int v = 0; v < s.nvt; v += s.slice) {
+        const bool last = v + s.slice >= s.nvt;
+        a.v_begin = v * BM;
+        a.nvt = last ? s.nvt - v : s.slice;
+        by_type(c.type, [&](auto, auto e, auto parts) {
+            typedef decltype(e) E;
+            constexpr int P = decltype(parts)::value;
+            const dim3 grid(blocks_for((long long)a.nvt * a.nrt));
+            auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WAVES), 0, c.stream, a); };
+            if constexpr (P == 1) {
+                if (s.direct) {
+                    if (s.BN == 64) go(xent_loss_kernel<E, 64, PLAIN, P>);
+                    else go(xent_loss_kernel<E, 128, PLAIN, P>);
+                    return;
+                }
+            }
+            if (s.BN == 64) go(xent_loss_kernel<E, 64, ALONG, P>);
+            else go(xent_loss_kernel<E, 128, ALONG, P>);
+        });
+        SV_LAUNCH_CHECK();
+        // (rows behind R: their statistics are kept, their lse is for the gradients)
+        float* const scale = grad && last ? (float*)(c.work + s.scale) : nullptr;
+        const unsigned blocks = (unsigned)(!few_rows ? s.Rp / 32 : grad || !last ? s.Rp : c.R) + (scale ? 1 : 0);
+        hipLaunchKernelGGL(few_rows ? xent_rows_kernel<true> : xent_rows_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, (const float2*)a.part, a.zt,
+                           a.tgt, c.R, s.Rp, a.nvt, (float2*)(c.work + s.run), v > 0, nll, last ? lse : nullptr, grad ? (float*)(c.work + s.lse) : nullptr,
+                           (const float*)(c.work + s.wrow), top_of(c.type), scale);
+        SV_LAUNCH_CHECK();
+    }
     return 0;
 }
 
@@ -1061,8 +1080,8 @@ inline int few(const Call& c, const Shape& s, float* nll, float* lse, const floa
             else go(few_logit_kernel<T, 4, false>, s.nvt, a);
         }
         if (nll)
-            go(xent_rows_kernel<true>, c.R, (const float2*)a.part, (const float*)a.zt, (const int*)a.tgt, c.R, s.Rp, s.nvt, nll, lse,
-               (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);
+            go(xent_rows_kernel<true>, c.R, (const float2*)a.part, (const float*)a.zt, (const int*)a.tgt, c.R, s.Rp, s.nvt, (float2*)nullptr, 0,
+               nll, lse, (float*)nullptr, (const float*)nullptr, 0.f, (float*)nullptr);
         if (!dh && !dw) return;
         const long long blocks = (long long)s.chunks * s.ndt;
         auto grad = [&](auto wide) {

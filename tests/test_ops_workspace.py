@@ -48,3 +48,13 @@ def test_gradient_workspace(R, V, D, kind):
     sums = max(4 * up(R, 128) * up(D, 32), 128 * MIB) + 2 * 129 * MIB
     most = copies(kind, R, V, D, True) + rows_and_columns(R, V) + max(statistics, pieces(kind, R)) + sums
     assert asked(kind, R, V, D, True) <= most
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("R,V,D", SIZES)
+def test_statistics_of_large_losses(R, V, D, kind):
+    """No more than 512 MiB of the tiles' statistics at a time, and eight bytes for a row where they are taken in several goes."""
+    statistics = min(8 * up(R, 128) * (up(V, 256) // 256), 512 * MIB) + 8 * up(R, 128)
+    assert asked(kind, R, V, D, False) <= copies(kind, R, V, D, False) + rows_and_columns(R, V) + statistics
+    sums = max(4 * up(R, 128) * up(D, 32), 128 * MIB) + 2 * 129 * MIB
+    assert asked(kind, R, V, D, True) <= copies(kind, R, V, D, True) + rows_and_columns(R, V) + 8 * up(R, 128) + pieces(kind, R) + sums
