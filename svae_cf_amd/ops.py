@@ -9,13 +9,15 @@ Conventions
   - sums, softmax statistics and losses are fp32; a result is rounded once, to its tensor's type;
   - results are the same in every run (no floating-point atomics).
 
-``embedding``, ``dropout`` and ``linear_cross_entropy`` take part in autograd; ``embedding_grad``, ``linear_nll`` and
-``linear_nll_grad`` are the same kernels for programs that run their own backward pass (and for graph capture).
+``embedding``, ``dropout`` and ``linear_cross_entropy`` take part in autograd (reverse mode, once; tensors with forward-mode
+tangents are refused); ``embedding_grad``, ``linear_nll`` and ``linear_nll_grad`` are the same kernels for programs that run their
+own backward pass (and for graph capture).
 """
 import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -43,6 +45,11 @@ class _On:
             torch.cuda.set_device(self.back)
 
 
+def _no_tangent(t, what):
+    if forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:      # (a kernel would drop it)
+        raise NotImplementedError("%s has a tangent: forward-mode differentiation is not supported" % what)
+
+
 def _check(t, what, types=_TYPES, device=None):
     """Type code of a tensor that has one of `types` and is on the GPU (the one of `device`, a number, if given)."""
     if not isinstance(t, torch.Tensor):
@@ -50,6 +57,7 @@ def _check(t, what, types=_TYPES, device=None):
     code = types.get(t.dtype)
     if code is None:
         raise TypeError("%s has type %s: %s are supported" % (what, t.dtype, ", ".join(str(k)[6:] for k in types)))
+    _no_tangent(t, what)
     if not t.is_cuda:
         raise RuntimeError("%s is on %s: the HIP path has no CPU fallback" % (what, t.device))
     if device is not None and t.get_device() != device:
@@ -390,4 +398,6 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, reduction="mean"):
     "none".  The backward pass makes the logits again in pieces of the vocabulary; gradients have the inputs' type."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be mean, sum or none, got %r" % (reduction,))
+    for t, what in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):        # (gone inside the function)
+        _no_tangent(t, what)
     return _LinearCrossEntropy.apply(hidden, weight, bias, targets, reduction)
