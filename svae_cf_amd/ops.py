@@ -90,6 +90,12 @@ def _apart(a, b):
     return not a.numel() or not b.numel() or a1 <= b0 or b1 <= a0
 
 
+def _written(t):
+    """Tells autograd that a caller's tensor has new values: a graph that has kept it refuses its backward pass."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _flat(t):
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
@@ -174,7 +180,8 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=No
     _size(V, "vocabulary")
     _size(D, "width", 1 << 24)
     _size(R + 1, "tokens + 1", (1 << 30) + 1)
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise ValueError("accumulate needs out")
         dtype = dout.dtype if dtype is None else dtype
@@ -198,6 +205,8 @@ def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=No
         _lib.call("svae_token_sort", tok.data_ptr(), _IDS[tok.dtype], R, V, pad, keys, perm, rest, n_sort, st)
         _lib.call("svae_lookup_bwd", dy.data_ptr(), _TYPES[dy.dtype], ld, keys, perm, R, V, D, scale, out.data_ptr(), _TYPES[out.dtype],
                   out.stride(0) if V > 1 else D, int(accumulate), rest, n_sum, st)
+    if given:
+        _written(out)
     return out
 
 
@@ -267,7 +276,10 @@ def dropout(x, p, seed, step=0, row_key=None, out=None):
             raise ValueError("out must be contiguous and shaped like x")
         if not _apart(x, out) and not (x.is_contiguous() and x.data_ptr() == out.data_ptr()):
             raise ValueError("out must be x itself or lie apart from it")
-    return _dropout(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key, out)
+    y = _dropout(x, p, int(seed), step if isinstance(step, torch.Tensor) else int(step), row_key, out)
+    if out is not None:
+        _written(out)
+    return y
 
 
 # ---- softmax cross entropy behind a linear layer ----------------------------------------------------------------------------
