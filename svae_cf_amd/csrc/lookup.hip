@@ -299,10 +299,17 @@ __device__ __forceinline__ void sum_rows(const T* __restrict__ dy, long long ldd
     for (int i = b; i < e; i += 16 * step) add_rows<16, VEC>(dy, ldd, place, i, e, step, c, acc);
 }
 
+// skip: columns at the front of a vector that reaches back, which another lane has too (written twice, but not added twice)
 template <int VEC, typename G>
-__device__ __forceinline__ void put_row(G* __restrict__ dst, float* acc, float scale, int accumulate) {
+__device__ __forceinline__ void put_row(G* __restrict__ dst, float* acc, float scale, int accumulate, int skip) {
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[q] *= scale;
+    if (accumulate && skip > 0) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q)
+            if (q >= skip) dst[q] = (G)(acc[q] + (float)dst[q]);
+        return;
+    }
     if (accumulate) {
         float old[VEC];
         sv_load<VEC>(dst, old);
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_kernel(const T* __restrict__ d
                 for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
                 if (far) sum_rows<VEC>(dy, ldd, [&](int i) { return perm[i]; }, s, e, 1, c, acc);
                 else if (e > s) sum_rows<VEC>(dy, ldd, [&](int i) { return __builtin_amdgcn_readlane(place, i - s0); }, s, e, 1, c, acc);
-                put_row<VEC>(dst + c, acc, scale, accumulate);
+                put_row<VEC>(dst + c, acc, scale, accumulate, c0 - c);
             }
         }
         s = e;
@@ -420,7 +427,7 @@ __global__ __launch_bounds__(256) void lookup_bwd_long_kernel(const int* __restr
 #pragma unroll
         for (int q = 0; q < VEC; ++q)
             acc[q] = (red[0][q * 64 + lane] + red[1][q * 64 + lane]) + (red[2][q * 64 + lane] + red[3][q * 64 + lane]);
-        put_row<VEC>(grad + (long long)k * ldg + c, acc, scale, accumulate);
+        put_row<VEC>(grad + (long long)k * ldg + c, acc, scale, accumulate, c0 - c);
     }
 }
 
@@ -533,14 +540,14 @@ extern "C" int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, con
     // rows of 256, 21800 tokens: 16 rows 16.6 us, 4 rows 12.7 us)
     const int group = V >= 8192 * MOST_GROUP ? MOST_GROUP : V >= 8192 * 8 ? 8 : 4;
     const long long nrow = ((long long)V + 4 * group - 1) / (4 * group);
-    int vec = sv_vec_for(8, D, accumulate);                  // (columns twice would be added twice)
+    int vec = sv_vec_for(8, D, false);
     while (vec > 2 && 32 * vec >= D) vec >>= 1;              // rather all 64 lanes with shorter vectors
-    const unsigned slices = (unsigned)((D + 64 * vec - 1) / (64 * vec));
-    SV_CHECK_ARG(slices <= 65535u, "svae_lookup_bwd: D %d is too wide for rows that start at odd places", D);
+    const long long slices = ((long long)D + 64 * vec - 1) / (64 * vec);
+    SV_CHECK_ARG(slices <= 65535, "svae_lookup_bwd: D %d is wider than %d", D, 65535 * 64 * 8);
     // (threads of a dimension are counted in 32 bits: more workgroups than 2^23 go on in the third one)
     auto grid = [&](long long blocks) {
         const long long most = 1ll << 23;
-        return dim3((unsigned)(blocks < most ? blocks : most), slices, (unsigned)((blocks + most - 1) / most));
+        return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)slices, (unsigned)((blocks + most - 1) / most));
     };
     sv_by_type(dy_type, [&](auto t) {
         sv_by_type(grad_type, [&](auto o) {
