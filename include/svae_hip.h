@@ -407,7 +407,8 @@ void svae_plan_destroy(void* plan);
 /* ---- embedding lookup of any width and type, gradient by sorted tokens -------------------------------------
  * No counterpart in the reference (its nn.Embedding is svae_embed_fwd / svae_embed_bwd: width 256, fp32, rows sorted by the
  * host's plan).  Types: 0 fp32, 1 bf16, 2 fp16; tokens: int32, or int64 with tok64 != 0; ld: elements from one row to the
- * next (>= D).  A token outside [0, V) marks a padded place.  R == 0 is allowed, pointers may then be NULL.
+ * next (>= D; D at most 2^30, in the gradient 65535 x 512; R at most 2^30 in sort and gradient).  A token outside [0, V) marks a
+ * padded place.  R == 0 is allowed, pointers may then be NULL.
  *   svae_lookup_fwd       out[r][0..D) = scale * table[tokens[r]][0..D), a zero row for a padded place
  *   svae_token_sort       stable sort of the places by token: keys [R] ascending (padded places and the token `pad` as V,
  *                         at the end; pad < 0: none), perm [R] the places; work: svae_token_sort_bytes(R, V, &bytes)
@@ -428,7 +429,7 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
 /* ---- softmax cross entropy behind a linear layer over a large vocabulary --------------------------------------
  * No counterpart in the reference (its loss over the catalogue is svae_proj_nll_*: width 150, next-k targets).
  * z = hidden weight^T + bias, [R][V], never kept.  hidden [R][D], weight [V][D] (rows ld elements apart), bias [V] or NULL, all
- * of one type (0 fp32, 1 bf16, 2 fp16); targets [R] int32, or int64 with tok64 != 0.  A row whose target is outside [0, V) is
+ * of one type (0 fp32, 1 bf16, 2 fp16); targets [R] int32, or int64 with tok64 != 0; R at most 2^24, V 2^28, D 2^16, ld_w 2^20.  A row whose target is outside [0, V) is
  * left out: nll = lse = 0, no gradient, whatever the row holds.  Products of bf16 / fp16 run on the matrix units as they are,
  * fp32 ones as six products of bf16 parts (24 bits) or, for few rows, in fp32; sums, statistics and losses are fp32.  In the
  * gradient w (softmax - onehot) is rounded to a 16-bit type after a scale by the largest row weight (16 rows or fewer: not at all).
@@ -464,7 +465,7 @@ int svae_xent_fwd_bwd(const void* hidden, long long ld_h, const void* weight, lo
  * k = round(65536 p), else 0; the bits come from Philox4x32-10 with key seed and counter (row_key[r], c / 8 + 2^31, step), as
  * csrc/dropout.hip says: replayable, never stored, independent of strides and of how rows are dealt to GPUs.  row_key [R] may
  * be NULL (the row's index); step_dev != NULL: the step is read there on the device (low 32 bits), so that replays of a
- * captured graph can draw new masks.  y may be x.  type: 0 fp32, 1 bf16, 2 fp16.  The gradient is the same call on dy. */
+ * captured graph can draw new masks.  y may be x.  C is at most 2^30.  type: 0 fp32, 1 bf16, 2 fp16.  The gradient is the same call on dy. */
 int svae_dropout(const void* x, long long ldx, void* y, long long ldy, int type, int R, int C, double p,
                  unsigned long long seed, unsigned step, const long long* step_dev, const long long* row_key, void* stream);
 

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, long long ldx,
 extern "C" int svae_dropout(const void* x, long long ldx, void* y, long long ldy, int type, int R, int C, double p,
                             unsigned long long seed, unsigned step, const long long* step_dev, const long long* row_key,
                             void* stream) {
-    SV_CHECK_ARG(R >= 0 && C > 0 && ldx >= C && ldy >= C, "svae_dropout: sizes R %d, C %d, ld %lld, %lld", R, C, ldx, ldy);
+    SV_CHECK_ARG(R >= 0 && C > 0 && C <= 1 << 30 && ldx >= C && ldy >= C, "svae_dropout: sizes R %d, C %d, ld %lld, %lld", R, C, ldx, ldy);
     SV_CHECK_ARG(type >= 0 && type <= 2, "svae_dropout: type %d", type);
     SV_CHECK_ARG(p >= 0.0 && p <= 1.0, "svae_dropout: p = %g is no probability", p);
     const unsigned below = (unsigned)(p * 65536.0 + 0.5);

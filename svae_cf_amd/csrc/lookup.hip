@@ -438,7 +438,8 @@ inline long long chunks_of(int R) { return ((long long)R + CHUNK - 1) / CHUNK; }
 
 extern "C" int svae_lookup_fwd(const void* table, int table_type, long long ld_table, const void* tokens, int tok64, void* out,
                                int out_type, long long ld_out, int R, int V, int D, float scale, void* stream) {
-    SV_CHECK_ARG(R >= 0 && V > 0 && D > 0 && ld_table >= D && ld_out >= D, "svae_lookup_fwd: sizes R %d, V %d, D %d, ld %lld, %lld", R, V, D, ld_table, ld_out);
+    // (the kernel counts columns in 32 bits, one step past the last)
+    SV_CHECK_ARG(R >= 0 && V > 0 && D > 0 && D <= 1 << 30 && ld_table >= D && ld_out >= D, "svae_lookup_fwd: sizes R %d, V %d, D %d, ld %lld, %lld", R, V, D, ld_table, ld_out);
     SV_CHECK_ARG(table_type >= 0 && table_type <= 2 && out_type >= 0 && out_type <= 2, "svae_lookup_fwd: types %d, %d", table_type, out_type);
     if (R == 0) return 0;
     SV_CHECK_ARG(table && tokens && out, "svae_lookup_fwd: null pointer");

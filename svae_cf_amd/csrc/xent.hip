@@ -1225,7 +1225,7 @@ extern "C" int svae_xent_fwd(const void* hidden, long long ld_h, const void* wei
 }
 
 extern "C" int svae_xent_reduce(const float* nll, const void* targets, int tok64, int R, int V, int mean, float* out, void* stream) {
-    SV_CHECK_ARG(nll && targets && out && R > 0 && V > 0, "svae_xent_reduce: bad arguments");
+    SV_CHECK_ARG(nll && targets && out && R > 0 && R <= 1 << 24 && V > 0, "svae_xent_reduce: bad arguments");
     hipLaunchKernelGGL(xent_reduce_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, nll, targets, tok64, R, V, mean, out);
     SV_LAUNCH_CHECK();
     return 0;
