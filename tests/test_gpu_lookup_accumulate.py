@@ -21,3 +21,23 @@ def test_each_column_is_added_once(R, V, D, dtype):
     here = tok >= 0
     want[:, 2:2 + D].index_add_(0, tok[here], dy[here].double())
     assert torch.equal(out, want.to(dtype))                # (rounded once)
+
+
+def test_captured_with_more_tokens_than_one_workgroup_sorts():
+    """A graph over 21 800 tokens, replayed on new ones between eager calls: the bits of the eager call, added to what is there."""
+    from svae_cf_amd import ops
+    R, V, D = 21800, 5000, 72
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tok, dy = torch.randint(-1, V, (R,), generator=g, device="cuda"), torch.randn(R, D, generator=g, device="cuda")
+    out = torch.zeros(V, D, device="cuda")
+    ops.embedding_grad(dy, tok, V, out=out.clone(), accumulate=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.embedding_grad(dy, tok, V, out=out, accumulate=True)
+    for _ in range(4):
+        tok.copy_(torch.randint(-1, V, (R,), generator=g, device="cuda"))
+        want = ops.embedding_grad(dy, tok, V, out=out.clone(), accumulate=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
