@@ -412,7 +412,7 @@ void svae_plan_destroy(void* plan);
  *   svae_lookup_fwd       out[r][0..D) = scale * table[tokens[r]][0..D), a zero row for a padded place
  *   svae_token_sort       stable sort of the places by token: keys [R] ascending (padded places and the token `pad` as V,
  *                         at the end; pad < 0: none), perm [R] the places; work: svae_token_sort_bytes(R, V, &bytes)
- *   svae_lookup_bwd       grad[v][0..D) = scale * sum of dy[perm[i]] over the places i with keys[i] == v, in their order; rows
+ *   svae_lookup_bwd       grad[v][0..D) = scale * sum of dy[perm[i]] over the places i with keys[i] == v, in a fixed order; rows
  *                         without a place are written as zeros.  accumulate != 0: the sums are added to grad, other rows are
  *                         left as they are.  work: svae_lookup_bwd_bytes(R, D, &bytes)
  * Sums are fp32, rounded once to grad's type; no atomics on them: the same bits in every run. */
@@ -428,11 +428,13 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
 
 /* ---- softmax cross entropy behind a linear layer over a large vocabulary --------------------------------------
  * No counterpart in the reference (its loss over the catalogue is svae_proj_nll_*: width 150, next-k targets).
- * z = hidden weight^T + bias, [R][V], never kept.  hidden [R][D], weight [V][D] (rows ld elements apart), bias [V] or NULL, all
+ * z = hidden weight^T + bias, [R][V], is not kept (few rows: in the workspace of a gradient).  hidden [R][D], weight [V][D] (rows ld elements apart), bias [V] or NULL, all
  * of one type (0 fp32, 1 bf16, 2 fp16); targets [R] int32, or int64 with tok64 != 0; R at most 2^24, V 2^28, D 2^16, ld_w 2^20.  A row whose target is outside [0, V) is
  * left out: nll = lse = 0, no gradient, whatever the row holds.  Products of bf16 / fp16 run on the matrix units as they are,
  * fp32 ones as six products of bf16 parts (24 bits) or, for few rows, in fp32; sums, statistics and losses are fp32.  In the
- * gradient w (softmax - onehot) is rounded to a 16-bit type after a scale by the largest row weight (16 rows or fewer: not at all).
+ * gradient of 16-bit types w (softmax - onehot) is rounded to that type after a scale by the largest row weight (fp16: in steps of 2^-38
+ * of that weight at the least; 16 rows or fewer: not at all), and softmax = exp(z - lse) is off by 2^-24 |lse|.  Low numbers of any
+ * size in the bias mask entries as -inf does.
  *   svae_xent_fwd     lse[r] = log sum_v exp z[r][v], nll[r] = lse[r] - z[r][target] (fp32)
  *   svae_xent_reduce  out[0] = the sum of nll or (mean != 0) its mean over the rows with a target (0 over none), out[1] = the
  *                     weight of a row in it
@@ -441,10 +443,13 @@ int svae_lookup_bwd(const void* dy, int dy_type, long long ld_dy, const int* key
  *                     takes no part, whatever it holds.
  *   svae_xent_fwd_bwd both in one call, for programs that know the rows' weights beforehand (copies of the inputs are made once)
  * Workspace, aligned to 256 bytes: svae_xent_bytes(address of weight modulo 16, ld_w, type, R, V, D, grad, &bytes), grad != 0 for
- * the gradients.  Up to 32 rows (64 of fp32, or against a weight of 2^23 numbers) read weight as it lies; their gradients have 4
- * bytes for each of the R x V logits in the workspace.  The loss of up to 512 rows of a 16-bit type takes weight as it lies too if
- * its address and rows are multiples of 16 bytes.  Else the workspace holds a copy of weight (16-bit types: of its size, fp32: one
- * and a half times that), and gradients have two pieces of up to 512 MiB, or of 256 columns if those are larger, in it. */
+ * the gradients.  It holds, with R rounded up to 128, V to 256 and D to 32:
+ *   up to 32 rows (64 of fp32, or against a weight of 2^23 numbers), which read weight as it lies: statistics, 8 bytes for a row and
+ *     256 entries of the vocabulary, and a copy of hidden; for gradients the logits, 4 bytes each, and up to 33 MiB of parts of dh;
+ *   more rows: hidden, 2 bytes a number (fp32: 6), for gradients twice; weight, as many bytes a number, but not for the loss of up to
+ *     512 rows of a 16-bit type whose weight's address and rows are multiples of 16 bytes; the statistics, 512 MiB at most; for
+ *     gradients in their place two pieces of w (softmax - onehot), each of up to 512 MiB or 256 entries of the vocabulary if those
+ *     are larger; sums of dh, 4 bytes a number or 128 MiB of parts; and up to 2 x 129 MiB of parts of dw and db. */
 int svae_xent_bytes(int weight_align, long long ld_w, int type, int R, int V, int D, int grad, long long* bytes);
 int svae_xent_fwd(const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                   const void* targets, int tok64, int type, int R, int V, int D, float* nll, float* lse, void* work,

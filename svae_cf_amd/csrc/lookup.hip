@@ -1,7 +1,8 @@
 // Embedding lookup with scaling for tables of any width and type, and its gradient by sorted tokens.
 //
 //   y[r][:]  = scale * table[t_r][:]                      (t_r outside [0, V): a padded place, zero row)
-//   dT[v][:] = scale * sum over { r : t_r = v } of dy[r][:], added in the order of r
+//   dT[v][:] = scale * sum over { r : t_r = v } of dy[r][:], added in an order that is the same in every run (that of r up to 64 rows;
+//              of more, sums of chunks and of every fourth row in them)
 //
 // Both are bound by HBM: the lookup reads a table row and writes an output row per token, the gradient reads every dy row
 // once and writes every table row once (rows without a token as zeros).  The gradient uses no atomics on sums: a stable radix

@@ -5,11 +5,15 @@
 //
 // Loss: one product over all tiles of z; each tile leaves the maximum and the sum of exponentials of its 256 columns per row and
 // the target's logit.  Gradient: for one piece of the vocabulary after the other, the tiles of z are made again and G of the
-// piece is written to the workspace, then two products take it up.  Everything is bound by the matrix units (6 R V D flops for
-// loss and gradient and 2 R V D for making z again), except that few rows leave the loss bound by reading W.
-// Loss and gradients, bf16: 8192 x 131072 x 1024 7.0 ms (8.8e12 operations, 1.26e15 a second; a library's products of these
-// shapes alone 1.10 .. 1.24e15), 21800 x 20000 x 200 1.0 ms; fp32 2049 x 17770 x 150 0.34 ms.  Loss alone, fp16: 256 x 1000000 x 256
-// 0.2 ms.
+// piece is written to the workspace, then two products take it up.
+// Bound by, and measured (the same commit is up to 7 % apart on different cards):
+//   wide rows, many of them: the matrix units, 6 R V D flops for loss and gradient and 2 R V D for making z again.  8192 x 131072 x 1024
+//     bf16 7.2 ms, 1.22e15 a second of these 8.8e12 (a library's products of these shapes alone 1.10 .. 1.24e15).
+//   many rows, width up to 256: G, which is written once and read twice.  21800 x 20000 x 200 bf16 1.03 ms; the launches of its
+//     gradients move 4.4 TB/s with the matrix units busy a third of the time.  fp32 has three parts of G: 2049 x 17770 x 150 0.345 ms,
+//     where its six bf16 products take 0.19.
+//   65 to some hundred rows against a large W: its copy in blocks, written once and read three times.  146 x 157269 x 1024 bf16 0.63 ms.
+//   loss alone, up to 512 rows of 16 bits: exponentials and pieces of 64 bytes of W's rows.  256 x 1000000 x 256 fp16 0.21 ms.
 //
 // All products run on one core: 256 x BN outputs a workgroup, steps of 32 along the contraction, three stages of LDS filled by
 // LDS-DMA (the stages are LDS variables of their own, so that the compiler can tell reads of one from writes to the other and
@@ -20,11 +24,15 @@
 //   z^T tile: A = W, B = H, both along the columns.  C has the row of H in the lane and four vocabulary entries in registers, so
 //     a row's maximum and sum are mostly in-lane work, and the eight values of G that a lane makes are two pieces of a block.
 //   G W: A = W over its rows, B = G along its columns.  G^T H: A = H, B = G, both over their rows.
-// Few rows and no gradient: W is read once, as it lies (16-bit types, aligned rows); that is bound by HBM.
+// Up to 512 rows of 16 bits and no gradient: W is read once, as it lies, if its address and rows are multiples of 16 bytes (PLAIN).
+// Up to 32 rows, or 64, with or without gradients: the kernels of xent_few.h, which take W as it lies at any address.
 //
 // Types: bf16 and fp16 go to the matrix units as they are; G is rounded to the inputs' type (relative 2^-8 / 2^-11 of each
-// term, as the inputs themselves are) after scaling by the largest row weight.  fp32 is carried as three bf16 parts (24 bits)
-// and every product by its six leading terms.  Few rows (xent_few.h) take other kernels.
+// term, as the inputs themselves are) after scaling by the largest row weight: the matrix units take 16-bit operands, and a second
+// part of G would make both products twice as long.  Relative error of bf16 gradients 0.0022 (0.0017 is the results' own rounding).
+// In fp16 steps of G end at 2^-38 of the largest weight: a row 2^20 lighter than it loses probabilities below 2^-19.  db is the sum of
+// the rounded G, so that it is the gradient that dW is.  fp32 is carried as three bf16 parts (24 bits) and every product by its six
+// leading terms.
 #include "elem.h"
 
 namespace {
@@ -783,7 +791,8 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict
     nll[r] = here ? l - zt[r] : 0.f;
 }
 
-// sum of the losses and number of rows with a target; in a fixed order, in 64 bits (a mean over no rows is 0)
+// sum of the losses and number of rows with a target; in a fixed order, in 64 bits (a mean over no rows is 0).  One workgroup: 21 800
+// rows 7 us, 131 072 31 us; of more its share of the loss and gradients is smaller (2^20 rows 0.6 ms, 2^24 9.5 ms: bound by latency)
 __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restrict__ nll, const void* __restrict__ tok, int tok64,
                                                            int R, int V, int mean, float* __restrict__ out) {
     __shared__ double red[1024];
@@ -818,8 +827,8 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float* __restri
 // Host side: shapes, workspace, launches
 // ------------------------------------------------------------------------------------------------
 // Up to here: the kernels for few rows.  More than 32 rows of 16 bits only for a W of 2^23 numbers or more, whose copy costs more than
-// those kernels' slower start (64 rows, loss and gradients in us, few | many: 5000 x 64 41 | 35, 32768 x 256 55 | 51, 32768 x 1024
-// 93 | 99, 65536 x 256 64 | 90; fp32 39 | 41, 83 | 114, 221 | 344, 113 | 285).
+// those kernels' slower start (64 rows, loss and gradients in us, few | many: 5000 x 64 41 | 35, 32768 x 256 (2^23: about even) 55 | 51,
+// 32768 x 1024 93 | 99, 65536 x 256 64 | 90; fp32 39 | 41, 83 | 114, 221 | 344, 113 | 285).
 constexpr int FEW_ROWS = 64, FEW_ROWS_16 = 32;
 constexpr long long FEW_WEIGHT_16 = 1ll << 23;
 // vocabulary tiles up to which logits of one tile of rows take H as it lies: without the launch for the copy, which however is

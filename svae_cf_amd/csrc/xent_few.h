@@ -13,8 +13,9 @@
 // reading W once takes 53 us (16 bits) or 106 us (fp32), writing its gradient as long.
 //
 // Measured there, loss | loss and gradients (us), against the kernels for many rows:
-//   fp32   1 row 133 | 358    (566 | 1285)     32 rows 144 | 411    (555 | 1320)     64 rows 235 | 754    (554 | 1333)
-//   bf16   1 row  48 | 203    ( 53 |  400)     32 rows  50 | 208    ( 52 |  397)     64 rows  55 | 239    ( 53 |  401)
+//   fp32   1 row 133 | 365    (566 | 1285)     32 rows 143 | 408    (555 | 1320)     64 rows 249 | 762    (554 | 1333)
+//   bf16   1 row  59 | 217    ( 53 |  400)     32 rows  58 | 207    ( 52 |  397)     64 rows  61 | 240    ( 53 |  401)
+// (inputs in rotation, so that W comes from memory; the same ones again and again: bf16 1 row 48 | 203.)
 // xent.hip has the limits.  The loss of 64 rows of 16 bits is the one that loses (a million x 256: 138 | 490 against 113 | 1065): loss
 // and gradients have to take the same kernels, as z has to have the same bits in both, or errors of z and of lse do not cancel in
 // the gradient of a confident row.
@@ -35,13 +36,8 @@ struct FewArgs {
     int tok64, V, D, Dp, R, R4, Rp, ndt, chunks;
 };
 
-// N numbers of any type from any address a number may have (the hardware's vector loads and stores need no more)
 template <typename T, int N>
-struct SomeOf {
-    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-};
-template <typename T, int N>
-using Some = typename SomeOf<T, N>::type;
+using Some = typename SvVec<T, N>::type;                               // from any address a number may have
 
 // the loss's copy of H and the rows' targets
 struct FewPrepArgs {

@@ -6,7 +6,8 @@ Conventions
   - tensors live on a GPU (there is no CPU fallback); work is enqueued on the current stream of the tensors' device, nothing
     synchronises, workspaces come from torch's allocator, so every call can be captured into a graph;
   - a token or target outside [0, vocabulary) marks a padded place: zero row, no loss, no gradient (the package pads with -1);
-  - sums, softmax statistics and losses are fp32; a result is rounded once, to its tensor's type;
+  - sums, softmax statistics and losses are fp32; a result is rounded once, to its tensor's type (the cross entropy's gradients of
+    more than 16 rows of bf16 or fp16 have w (softmax - onehot) in that type too, see ``linear_nll_grad``);
   - results are the same in every run (no floating-point atomics).
 
 ``embedding``, ``dropout`` and ``linear_cross_entropy`` take part in autograd (reverse mode, once; tensors with forward-mode
@@ -170,7 +171,7 @@ def embedding(table, tokens, scale=1.0, padding_idx=None, out_dtype=None):
 def embedding_grad(dout, tokens, num_rows, scale=1.0, padding_idx=None, dtype=None, out=None, accumulate=False):
     """Gradient of ``embedding`` for the table: ``[num_rows, D]`` in ``dtype`` (default: dout's), every row written.
 
-    Tokens are sorted on the device (stable, so equal tokens are added in their order).  ``out``: the tensor to write (rows may
+    Tokens are sorted on the device (stable; equal tokens are added in an order that is the same in every run).  ``out``: the tensor to write (rows may
     be strided); with ``accumulate`` the sums are added to what ``out`` holds, as for a table that another gradient shares."""
     _check(dout, "dout")
     _check(tokens, "tokens", _IDS, dout.get_device())
@@ -341,6 +342,8 @@ def _xent_grads(args, need):
 def linear_nll(hidden, weight, targets, bias=None):
     """(nll, lse) of ``softmax(hidden @ weight.T + bias)`` for the targets, fp32, shaped like targets; no logits are kept.
 
+    Entries of the vocabulary are masked by -inf or any low number in the bias (with -inf for all of them loss and gradients are
+    NaN, as the formula is).
     hidden [..., D], weight [V, D], bias [V] of one type; targets int32 / int64.  A row whose target is outside [0, V) is left
     out: both are 0.  For scoring, and for programs that run their own backward pass (``linear_nll_grad``)."""
     args = _xent_args(hidden, weight, targets, bias)
@@ -353,7 +356,12 @@ def linear_nll(hidden, weight, targets, bias=None):
 
 def linear_nll_grad(hidden, weight, targets, row_weight, bias=None):
     """(nll, lse, dhidden, dweight, dbias): ``linear_nll`` and the gradients of ``sum(row_weight * nll)`` in the inputs' type
-    (dbias None without a bias).  row_weight: fp32, shaped like targets; a row of weight 0 takes no part in the gradient."""
+    (dbias None without a bias).  row_weight: fp32, shaped like targets; a row of weight 0 takes no part in the gradient.
+
+    For bf16 and fp16, w (softmax - onehot) is rounded to that type in front of its products, but for 16 rows or fewer: off by half a
+    step of it, and in fp16 by 2^-39 of the largest weight at least, so that rows 2^20 lighter lose probabilities below 2^-19.
+    softmax is exp(logit - lse) with the lse that comes back, in fp32: off by 2^-24 |lse|.  Logits are not kept, but for few rows (up
+    to 32, or 64), whose R x V logits lie in the workspace of the call."""
     args = _xent_args(hidden, weight, targets, bias)
     _check(row_weight, "row_weight", _FLOAT, hidden.get_device())
     if row_weight.shape != targets.shape:
@@ -403,11 +411,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 
 def linear_cross_entropy(hidden, weight, targets, bias=None, reduction="mean"):
-    """Softmax cross entropy of the logits ``hidden @ weight.T + bias`` without ever keeping them, fp32.
+    """Softmax cross entropy of the logits ``hidden @ weight.T + bias``, fp32, without keeping them from forward to backward.
 
     hidden [..., D], weight [V, D], bias [V] of one type (fp32, bf16, fp16); targets int32 / int64, shaped ``hidden.shape[:-1]``;
     a target outside [0, V) leaves its row out.  reduction: "mean" over the rows with a target (0 if there are none), "sum" or
-    "none".  The backward pass makes the logits again in pieces of the vocabulary; gradients have the inputs' type."""
+    "none".  The backward pass makes the logits again, in pieces of the vocabulary (of few rows all of them, in its workspace);
+    gradients have the inputs' type, with the roundings that ``linear_nll_grad`` names."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be mean, sum or none, got %r" % (reduction,))
     for t, what in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):        # (gone inside the function)

@@ -58,3 +58,14 @@ def test_statistics_of_large_losses(R, V, D, kind):
     assert asked(kind, R, V, D, False) <= copies(kind, R, V, D, False) + rows_and_columns(R, V) + statistics
     sums = max(4 * up(R, 128) * up(D, 32), 128 * MIB) + 2 * 129 * MIB
     assert asked(kind, R, V, D, True) <= copies(kind, R, V, D, True) + rows_and_columns(R, V) + 8 * up(R, 128) + pieces(kind, R) + sums
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("R", [1, 16, 17, 32, 33, 64])
+def test_few_rows(R, kind):
+    """Statistics, a copy of hidden, the logits, 33 MiB of parts of dH; no copy of the weight."""
+    for V in (1, 1000, 70000, 1 << 24):
+        for D in (1, 64, 65, 260, 5000, 65536):
+            if kind == 0 or R <= 32 or V * D >= 1 << 23:
+                loss = 8 * up(R, 64) * -(-V // 256) + up(R, 64) * up(D, 64) * SIZE[kind] + 8 * 1024
+                assert asked(kind, R, V, D, False) <= loss and asked(kind, R, V, D, True) <= loss + 4 * V * up(R, 4) + 33 * MIB
